@@ -141,6 +141,19 @@ PA_API pa_status_t pa_decode_plan(const pa_decode_params* p, pa_decode_plan_info
  * kernel was queued, `out` and `lse` are undefined for that step. */
 PA_API pa_status_t pa_decode(const pa_decode_params* p, cudaStream_t stream);
 
+/* The same step under a sliding window: the query of a row of S tokens (at
+ * position S - 1) sees the row's last `window` tokens and its first `num_sinks`
+ * tokens. No other page is read: their block-table entries may be anything
+ * (pages given back to the pool hold -1). window >= 1, num_sinks >= 0, else
+ * PA_ERR_ARG; the split schedule (num_splits > 0, partial buffers) has no
+ * windowed form: PA_ERR_UNSUPPORTED. Workspace and counters as
+ * pa_window_decode_workspace reports. It has no counterpart in the reference. */
+PA_API pa_status_t pa_window_decode_workspace(const pa_decode_params* p, int32_t window,
+                                       int32_t num_sinks, size_t* workspace_bytes,
+                                       size_t* counter_count);
+PA_API pa_status_t pa_window_decode(const pa_decode_params* p, int32_t window, int32_t num_sinks,
+                             cudaStream_t stream);
+
 /* New tokens' K/V rows into the paged caches (the step before decode in a
  * serving loop; the reference fills its caches in test code,
  * tests/correctness.py:30-36). Row t of key/value ([num_tokens, num_kv_heads,

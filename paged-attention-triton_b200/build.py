@@ -26,8 +26,9 @@ EXT_SOURCE = os.path.join(HERE, "csrc", "torch_ext.cpp")
 EXT_OUTPUT = os.path.join(HERE, "paged_attention", "_pa_ext.so")
 BUILD_DIR = os.path.join(HERE, "_build")
 # pa_decode.cu compiles as parts in parallel: 0 = host API and small kernels,
-# 1-4 = decode-kernel instantiations (see the PA_PART blocks in the source).
-PARTS = (0, 1, 2, 3, 4)
+# 1-4 = decode-kernel instantiations, 5-8 = the same with a sliding window (see
+# the PA_PART blocks in the source).
+PARTS = (0, 1, 2, 3, 4, 5, 6, 7, 8)
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMPILE_FLAGS = ARCH_FLAGS + [

@@ -36,7 +36,8 @@
 
 // The library can be compiled as one translation unit, or as parts in
 // parallel (build.py): part 0 holds the host API and the small kernels, parts
-// 1-4 instantiate the decode kernels (explicit instantiations at the end).
+// 1-4 instantiate the decode kernels and parts 5-8 their windowed form
+// (explicit instantiations at the end).
 #if !defined(PA_PART) || PA_PART == 0
 #define PA_HOST_PART 1
 #else
@@ -134,6 +135,9 @@ struct KParams {
   // it; the CTAs' pieces meet in distributed shared memory (at byte offset
   // clu_off of every CTA's aligned shared memory) instead of through L2.
   int clu, clu_off;
+  // Sliding window (kWin kernels): the row's last `window` tokens and its first
+  // `sinks` tokens are visible.
+  int window, sinks;
 };
 // ----------------------------------------------------------------------------
 // PTX helpers
@@ -340,11 +344,58 @@ __device__ __forceinline__ int clamp_len(const KParams& p, int s, bool& bad) {
 }
 
 // Length of row b: the uniform length, or (kCum: per-row lengths) seq_lens[b].
-template <bool kCum>
+// The windowed kernels take both through the per-row schedule (seq_lens may be
+// null there).
+template <bool kCum, bool kWin = false>
 __device__ __forceinline__ int row_len(const KParams& p, int b) {
   if constexpr (!kCum) return p.seq_len;
+  if constexpr (kWin)
+    if (!p.seq_lens) return p.seq_len;
   bool bad = false;
   return clamp_len(p, __ldg(p.seq_lens + b), bad);
+}
+
+// Sliding window. The query of a row of S tokens sits at position S - 1 and
+// sees [0, a) and [w0, S): w0 = max(0, S - window), a = min(sinks, w0). The
+// row's tiles are those that hold a sink, then those from the window's first
+// token on, in one list: a row costs its visible tokens, whatever its length,
+// and the schedule, the merges and the page prefetch see shorter rows. A tile
+// that holds the last sink and the window's first token is listed twice, each
+// time with its own token range.
+struct WinRange {
+  int a, w0;          // sinks [0, a), window [w0, S)
+  int na, wt;         // sink tiles; first window tile
+};
+template <int TILE>
+__host__ __device__ __forceinline__ WinRange win_range(int window, int sinks, int S) {
+  WinRange w;
+  w.w0 = S > window ? S - window : 0;
+  w.a = sinks < w.w0 ? sinks : w.w0;
+  w.na = (w.a + TILE - 1) / TILE;
+  w.wt = w.w0 / TILE;
+  return w;
+}
+// Tiles of a row of S tokens.
+template <int TILE, bool kWin>
+__device__ __forceinline__ int row_tiles(const KParams& p, int S) {
+  const int all = (S + TILE - 1) / TILE;
+  if constexpr (!kWin) return all;
+  const WinRange w = win_range<TILE>(p.window, p.sinks, S);
+  return w.na + all - w.wt;
+}
+// Tile `i` of a row's list: its place in the sequence, and the token range
+// [t0, t1) that it serves.
+template <int TILE>
+__device__ __forceinline__ int win_tile(const KParams& p, int S, int i, int& t0, int& t1) {
+  const WinRange w = win_range<TILE>(p.window, p.sinks, S);
+  if (i < w.na) {
+    t0 = 0;
+    t1 = w.a;
+    return i;
+  }
+  t0 = w.w0;
+  t1 = S;
+  return w.wt + i - w.na;
 }
 
 // Largest b in [0, B) with cum[b] <= u (cum non-decreasing, cum[0] = 0).
@@ -376,14 +427,14 @@ struct Cursor {
   int seg_lo;         // unit index of the segment's tile 0 (balanced)
 };
 
-template <int TILE, bool kCum>
+template <int TILE, bool kCum, bool kWin>
 __device__ __forceinline__ void decode_unit(Cursor& c, const KParams& p, const int* cum, int u) {
   int row_base;
   if constexpr (kCum) {
     c.b = find_row(cum, p.B, u);
     row_base = cum[c.b];
-    c.S = row_len<true>(p, c.b);
-    c.nt = (c.S + TILE - 1) / TILE;
+    c.S = row_len<true, kWin>(p, c.b);
+    c.nt = row_tiles<TILE, kWin>(p, c.S);
   } else {
     c.S = p.seq_len;
     c.nt = p.nt_u;
@@ -399,7 +450,7 @@ __device__ __forceinline__ void decode_unit(Cursor& c, const KParams& p, const i
 }
 
 // Next unit in flattened order (balanced).
-template <int TILE, bool kCum>
+template <int TILE, bool kCum, bool kWin>
 __device__ __forceinline__ void cursor_next(Cursor& c, const KParams& p) {
   if (++c.tile < c.nt) return;
   c.tile = 0;
@@ -411,8 +462,8 @@ __device__ __forceinline__ void cursor_next(Cursor& c, const KParams& p) {
   do {   // next row that owns tiles (rows of length 0 own none)
     if (c.b + 1 >= p.B) { c.nt = 1; return; }   // past the end: never used
     ++c.b;
-    c.S = row_len<kCum>(p, c.b);
-    c.nt = (c.S + TILE - 1) / TILE;
+    c.S = row_len<kCum, kWin>(p, c.b);
+    c.nt = row_tiles<TILE, kWin>(p, c.S);
   } while (c.nt == 0);
 }
 
@@ -423,15 +474,19 @@ constexpr int kWarpSeg = 4;    // the warp's piece is the whole segment
 constexpr int kWarpGroup = 8;  // the warp's piece is the group's whole piece
 constexpr int kGroupSeg = 16;  // the group's piece is the whole segment
 
-template <int TILE>
-__device__ __forceinline__ void piece_of(const Cursor& c, const Ranges& rg, int& t0, int& t1,
-                                         int& flags) {
+// (kWin: [t0, t1) is the tile's own token range instead of the piece's; `tile`
+// is the tile's place in the sequence.)
+template <int TILE, bool kWin>
+__device__ __forceinline__ void piece_of(const KParams& p, const Cursor& c, const Ranges& rg,
+                                         int& tile, int& t0, int& t1, int& flags) {
   const int u = c.seg_lo + c.tile;
   const int seg_hi = c.seg_lo + c.nt;
   const int plo = max(c.seg_lo, rg.wr0), phi = min(seg_hi, rg.wr1);
   const int glo = max(c.seg_lo, rg.gr0), ghi = min(seg_hi, rg.gr1);
   t0 = (plo - c.seg_lo) * TILE;
   t1 = min(c.S, (phi - c.seg_lo) * TILE);
+  tile = c.tile;
+  if constexpr (kWin) tile = win_tile<TILE>(p, c.S, c.tile, t0, t1);
   flags = (u == plo ? kFirst : 0) | (u == phi - 1 ? kLast : 0) |
           ((plo == c.seg_lo && phi == seg_hi) ? kWarpSeg : 0) |
           ((plo == glo && phi == ghi) ? kWarpGroup : 0) |
@@ -470,7 +525,7 @@ __device__ __forceinline__ void flag(const KParams& p, unsigned bits) {
 // serves box (L & (spt-1)) of tile (L >> lspt) of the batch [u0, u1) (units of
 // the warp range, or tile ordinals of a split). INT_MIN: the box holds no token
 // of its piece (not loaded; the consumer masks it). One load per lane.
-template <int TILE, bool kSplit, bool kCum>
+template <int TILE, bool kSplit, bool kCum, bool kWin>
 __device__ __forceinline__ void batch_pages(const KParams& p, const int* cum, const Ranges& rg,
                                             const Work& w, int u0, int u1, int lane, int& phys,
                                             int& slot) {
@@ -482,10 +537,9 @@ __device__ __forceinline__ void batch_pages(const KParams& p, const int* cum, co
     int tile, b, t0, t1;
     if constexpr (!kSplit) {
       Cursor c;
-      decode_unit<TILE, kCum>(c, p, cum, u0 + ord);
+      decode_unit<TILE, kCum, kWin>(c, p, cum, u0 + ord);
       int fl;
-      piece_of<TILE>(c, rg, t0, t1, fl);
-      tile = c.tile;
+      piece_of<TILE, kWin>(p, c, rg, tile, t0, t1, fl);
       b = c.b;
     } else {
       tile = w.tl0 + u0 + ord;
@@ -905,7 +959,7 @@ __device__ __noinline__ void zero_length_rows(int B, int Hq, char* out, long lon
 // Kernel
 // ----------------------------------------------------------------------------
 template <typename T, bool kDup, int TILE, int NW, int NS, int D, bool kSplit, bool kCum,
-          bool kClu>
+          bool kClu, bool kWin>
 __global__ void __launch_bounds__(NW * 32, 1)
     pa_decode_kernel(const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const KParams p) {
@@ -1015,8 +1069,8 @@ __global__ void __launch_bounds__(NW * 32, 1)
     bool bad = false;
     int local = 0;
     for (int b = lo; b < hi; ++b) {
-      const int S = clamp_len(p, __ldg(p.seq_lens + b), bad);
-      local += nseg * ((S + TILE - 1) / TILE);
+      const int S = (kWin && !p.seq_lens) ? p.seq_len : clamp_len(p, __ldg(p.seq_lens + b), bad);
+      local += nseg * row_tiles<TILE, kWin>(p, S);
     }
     if (bad && blockIdx.x == 0) flag(p, PA_STATUS_BAD_SEQLEN);
     int incl = local;
@@ -1032,8 +1086,8 @@ __global__ void __launch_bounds__(NW * 32, 1)
     int run = before + incl - local;
     for (int b = lo; b < hi; ++b) {
       cum[b] = run;
-      const int S = clamp_len(p, __ldg(p.seq_lens + b), bad);
-      run += nseg * ((S + TILE - 1) / TILE);
+      const int S = (kWin && !p.seq_lens) ? p.seq_len : clamp_len(p, __ldg(p.seq_lens + b), bad);
+      run += nseg * row_tiles<TILE, kWin>(p, S);
     }
     if (threadIdx.x == blockDim.x - 1) cum[B] = before + incl;
     __syncthreads();
@@ -1125,23 +1179,24 @@ __global__ void __launch_bounds__(NW * 32, 1)
   int u0c = range0, u1c = min(range1, range0 + bt_tiles);
   int u0n = u1c, u1n = min(range1, u1c + bt_tiles);
   int pg_c = INT_MIN, sl_c = 0, pg_n = INT_MIN, sl_n = 0;
-  if (u0c < u1c) batch_pages<TILE, kSplit, kCum>(p, cum, rg, w, u0c, u1c, lane, pg_c, sl_c);
+  if (u0c < u1c) batch_pages<TILE, kSplit, kCum, kWin>(p, cum, rg, w, u0c, u1c, lane, pg_c, sl_c);
   Cursor ic;
   ic.b = w.b;
   ic.kvh = w.kvh;
   ic.qc = w.qc;
   ic.tile = w.tl0;
   ic.nt = ic.S = ic.seg_lo = 0;
-  if (!kSplit && n_tiles > 0) decode_unit<TILE, kCum>(ic, p, cum, range0);
+  if (!kSplit && n_tiles > 0) decode_unit<TILE, kCum, kWin>(ic, p, cum, range0);
   int ord = 0;          // tile ordinal within the current batch
   int issued = 0;
 
   auto issue = [&](int st) {
-    int t0, t1, fl;
+    int tile, t0, t1, fl;
     if (!kSplit) {
-      piece_of<TILE>(ic, rg, t0, t1, fl);
+      piece_of<TILE, kWin>(p, ic, rg, tile, t0, t1, fl);
     } else {
       const int k = u0c + ord;
+      tile = ic.tile;
       t0 = w.t0;
       t1 = w.t1;
       fl = (k == 0 ? kFirst : 0) | (k == w.n - 1 ? kLast : 0);
@@ -1161,7 +1216,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
     const bool first = fl & kFirst;
     if (lane == 0) {
       int* d = desc0 + st * kDescInts;
-      reinterpret_cast<int4*>(d)[0] = make_int4(ic.b, ic.kvh, ic.qc, ic.tile * TILE);
+      reinterpret_cast<int4*>(d)[0] = make_int4(ic.b, ic.kvh, ic.qc, tile * TILE);
       reinterpret_cast<int4*>(d)[1] = make_int4(t0, t1, ic.seg_lo, ic.seg_lo + ic.nt);
       reinterpret_cast<int4*>(d)[2] = make_int4(fl, gc, 0, 0);
       // per box: K and V, D/64 chunks of R rows x 128 B each; plus the query rows
@@ -1180,7 +1235,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
     }
     ++issued;
     // advance to the next tile
-    if (!kSplit) cursor_next<TILE, kCum>(ic, p); else ++ic.tile;
+    if (!kSplit) cursor_next<TILE, kCum, kWin>(ic, p); else ++ic.tile;
     if (u0c + ++ord < u1c) return;
     u0c = u0n;
     u1c = u1n;
@@ -1189,7 +1244,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
     ord = 0;
     u0n = u1c;
     u1n = min(range1, u1c + bt_tiles);
-    if (u0n < u1n) batch_pages<TILE, kSplit, kCum>(p, cum, rg, w, u0n, u1n, lane, pg_n, sl_n);
+    if (u0n < u1n) batch_pages<TILE, kSplit, kCum, kWin>(p, cum, rg, w, u0n, u1n, lane, pg_n, sl_n);
   };
 
   for (int s = 0; s < NS && issued < n_tiles; ++s) issue(s);
@@ -1197,7 +1252,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
   // batch holds at least 8 tiles (32 boxes of >= 8 rows), more than the NS
   // issued above, so those never reached it (a range that ended inside the
   // first batch has no second one).
-  if (u0n < u1n) batch_pages<TILE, kSplit, kCum>(p, cum, rg, w, u0n, u1n, lane, pg_n, sl_n);
+  if (u0n < u1n) batch_pages<TILE, kSplit, kCum, kWin>(p, cum, rg, w, u0n, u1n, lane, pg_n, sl_n);
   if (!kSplit) __syncthreads();   // gcnt is zero for every warp's merges
   if constexpr (kClu) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   // The next kernel in the stream may start its own prologue on SMs this grid
@@ -1675,11 +1730,26 @@ struct MergeParams {
   int tile;                 // tokens per unit
   int ngroups, gsz;
   int U, P, nt_u, per_row;  // same-length rows; P: units per group
+  int window, sinks, seq_len;   // sliding window (kWin); seq_len when seq_lens is null
   int by_segment;           // 1: block x is a segment, 0: block x + 1 is a group boundary
   int col_split;            // 1: block y is one query column (segments of many pieces)
 };
 
-template <typename T, int D, bool kCum>
+// Units of a row in the merge pass (kWin: the windowed decode kernel's count).
+template <bool kWin>
+__device__ __forceinline__ int merge_row_tiles(const MergeParams& m, int b) {
+  int S = 0;
+  if (kWin && !m.seq_lens)
+    S = m.seq_len;
+  else
+    S = min(max(__ldg(m.seq_lens + b), 0), m.cap);
+  const int all = (S + m.tile - 1) / m.tile;
+  if constexpr (!kWin) return all;
+  const int w0 = max(0, S - m.window);
+  return (min(m.sinks, w0) + m.tile - 1) / m.tile + all - w0 / m.tile;
+}
+
+template <typename T, int D, bool kCum, bool kWin>
 __global__ void __launch_bounds__(256) merge_segments_kernel(const MergeParams m) {
   constexpr int N = HD<D>::kLaneF;
   constexpr int kRows = 64 / N;   // pieces in flight per lane
@@ -1702,10 +1772,7 @@ __global__ void __launch_bounds__(256) merge_segments_kernel(const MergeParams m
     const int lo = min(m.B, static_cast<int>(threadIdx.x) * chunk);
     const int hi = min(m.B, lo + chunk);
     int local = 0;
-    for (int b = lo; b < hi; ++b) {
-      const int S = min(max(__ldg(m.seq_lens + b), 0), m.cap);
-      local += nseg * ((S + m.tile - 1) / m.tile);
-    }
+    for (int b = lo; b < hi; ++b) local += nseg * merge_row_tiles<kWin>(m, b);
     int incl = local;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -1718,8 +1785,7 @@ __global__ void __launch_bounds__(256) merge_segments_kernel(const MergeParams m
     for (int k = 0; k < warp; ++k) run += s_tot[k];
     for (int b = lo; b < hi; ++b) {
       s_cum[b] = run;
-      const int S = min(max(__ldg(m.seq_lens + b), 0), m.cap);
-      run += nseg * ((S + m.tile - 1) / m.tile);
+      run += nseg * merge_row_tiles<kWin>(m, b);
     }
     if (threadIdx.x == 255) s_cum[m.B] = run;
     __syncthreads();
@@ -1733,8 +1799,7 @@ __global__ void __launch_bounds__(256) merge_segments_kernel(const MergeParams m
     b = blockIdx.x / nseg;
     seg = blockIdx.x - b * nseg;
     if constexpr (kCum) {
-      const int S = min(max(__ldg(m.seq_lens + b), 0), m.cap);
-      nt = (S + m.tile - 1) / m.tile;
+      nt = merge_row_tiles<kWin>(m, b);
       seg_lo = s_cum[b] + seg * nt;
     } else {
       nt = m.nt_u;
@@ -1749,8 +1814,7 @@ __global__ void __launch_bounds__(256) merge_segments_kernel(const MergeParams m
     if constexpr (kCum) {
       b = find_row(s_cum, m.B, u);
       row_base = s_cum[b];
-      const int S = min(max(__ldg(m.seq_lens + b), 0), m.cap);
-      nt = (S + m.tile - 1) / m.tile;
+      nt = merge_row_tiles<kWin>(m, b);
     } else {
       b = u / m.per_row;
       row_base = b * m.per_row;
@@ -1940,6 +2004,7 @@ struct GenParams {
   const int* seq_lens;
   int seq_len;
   int B, Hq, G, bs, NB, ns;
+  int window, sinks;                        // sliding window (kWin)
   float scale_log2;
   float* o_part;
   float* lse_part;
@@ -1985,7 +2050,9 @@ __device__ __forceinline__ void load_halfs(const char* p, float (&f)[N]) {
   for (int i = 0; i < N; ++i) f[i] = half_bits_to_float<T>(h[i]);
 }
 
-template <typename T, int D>
+// kWin: the splits divide the row's visible tokens, numbered 0 .. n - 1: the
+// sinks [0, a), then the window [w0, S).
+template <typename T, int D, bool kWin>
 __global__ void __launch_bounds__(128) generic_split_kernel(const GenParams g) {
   constexpr int N = D / 32;   // dimensions per lane in the PV product
   __shared__ float qs[4][D];
@@ -2006,6 +2073,13 @@ __global__ void __launch_bounds__(128) generic_split_kernel(const GenParams g) {
     if ((raw < 0 || raw > cap) && lane == 0 && s == 0 && hq == 0 && g.status)
       atomicOr(g.status, PA_STATUS_BAD_SEQLEN);
   }
+  int jump_at = 0, jump = 0;                 // visible token v >= jump_at is token v + jump
+  if constexpr (kWin) {
+    const WinRange w = win_range<32>(g.window, g.sinks, S);
+    jump_at = w.a;
+    jump = w.w0 - w.a;
+    S -= jump;
+  }
   const int ss = (S + g.ns - 1) / g.ns;      // torch_kernel.py:30
   const int t0 = s * ss;
   const int t1 = min(t0 + ss, S);
@@ -2022,9 +2096,10 @@ __global__ void __launch_bounds__(128) generic_split_kernel(const GenParams g) {
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
   for (int c = t0; c < t1; c += 32) {
-    const int t = c + lane;
+    int t = c + lane;
     int page = -1, slot = 0;
     if (t < t1) {                            // split_kv_kernel.py:52-58
+      if constexpr (kWin) t += t >= jump_at ? jump : 0;
       const int lb = t / g.bs;
       page = __ldg(g.bt + b * g.bt_sb + lb);
       slot = t - lb * g.bs;
@@ -2458,7 +2533,7 @@ static void plan_cluster(const pa_decode_params* p, int sms, Plan& pl) {
 }
 
 static pa_status_t make_plan(const pa_decode_params* p, int sms, Plan& pl,
-                             bool allow_cluster = true) {
+                             bool allow_cluster = true, bool windowed = false) {
   pl.G = p->num_heads / p->num_kv_heads;
   pl.QC = (pl.G + 7) / 8;
   pl.dup = (pl.G == 1 || pl.G == 2 || pl.G == 4);
@@ -2504,7 +2579,7 @@ static pa_status_t make_plan(const pa_decode_params* p, int sms, Plan& pl,
   if (pl.ns == 0) {
     pl.grid = sms;
     pl.W = pl.grid * v.nw;
-    pl.use_cum = p->seq_lens != nullptr;
+    pl.use_cum = p->seq_lens != nullptr || windowed;
     // Merge pieces inside a CTA through shared memory when the warps' rows fit.
     const int base = variant_smem_base(pl.variant, pl.dup, pl.D);
     // Groups are whole CTAs whose warps merge through shared memory when their
@@ -2635,7 +2710,7 @@ static bool cached_cache_map(CUtensorMap* map, const pa_decode_params* p, int de
 #endif  // PA_HOST_PART
 
 template <typename T, bool kDup, int TILE, int NW, int NS, int D, bool kSplit, bool kCum,
-          bool kClu>
+          bool kClu, bool kWin>
 cudaError_t launch_kernel(const Plan& pl, const CUtensorMap& mk, const CUtensorMap& mv,
                           const KParams& kp, cudaStream_t stream, int dev) {
   using C = Cfg<kDup, TILE, NW, NS, D>;
@@ -2645,7 +2720,7 @@ cudaError_t launch_kernel(const Plan& pl, const CUtensorMap& mk, const CUtensorM
   {
     std::lock_guard<std::mutex> lk(mu);
     if (!attr_set[dev]) {
-      const cudaError_t e = cudaFuncSetAttribute(pa_decode_kernel<T, kDup, TILE, NW, NS, D, kSplit, kCum, kClu>,
+      const cudaError_t e = cudaFuncSetAttribute(pa_decode_kernel<T, kDup, TILE, NW, NS, D, kSplit, kCum, kClu, kWin>,
                                                  cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                  kMaxSmem);
       if (e != cudaSuccess) return e;
@@ -2685,7 +2760,7 @@ cudaError_t launch_kernel(const Plan& pl, const CUtensorMap& mk, const CUtensorM
     if (ok < 0) {
       int n = 0;
       const cudaError_t q = cudaOccupancyMaxActiveClusters(
-          &n, pa_decode_kernel<T, kDup, TILE, NW, NS, D, kSplit, kCum, kClu>, &cfg);
+          &n, pa_decode_kernel<T, kDup, TILE, NW, NS, D, kSplit, kCum, kClu, kWin>, &cfg);
       ok = (q == cudaSuccess && n * pl.clu >= pl.grid) ? 1 : 0;
       if (q != cudaSuccess) (void)cudaGetLastError();
       std::lock_guard<std::mutex> lk(mu);
@@ -2693,19 +2768,31 @@ cudaError_t launch_kernel(const Plan& pl, const CUtensorMap& mk, const CUtensorM
     }
     if (!ok) return cudaErrorCooperativeLaunchTooLarge;   // the caller re-plans without clusters
   }
-  return cudaLaunchKernelEx(&cfg, pa_decode_kernel<T, kDup, TILE, NW, NS, D, kSplit, kCum, kClu>, mk, mv, kp);
+  return cudaLaunchKernelEx(&cfg, pa_decode_kernel<T, kDup, TILE, NW, NS, D, kSplit, kCum, kClu, kWin>, mk, mv, kp);
 }
 
 // Every decode kernel the dispatch below can launch, as (variant, layout) per
 // head_dim and dtype; PFX is `extern` for declarations, empty for definitions.
-#define PA_LK(T, DUP, TILE, NW, NS, D, SPLIT, CUM, CLU)                                     \
-  cudaError_t launch_kernel<T, DUP, TILE, NW, NS, D, SPLIT, CUM, CLU>(                      \
+// PA_BOTH: the full-length schedules; parts 5-8 define PA_WIN_PART and get the
+// windowed kernels from the same lists.
+#define PA_LK(T, DUP, TILE, NW, NS, D, SPLIT, CUM, CLU, WIN)                                \
+  cudaError_t launch_kernel<T, DUP, TILE, NW, NS, D, SPLIT, CUM, CLU, WIN>(                 \
       const Plan&, const CUtensorMap&, const CUtensorMap&, const KParams&, cudaStream_t, int)
-#define PA_BOTH(PFX, T, DUP, TILE, NW, NS, D)                        \
-  PFX template PA_LK(T, DUP, TILE, NW, NS, D, false, false, false);  \
-  PFX template PA_LK(T, DUP, TILE, NW, NS, D, false, false, true);   \
-  PFX template PA_LK(T, DUP, TILE, NW, NS, D, false, true, false);   \
-  PFX template PA_LK(T, DUP, TILE, NW, NS, D, true, false, false);
+#define PA_FULL(PFX, T, DUP, TILE, NW, NS, D)                               \
+  PFX template PA_LK(T, DUP, TILE, NW, NS, D, false, false, false, false);  \
+  PFX template PA_LK(T, DUP, TILE, NW, NS, D, false, false, true, false);   \
+  PFX template PA_LK(T, DUP, TILE, NW, NS, D, false, true, false, false);   \
+  PFX template PA_LK(T, DUP, TILE, NW, NS, D, true, false, false, false);
+#define PA_WIN(PFX, T, DUP, TILE, NW, NS, D) \
+  PFX template PA_LK(T, DUP, TILE, NW, NS, D, false, true, false, true);
+#if !defined(PA_PART) || PA_PART == 0
+#define PA_BOTH(PFX, T, DUP, TILE, NW, NS, D) \
+  PA_FULL(PFX, T, DUP, TILE, NW, NS, D) PA_WIN(PFX, T, DUP, TILE, NW, NS, D)
+#elif PA_PART >= 5
+#define PA_BOTH PA_WIN
+#else
+#define PA_BOTH PA_FULL
+#endif
 #define PA_D128(PFX, T)                                                              \
   PA_BOTH(PFX, T, true, 32, 4, 3, 128) PA_BOTH(PFX, T, false, 32, 4, 3, 128)         \
   PA_BOTH(PFX, T, true, 16, 8, 3, 128)                                               \
@@ -2724,7 +2811,7 @@ cudaError_t launch_kernel(const Plan& pl, const CUtensorMap& mk, const CUtensorM
 
 #if PA_HOST_PART
 #if defined(PA_PART)
-// Parts 1-4 hold the definitions.
+// Parts 1-8 hold the definitions.
 PA_D128(extern, __half)
 PA_D128(extern, __nv_bfloat16)
 PA_D64(extern, __half)
@@ -2740,13 +2827,15 @@ PA_D256(extern, __nv_bfloat16)
 template <typename T, bool kDup, int TILE, int NW, int NS, int D>
 static cudaError_t launch_one(const Plan& pl, const CUtensorMap& mk, const CUtensorMap& mv,
                               const KParams& kp, cudaStream_t stream, int dev) {
+  if (kp.window)
+    return launch_kernel<T, kDup, TILE, NW, NS, D, false, true, false, true>(pl, mk, mv, kp, stream, dev);
   if (pl.ns != 0)
-    return launch_kernel<T, kDup, TILE, NW, NS, D, true, false, false>(pl, mk, mv, kp, stream, dev);
+    return launch_kernel<T, kDup, TILE, NW, NS, D, true, false, false, false>(pl, mk, mv, kp, stream, dev);
   if (pl.use_cum)
-    return launch_kernel<T, kDup, TILE, NW, NS, D, false, true, false>(pl, mk, mv, kp, stream, dev);
+    return launch_kernel<T, kDup, TILE, NW, NS, D, false, true, false, false>(pl, mk, mv, kp, stream, dev);
   if (pl.clu)
-    return launch_kernel<T, kDup, TILE, NW, NS, D, false, false, true>(pl, mk, mv, kp, stream, dev);
-  return launch_kernel<T, kDup, TILE, NW, NS, D, false, false, false>(pl, mk, mv, kp, stream, dev);
+    return launch_kernel<T, kDup, TILE, NW, NS, D, false, false, true, false>(pl, mk, mv, kp, stream, dev);
+  return launch_kernel<T, kDup, TILE, NW, NS, D, false, false, false, false>(pl, mk, mv, kp, stream, dev);
 }
 
 template <typename T, bool kDup>
@@ -2781,7 +2870,7 @@ static cudaError_t launch(const Plan& pl, const CUtensorMap& mk, const CUtensorM
   return launch_one<T, kDup, 32, 4, 3, 128>(pl, mk, mv, kp, stream, dev);
 }
 
-template <typename T, int D, bool kCum>
+template <typename T, int D, bool kCum, bool kWin = false>
 static cudaError_t launch_merge_kernel(const MergeParams& m, dim3 grid, cudaStream_t stream) {
   // Dependent launch: the grid may be scheduled while the decode kernel runs;
   // griddepcontrol.wait orders its reads after that kernel's completion.
@@ -2795,12 +2884,17 @@ static cudaError_t launch_merge_kernel(const MergeParams& m, dim3 grid, cudaStre
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, merge_segments_kernel<T, D, kCum>, m);
+  return cudaLaunchKernelEx(&cfg, merge_segments_kernel<T, D, kCum, kWin>, m);
 }
 
 template <typename T>
 static cudaError_t launch_merge(const MergeParams& m, int D, bool cum, dim3 grid,
                                 cudaStream_t stream) {
+  if (m.window) {   // the windowed kernels run the per-row schedule
+    if (D == 64) return launch_merge_kernel<T, 64, true, true>(m, grid, stream);
+    if (D == 256) return launch_merge_kernel<T, 256, true, true>(m, grid, stream);
+    return launch_merge_kernel<T, 128, true, true>(m, grid, stream);
+  }
   if (D == 64)
     return cum ? launch_merge_kernel<T, 64, true>(m, grid, stream)
                : launch_merge_kernel<T, 64, false>(m, grid, stream);
@@ -2812,7 +2906,7 @@ static cudaError_t launch_merge(const MergeParams& m, int D, bool cum, dim3 grid
 }
 
 // The CUDA-core path: the split kernel, then the reduce kernel, on `stream`.
-static cudaError_t launch_generic(const pa_decode_params* p, const Plan& pl,
+static cudaError_t launch_generic(const pa_decode_params* p, const Plan& pl, int window, int sinks,
                                   cudaStream_t stream) {
   GenParams g;
   memset(&g, 0, sizeof(g));
@@ -2838,6 +2932,8 @@ static cudaError_t launch_generic(const pa_decode_params* p, const Plan& pl,
   g.bs = p->block_size;
   g.NB = p->num_blocks;
   g.ns = pl.ns;
+  g.window = window;
+  g.sinks = sinks;
   g.scale_log2 = p->scale * kLog2e;
   if (p->o_partial && p->lse_partial) {
     g.o_part = p->o_partial;
@@ -2858,10 +2954,16 @@ static cudaError_t launch_generic(const pa_decode_params* p, const Plan& pl,
 #define PA_GENERIC(DIM)                                                                  \
   if (pl.D == DIM) {                                                                     \
     if (bf) {                                                                            \
-      generic_split_kernel<__nv_bfloat16, DIM><<<grid_split, 128, 0, stream>>>(g);       \
+      if (window)                                                                        \
+        generic_split_kernel<__nv_bfloat16, DIM, true><<<grid_split, 128, 0, stream>>>(g); \
+      else                                                                               \
+        generic_split_kernel<__nv_bfloat16, DIM, false><<<grid_split, 128, 0, stream>>>(g); \
       generic_reduce_kernel<__nv_bfloat16, DIM><<<grid_reduce, 128, 0, stream>>>(g);     \
     } else {                                                                             \
-      generic_split_kernel<__half, DIM><<<grid_split, 128, 0, stream>>>(g);              \
+      if (window)                                                                        \
+        generic_split_kernel<__half, DIM, true><<<grid_split, 128, 0, stream>>>(g);      \
+      else                                                                               \
+        generic_split_kernel<__half, DIM, false><<<grid_split, 128, 0, stream>>>(g);     \
       generic_reduce_kernel<__half, DIM><<<grid_reduce, 128, 0, stream>>>(g);            \
     }                                                                                    \
     return cudaGetLastError();                                                           \
@@ -3092,24 +3194,39 @@ pa_status_t pa_decode_plan(const pa_decode_params* p, pa_decode_plan_info* info)
   return PA_OK;
 }
 
-pa_status_t pa_decode(const pa_decode_params* p, cudaStream_t stream) {
-  const pa_status_t v = validate_launch(p);
-  if (v != PA_OK) return v;
+}  // extern "C"
+
+namespace pa {
+
+// One decode step. Full length (window 0): `p` and `q` are the same. Windowed:
+// `q` is what the plan is made from (window_plan_params), `p` the caller's
+// parameters, whose real table width and lengths the kernel gets.
+static pa_status_t run_decode(const pa_decode_params* p, const pa_decode_params* q, int window,
+                              int sinks, cudaStream_t stream) {
   const int dev = current_device();
   const int sms = sm_count(dev);
   if (sms <= 0) return PA_ERR_LAUNCH;
   Plan pl;
-  pa_status_t s = make_plan(p, sms, pl);
+  pa_status_t s = make_plan(q, sms, pl, window == 0, window != 0);
   if (s != PA_OK) return s;
+  if (window && pl.ns != 0 && !pl.generic) return PA_ERR_UNSUPPORTED;   // units beyond int32
   if (p->batch == 0) return PA_OK;
   if (pl.counters > 0 && (pl.counters > p->counter_count || !p->counters)) return PA_ERR_WORKSPACE;
   if (pl.ws_bytes > p->workspace_bytes || (pl.ws_bytes && !p->workspace)) return PA_ERR_WORKSPACE;
   if (!aligned16(p->workspace)) return PA_ERR_ARG;
-  if (pl.generic) return launch_generic(p, pl, stream) == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
+  if (pl.generic)
+    return launch_generic(p, pl, window, sinks, stream) == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 
   KParams kp;
   const int tile = kVariants[pl.variant - 1].tile;
-  build_kparams(p, pl, kp);
+  build_kparams(q, pl, kp);
+  if (window) {
+    kp.max_blocks = p->max_blocks;
+    kp.seq_len = p->seq_lens ? 0 : p->seq_len;
+    kp.zero_rows = 1;
+    kp.window = window;
+    kp.sinks = sinks;
+  }
 
   CUtensorMap mk, mv;
   if (!cached_cache_map(&mk, p, dev, p->k_cache, p->k_stride_block, p->k_stride_slot,
@@ -3120,7 +3237,7 @@ pa_status_t pa_decode(const pa_decode_params* p, cudaStream_t stream) {
 
   dim3 merge_grid(1);
   int by_segment = 0, col_split = 0;
-  kp.post_merge = want_post_merge(p, pl, kp, merge_grid, by_segment, col_split) ? 1 : 0;
+  kp.post_merge = want_post_merge(q, pl, kp, merge_grid, by_segment, col_split) ? 1 : 0;
   // A snapped boundary moves by up to half the longest segment, which one CTA
   // then streams on top of its share: only worth it while that is about the
   // cost of the cross-CTA merge it saves (<= 64 KB of K+V, ~1.5 us of one
@@ -3167,6 +3284,9 @@ pa_status_t pa_decode(const pa_decode_params* p, cudaStream_t stream) {
     m.QC = kp.QC;
     m.slot_cols = kp.slot_cols;
     m.tile = tile;
+    m.window = window;
+    m.sinks = sinks;
+    m.seq_len = kp.seq_len;
     m.ngroups = pl.W / pl.gsz;
     m.gsz = pl.gsz;
     m.U = kp.U;
@@ -3179,6 +3299,97 @@ pa_status_t pa_decode(const pa_decode_params* p, cudaStream_t stream) {
                            : launch_merge<__nv_bfloat16>(m, pl.D, pl.use_cum, merge_grid, stream);
   }
   return e == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
+}
+
+// The checks of a windowed step beyond those of a full one.
+static pa_status_t validate_window(const pa_decode_params* p, int32_t window, int32_t num_sinks) {
+  if (!p || window <= 0 || num_sinks < 0) return PA_ERR_ARG;
+  if (p->num_splits != 0 || p->o_partial || p->lse_partial) return PA_ERR_UNSUPPORTED;
+  return PA_OK;
+}
+
+// Rows of one windowed launch: the per-row schedule's limit.
+static int window_rows(const pa_decode_params* p) {
+  return generic_shape(p) ? p->batch : std::min<int>(p->batch, kCumMax);
+}
+
+// What a windowed step of `rows` rows is planned from: the same step over
+// tables no longer than a row's tile list (sinks and window, each with a
+// partly used tile at its ends), so that the variant, merge group and
+// workspace rules see the tokens that are read, not those that are stored.
+static pa_decode_params window_plan_params(const pa_decode_params* p, int32_t window,
+                                           int32_t num_sinks, int rows) {
+  pa_decode_params q = *p;
+  const long long cap = static_cast<long long>(p->max_blocks) * p->block_size;
+  const long long seen =
+      std::min(cap, static_cast<long long>(window) + num_sinks) + (cap > 0 ? 3 * 64 : 0);
+  q.max_blocks = static_cast<int32_t>((seen + p->block_size - 1) / p->block_size);
+  q.seq_len = static_cast<int32_t>(std::min<long long>(p->seq_len, seen));
+  q.batch = rows;
+  return q;
+}
+
+}  // namespace pa
+
+extern "C" {
+
+pa_status_t pa_decode(const pa_decode_params* p, cudaStream_t stream) {
+  const pa_status_t v = validate_launch(p);
+  if (v != PA_OK) return v;
+  return run_decode(p, p, 0, 0, stream);
+}
+
+pa_status_t pa_window_decode_workspace(const pa_decode_params* p, int32_t window,
+                                       int32_t num_sinks, size_t* workspace_bytes,
+                                       size_t* counter_count) {
+  pa_status_t v = validate_window(p, window, num_sinks);
+  if (v != PA_OK) return v;
+  v = validate(p);
+  if (v != PA_OK) return v;
+  const int sms = sm_count(current_device());
+  if (sms <= 0) return PA_ERR_LAUNCH;
+  // The launches of a batch beyond the per-row schedule's limit share the
+  // workspace; the last, of fewer rows, may plan differently.
+  const int step = window_rows(p);
+  const int rows[2] = {step, step > 0 ? p->batch % step : 0};
+  size_t bytes = 0, counters = 0;
+  for (int i = 0; i < 2; ++i) {
+    if (i == 1 && rows[i] == 0) break;
+    const pa_decode_params q = window_plan_params(p, window, num_sinks, rows[i]);
+    Plan pl;
+    const pa_status_t s = make_plan(&q, sms, pl, false, true);
+    if (s != PA_OK) return s;
+    bytes = std::max(bytes, pl.ws_bytes);
+    counters = std::max(counters, pl.counters);
+  }
+  if (workspace_bytes) *workspace_bytes = bytes;
+  if (counter_count) *counter_count = counters;
+  return PA_OK;
+}
+
+pa_status_t pa_window_decode(const pa_decode_params* p, int32_t window, int32_t num_sinks,
+                             cudaStream_t stream) {
+  pa_status_t v = validate_window(p, window, num_sinks);
+  if (v != PA_OK) return v;
+  v = validate_launch(p);
+  if (v != PA_OK) return v;
+  // Batches beyond the per-row schedule's limit run as several launches over
+  // the same workspace, in stream order.
+  const int step = window_rows(p);
+  for (int b = 0; b == 0 || b < p->batch; b += step) {
+    pa_decode_params r = *p;
+    r.batch = std::min(step, p->batch - b);
+    r.q = static_cast<const char*>(p->q) + 2 * b * p->q_stride_b;
+    r.out = static_cast<char*>(p->out) + 2 * b * p->out_stride_b;
+    r.block_table = p->block_table + b * p->bt_stride_b;
+    if (p->seq_lens) r.seq_lens = p->seq_lens + b;
+    if (p->lse) r.lse = p->lse + static_cast<size_t>(b) * p->num_heads;
+    const pa_decode_params q = window_plan_params(&r, window, num_sinks, r.batch);
+    v = run_decode(&r, &q, window, num_sinks, stream);
+    if (v != PA_OK) return v;
+    if (step == 0) break;
+  }
+  return PA_OK;
 }
 
 }  // extern "C"
@@ -3326,6 +3537,16 @@ PA_D128(, __nv_bfloat16)
 PA_D64(, __half)
 PA_D64(, __nv_bfloat16)
 #elif PA_PART == 4
+PA_D256(, __half)
+PA_D256(, __nv_bfloat16)
+#elif PA_PART == 5
+PA_D128(, __half)
+#elif PA_PART == 6
+PA_D128(, __nv_bfloat16)
+#elif PA_PART == 7
+PA_D64(, __half)
+PA_D64(, __nv_bfloat16)
+#elif PA_PART == 8
 PA_D256(, __half)
 PA_D256(, __nv_bfloat16)
 #endif

@@ -38,7 +38,8 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> decode(
     const c10::optional<at::Tensor>& seq_lens, int64_t seq_len, int64_t block_size,
     int64_t num_splits, double scale, bool return_lse, bool return_partials,
     const at::Tensor& ws_buffer, const at::Tensor& ws_counters, const at::Tensor& ws_status,
-    int64_t kernel_variant, const c10::optional<at::Tensor>& out_opt) {
+    int64_t kernel_variant, const c10::optional<at::Tensor>& out_opt, int64_t window,
+    int64_t num_sinks) {
   check(q.is_cuda() && k.is_cuda() && v.is_cuda() && bt.is_cuda(),
         "Q, K_Cache, V_Cache and Block_Table must be CUDA tensors");
   check(q.dim() == 3, "Q must be [B, H, D]");
@@ -79,6 +80,12 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> decode(
     check(seq_len >= 0 && seq_len <= max_blocks * bs, "seq_len exceeds the Block_Table capacity");
   }
   check(num_splits >= 0, "num_splits must be >= 0");
+  // window 0: every cached token is visible
+  check(window >= 0 && window <= INT32_MAX && num_sinks >= 0 && num_sinks <= INT32_MAX,
+        "window must be at least 1 and num_sinks at least 0");
+  check(window > 0 || num_sinks == 0, "num_sinks goes with a window");
+  check(window == 0 || (num_splits == 0 && !return_partials),
+        "a window goes with the default schedule (no num_splits, no return_partials)");
   int64_t ns = num_splits;
   if (return_partials && ns == 0) {
     const int64_t s = seq_lens.has_value() ? max_blocks * bs : seq_len;
@@ -134,7 +141,9 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> decode(
   p.kernel_variant = static_cast<int32_t>(kernel_variant);
 
   size_t ws_bytes = 0, n_counters = 0;
-  pa_status_t rc = pa_decode_workspace(&p, &ws_bytes, &n_counters);
+  const auto win = static_cast<int32_t>(window), sinks = static_cast<int32_t>(num_sinks);
+  pa_status_t rc = window ? pa_window_decode_workspace(&p, win, sinks, &ws_bytes, &n_counters)
+                          : pa_decode_workspace(&p, &ws_bytes, &n_counters);
   TORCH_CHECK(rc == PA_OK, "pa_decode_workspace failed: ", pa_status_string(rc));
   if (ws_bytes > static_cast<size_t>(ws_buffer.numel()) ||
       n_counters > static_cast<size_t>(ws_counters.numel())) {
@@ -146,7 +155,8 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> decode(
   p.counter_count = static_cast<size_t>(ws_counters.numel());
   p.status = reinterpret_cast<uint32_t*>(ws_status.data_ptr<int32_t>());
 
-  rc = pa_decode(&p, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  const cudaStream_t stream = c10::cuda::getCurrentCUDAStream(dev.index()).stream();
+  rc = window ? pa_window_decode(&p, win, sinks, stream) : pa_decode(&p, stream);
   TORCH_CHECK(rc == PA_OK, "pa_decode failed: ", pa_status_string(rc));
 
   std::vector<at::Tensor> res{out};

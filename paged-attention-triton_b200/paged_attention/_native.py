@@ -132,6 +132,12 @@ _SIGNATURES = {
     "pa_decode_plan": (ctypes.c_int, [ctypes.POINTER(DecodeParams), ctypes.POINTER(PlanInfo)]),
     "pa_decode": (ctypes.c_int, [ctypes.POINTER(DecodeParams), ctypes.c_void_p]),
     "pa_decode_noalloc": (ctypes.c_int, [ctypes.POINTER(DecodeParams), ctypes.c_void_p]),
+    "pa_window_decode_workspace": (ctypes.c_int, [ctypes.POINTER(DecodeParams), ctypes.c_int32,
+                                                  ctypes.c_int32,
+                                                  ctypes.POINTER(ctypes.c_size_t),
+                                                  ctypes.POINTER(ctypes.c_size_t)]),
+    "pa_window_decode": (ctypes.c_int, [ctypes.POINTER(DecodeParams), ctypes.c_int32,
+                                        ctypes.c_int32, ctypes.c_void_p]),
     "pa_cache_append": (ctypes.c_int, [ctypes.POINTER(AppendParams), ctypes.c_void_p]),
     "pa_num_splits_heuristic": (ctypes.c_int32, [ctypes.c_int32] * 5),
     "pa_selftest_wait_timeout": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p,

@@ -14,7 +14,8 @@ zero at the end of every replay, so nothing needs re-initialising.
 Extensions (keyword-only): ``num_kv_heads`` (GQA caches), ``dynamic_seq_lens``
 (a static int32 ``[B]`` length buffer, so one graph serves any lengths up to
 ``max_seq_len``; the reference bakes its scalar ``seq_len`` into the graph),
-``num_splits``, ``scale`` and ``return_lse``.
+``num_splits``, ``scale``, ``return_lse``, and ``window`` with ``num_sinks`` (a
+sliding window, fixed in the graph).
 """
 from __future__ import annotations
 
@@ -30,7 +31,7 @@ class PagedAttnGraphRunner:
                  dtype=torch.float16, *, num_kv_heads: Optional[int] = None,
                  dynamic_seq_lens: bool = False, max_seq_len: Optional[int] = None,
                  num_splits: Optional[int] = None, scale: Optional[float] = None,
-                 return_lse: bool = False):
+                 return_lse: bool = False, window: Optional[int] = None, num_sinks: int = 0):
         self.seq_len = seq_len
         self.block_size = block_size
         kv_heads = H if num_kv_heads is None else num_kv_heads
@@ -59,7 +60,8 @@ class PagedAttnGraphRunner:
         def call():
             return paged_attention(self.static_q, self.static_k, self.static_v, self.static_bt,
                                    lengths, block_size, num_splits, scale=scale,
-                                   return_lse=return_lse, workspace=self.workspace)
+                                   return_lse=return_lse, workspace=self.workspace,
+                                   window=window, num_sinks=num_sinks)
 
         # graph_runner.py:20-27: warm up on a side stream (sizes the workspace).
         warmup_stream = torch.cuda.Stream(device=device)

@@ -24,6 +24,9 @@ Superset of the reference API (keyword-only extensions):
 * ``return_partials=True`` runs the reference's split schedule and also
   returns ``O_partial [B, Hq, ns, D]`` / ``LSE_partial [B, Hq, ns]`` (fp32;
   empty splits hold LSE ``-1e30``, ``split_kv_kernel.py:7-9,32-33``).
+* ``window=W, num_sinks=s``: sliding window. The new token of a row of S tokens
+  sees the last W tokens (its own among them) and the first s; pages that hold
+  none of these are not read, so their table entries may be -1.
 * ``num_splits``: ``None`` or ``0`` selects the token-balanced persistent
   schedule; a positive value selects the reference's split schedule
   (``ns`` equal token ranges per sequence, ``torch_kernel.py:30``).
@@ -130,14 +133,26 @@ def _check(cond: bool, msg: str) -> None:
         raise ValueError(msg)
 
 
+def window_args(who: str, window: Optional[int], num_sinks: int) -> Tuple[int, int]:
+    """(window, sinks) as the C ABI takes them: window 0 stands for none."""
+    if window is None:
+        _check(num_sinks == 0, f"{who}: num_sinks goes with a window")
+        return 0, 0
+    _check(int(window) >= 1, f"{who}: window must be at least 1")
+    _check(int(num_sinks) >= 0, f"{who}: num_sinks must not be negative")
+    # lengths are int32: a longer window sees the same tokens
+    return min(int(window), 2 ** 31 - 1), min(int(num_sinks), 2 ** 31 - 1)
+
+
 def _decode(Q: torch.Tensor, K_Cache: torch.Tensor, V_Cache: torch.Tensor,
             Block_Table: torch.Tensor, seq_len: Union[int, torch.Tensor], block_size: int,
             num_splits: Optional[int] = None, scale: Optional[float] = None,
             return_lse: bool = False, return_partials: bool = False,
             workspace: Optional[DecodeWorkspace] = None, out: Optional[torch.Tensor] = None,
-            kernel_variant: int = 0):
+            kernel_variant: int = 0, window: Optional[int] = None, num_sinks: int = 0):
     # Argument checks, allocation of the outputs and the launch happen in C++
     # (paged_attention/_pa_ext, csrc/torch_ext.cpp) over the C ABI.
+    win, sinks = window_args("paged_attention", window, num_sinks)
     if not (Q.is_cuda and K_Cache.is_cuda and V_Cache.is_cuda and Block_Table.is_cuda):
         raise ValueError("paged_attention: Q, K_Cache, V_Cache and Block_Table must be CUDA tensors")
     ws = workspace if workspace is not None else default_workspace(Q.device)
@@ -150,11 +165,11 @@ def _decode(Q: torch.Tensor, K_Cache: torch.Tensor, V_Cache: torch.Tensor,
             0.0 if scale is None else float(scale), bool(return_lse), bool(return_partials))
     ext = _native.ext()
     status, res, need_bytes, need_counters = ext.decode(
-        *args, ws.buffer, ws.counters, ws.status, int(kernel_variant), out)
+        *args, ws.buffer, ws.counters, ws.status, int(kernel_variant), out, win, sinks)
     if status != 0:
         ws.ensure(need_bytes, need_counters)
         status, res, _, _ = ext.decode(*args, ws.buffer, ws.counters, ws.status,
-                                       int(kernel_variant), out)
+                                       int(kernel_variant), out, win, sinks)
         if status != 0:
             raise PagedAttentionError("pa_decode", _native.PA_ERR_WORKSPACE)
     return res[0] if len(res) == 1 else tuple(res)
@@ -226,7 +241,7 @@ class PagedAttentionV2Function(torch.autograd.Function):
 
 def paged_attention(Q, K_Cache, V_Cache, Block_Table, seq_len, block_size, num_splits=None, *,
                     scale=None, return_lse=False, return_partials=False, workspace=None, out=None,
-                    kernel_variant=0):
+                    kernel_variant=0, window=None, num_sinks=0):
     """Decode attention of one new token per sequence over a paged KV cache.
 
     Reference signature: ``paged_attention/torch_kernel.py:71-73``.
@@ -235,9 +250,9 @@ def paged_attention(Q, K_Cache, V_Cache, Block_Table, seq_len, block_size, num_s
     """
     if torch.is_grad_enabled() and (Q.requires_grad or K_Cache.requires_grad
                                     or V_Cache.requires_grad):
-        if scale is None and not return_lse and not return_partials:
+        if scale is None and not return_lse and not return_partials and window is None:
             return PagedAttentionV2Function.apply(Q, K_Cache, V_Cache, Block_Table, seq_len,
                                                   block_size, num_splits)
         raise RuntimeError("PagedAttentionV2 is inference-only.")
     return _decode(Q, K_Cache, V_Cache, Block_Table, seq_len, block_size, num_splits, scale,
-                   return_lse, return_partials, workspace, out, kernel_variant)
+                   return_lse, return_partials, workspace, out, kernel_variant, window, num_sinks)

@@ -1,0 +1,66 @@
+"""CPU tests of the windowed operators' argument checks. Nothing here launches a kernel."""
+import ctypes
+
+import pytest
+import torch
+
+import paged_attention as pa
+from paged_attention import _native
+
+
+def _decode_args():
+    q = torch.randn(1, 2, 128, dtype=torch.float16)
+    k = torch.randn(2, 16, 2, 128, dtype=torch.float16)
+    return q, k, k, torch.zeros(1, 2, dtype=torch.int32), 16, 16
+
+
+@pytest.mark.parametrize("kw,match", [
+    (dict(window=0), "window must be at least 1"),
+    (dict(window=-5), "window must be at least 1"),
+    (dict(window=8, num_sinks=-1), "num_sinks must not be negative"),
+    (dict(num_sinks=2), "num_sinks goes with a window"),
+])
+def test_window_arguments_refused(kw, match):
+    with pytest.raises(ValueError, match=match):
+        pa.paged_attention(*_decode_args(), **kw)
+
+
+def test_window_with_grad_is_inference_only():
+    q, k, v, bt, s, bs = _decode_args()
+    q.requires_grad_()
+    with pytest.raises(RuntimeError, match="inference-only"):
+        pa.paged_attention(q, k, v, bt, s, bs, window=4)
+
+
+def _params(**kw):
+    p = _native.DecodeParams()
+    p.batch, p.num_heads, p.num_kv_heads, p.head_dim = 2, 8, 2, 128
+    p.block_size, p.num_blocks, p.max_blocks, p.seq_len = 16, 8, 4, 50
+    p.scale, p.dtype = 0.088, _native.PA_F16
+    for k, v in kw.items():
+        setattr(p, k, v)
+    return p
+
+
+@pytest.mark.parametrize("kw,window,sinks,code", [
+    ({}, 0, 0, _native.PA_ERR_ARG),
+    ({}, -1, 0, _native.PA_ERR_ARG),
+    ({}, 16, -1, _native.PA_ERR_ARG),
+    ({"num_splits": 2}, 16, 0, _native.PA_ERR_UNSUPPORTED),
+    ({"head_dim": 96}, 16, 0, _native.PA_ERR_UNSUPPORTED),
+    ({"num_heads": 6, "num_kv_heads": 4}, 16, 0, _native.PA_ERR_ARG),
+    ({"seq_len": 65}, 16, 0, _native.PA_ERR_ARG),
+])
+def test_window_c_abi_refusals(kw, window, sinks, code):
+    lib = _native.lib()
+    p = _params(**kw)
+    a, b = ctypes.c_size_t(0), ctypes.c_size_t(0)
+    assert lib.pa_window_decode_workspace(ctypes.byref(p), window, sinks, ctypes.byref(a),
+                                          ctypes.byref(b)) == code
+    assert lib.pa_window_decode(ctypes.byref(p), window, sinks, None) == code
+
+
+def test_window_c_abi_null():
+    lib = _native.lib()
+    assert lib.pa_window_decode(None, 4, 0, None) == _native.PA_ERR_ARG
+    assert lib.pa_window_decode(ctypes.byref(_params()), 4, 0, None) == _native.PA_ERR_ARG

@@ -1,0 +1,180 @@
+"""GPU tests of windowed decode (``paged_attention(..., window=, num_sinks=)``)
+against the definition in 64 bits, over caches whose invisible slots are NaN and
+whose invisible pages are not there."""
+import ctypes
+
+import pytest
+import torch
+
+from window_helpers import PoisonedCache, assert_lse, assert_matches, reference
+
+pytestmark = pytest.mark.gpu
+
+
+def _lens(window, sinks, bs):
+    """Lengths where the window, the sinks and the pages meet."""
+    base = [0, 1, 2, bs - 1, bs, bs + 1, window - 1, window, window + 1, window + sinks - 1,
+            window + sinks, window + sinks + 1, window + bs, window + sinks + 2 * bs + 1,
+            window + 16, window + 32, window + 33, 3 * window + 5, 1500]
+    return sorted({max(0, min(1500, x)) for x in base})
+
+
+def _run(lens, hq, hkv, d, bs, dtype, window, sinks, seed, **kw):
+    import paged_attention as pa
+    c = PoisonedCache(lens, [1] * len(lens), hkv, d, bs, dtype, window, sinks, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    q = torch.randn(len(lens), hq, d, generator=g).to(dtype).cuda()
+    ws = pa.DecodeWorkspace("cuda")
+    o, lse = pa.paged_attention(q, c.k, c.v, c.table, c.lens, bs, window=window,
+                                num_sinks=sinks, return_lse=True, workspace=ws, **kw)
+    torch.cuda.synchronize()
+    assert ws.read_status() == 0
+    return c, q, o, lse
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("window,sinks", [(1, 0), (1, 3), (7, 1), (64, 4), (100, 40), (512, 0),
+                                          (4000, 4)])
+@pytest.mark.parametrize("hkv,g,d,bs", [(2, 4, 128, 16), (3, 1, 64, 32), (2, 8, 128, 16),
+                                        (1, 3, 128, 8), (2, 2, 256, 16), (2, 12, 64, 64),
+                                        (1, 2, 32, 16), (2, 1, 64, 1), (1, 5, 128, 24),
+                                        (2, 1, 128, 12)])
+def test_window_decode(dtype, window, sinks, hkv, g, d, bs):
+    lens = _lens(window, sinks, bs)
+    c, q, o, lse = _run(lens, hkv * g, hkv, d, bs, dtype, window, sinks, seed=d + bs + g)
+    want, wl, tol = reference(q, c.k, c.v, c.table, c.lens, bs, window, sinks)
+    what = f"{dtype} w{window} s{sinks} d{d} bs{bs} g{g}"
+    assert_matches(o, want, tol, what)
+    assert_lse(lse, wl, d, what)
+
+
+@pytest.mark.parametrize("length", [1, 40, 300, 5000])
+@pytest.mark.parametrize("hkv,g,d", [(8, 4, 128), (32, 1, 128), (4, 8, 64)])
+def test_window_decode_scalar_length(length, hkv, g, d):
+    """One length for every row (an int), and a single long stream (merge pass)."""
+    import paged_attention as pa
+    window, sinks, bs = 1024, 4, 16
+    for batch in (1, 3):
+        lens = [length] * batch
+        c = PoisonedCache(lens, [1] * batch, hkv, d, bs, torch.bfloat16, window, sinks, 11)
+        q = torch.randn(batch, hkv * g, d, device="cuda").bfloat16()
+        o, lse = pa.paged_attention(q, c.k, c.v, c.table, length, bs, window=window,
+                                    num_sinks=sinks, return_lse=True)
+        o2, lse2 = pa.paged_attention(q, c.k, c.v, c.table, c.lens, bs, window=window,
+                                      num_sinks=sinks, return_lse=True)
+        want, wl, tol = reference(q, c.k, c.v, c.table, lens, bs, window, sinks)
+        assert_matches(o, want, tol, f"scalar {length}")
+        assert_lse(lse, wl, d, f"scalar {length}")
+        assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+def test_window_that_covers_everything_is_full_attention():
+    import paged_attention as pa
+    from paged_attention import workloads
+    lens = torch.tensor([1, 17, 300, 999, 64], dtype=torch.int32, device="cuda")
+    w = workloads.build("wide", 5, 16, 4, 16, torch.bfloat16, lens, 63, 400, seed=3)
+    full = pa.paged_attention(w.q, w.k_cache, w.v_cache, w.block_table, lens, 16)
+    for window in (999, 1000, 10 ** 6, 2 ** 40):
+        got = pa.paged_attention(w.q, w.k_cache, w.v_cache, w.block_table, lens, 16,
+                                 window=window, num_sinks=4)
+        # the schedules may split rows elsewhere: one rounding of the output apart
+        assert_matches(got, full.double().cpu(), 2 * 2.0 ** -8 * full.double().cpu().abs() + 1e-5,
+                       f"window {window}")
+
+
+@pytest.mark.parametrize("batch", [1024, 1025, 2100])
+def test_window_decode_beyond_the_per_row_limit(batch):
+    """More rows than one launch's schedule holds."""
+    lens = [(i * 37) % 90 for i in range(batch)]
+    c, q, o, lse = _run(lens, 2, 1, 64, 16, torch.float16, 20, 3, seed=5)
+    want, wl, tol = reference(q, c.k, c.v, c.table, c.lens, 16, 20, 3)
+    assert_matches(o, want, tol, f"batch {batch}")
+    assert_lse(lse, wl, 64, f"batch {batch}")
+
+
+def test_window_decode_strided_inputs_and_out():
+    """Caches that are slices of a joint [pages, 2, slots, heads, D] buffer, a strided q, a given out."""
+    import paged_attention as pa
+    lens, window, sinks, bs, hkv, d = [5, 700, 90], 100, 4, 16, 2, 128
+    c = PoisonedCache(lens, [1] * 3, hkv, d, bs, torch.float16, window, sinks, 7)
+    kv = torch.stack([c.k, c.v], 1)
+    qbig = torch.randn(3, 5, 2 * hkv, d, device="cuda").half()
+    q = qbig[:, 2]
+    out = torch.full((4, 2 * hkv, d), 7.0, device="cuda").half()
+    got = pa.paged_attention(q, kv[:, 0], kv[:, 1], c.table, c.lens, bs, window=window,
+                             num_sinks=sinks, out=out[:3])
+    want, _, tol = reference(q, c.k, c.v, c.table, lens, bs, window, sinks)
+    assert got.data_ptr() == out.data_ptr()
+    assert_matches(got, want, tol, "strided")
+    assert (out[3] == 7).all()
+
+
+def test_window_graph_runner_follows_lengths():
+    import paged_attention as pa
+    window, sinks, bs, hkv, g, d, b = 50, 4, 16, 2, 4, 128, 4
+    runner = pa.PagedAttnGraphRunner(b, hkv * g, d, 16, bs, 64, dtype=torch.bfloat16,
+                                     num_kv_heads=hkv, dynamic_seq_lens=True, max_seq_len=640,
+                                     window=window, num_sinks=sinks)
+    for k, lens in enumerate(([1, 40, 300, 640], [0, 55, 54, 90], [640, 640, 1, 2])):
+        c = PoisonedCache(lens, [1] * b, hkv, d, bs, torch.bfloat16, window, sinks, k, width=40)
+        q = torch.randn(b, hkv * g, d, device="cuda").bfloat16()
+        pool = torch.full((64, bs, hkv, d), float("nan"), device="cuda").bfloat16()
+        kk, vv = pool.clone(), pool.clone()
+        kk[: c.k.shape[0]], vv[: c.v.shape[0]] = c.k, c.v
+        out = runner.run(q, kk, vv, c.table, copy_kv=True, seq_lens=c.lens)
+        want, _, tol = reference(q, c.k, c.v, c.table, lens, bs, window, sinks)
+        assert_matches(out, want, tol, f"graph {lens}")
+
+
+def test_window_decode_on_another_stream():
+    lens = [2000] * 6
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        c, q, o, lse = _run(lens, 8, 2, 128, 16, torch.bfloat16, 300, 4, seed=9)
+    want, wl, tol = reference(q, c.k, c.v, c.table, c.lens, 16, 300, 4)
+    assert_matches(o, want, tol, "side stream")
+
+
+def test_window_decode_flags_bad_page_and_length():
+    """A visible page outside the pool and a length beyond the table are flagged, not fatal;
+    an invisible page may be anything."""
+    import paged_attention as pa
+    from paged_attention import _native
+    c = PoisonedCache([200, 200], [1, 1], 1, 64, 16, torch.float16, 50, 4, 3)
+    q = torch.randn(2, 1, 64, device="cuda").half()
+    ws = pa.DecodeWorkspace("cuda")
+    c.table[0, 5] = 10 ** 6                      # tokens 80..95: not visible
+    pa.paged_attention(q, c.k, c.v, c.table, c.lens, 16, window=50, num_sinks=4, workspace=ws)
+    assert ws.read_status() == 0
+    c.table[0, 11] = 10 ** 6                     # tokens 176..191: visible
+    pa.paged_attention(q, c.k, c.v, c.table, c.lens, 16, window=50, num_sinks=4, workspace=ws)
+    assert ws.read_status() == _native.PA_STATUS_BAD_BLOCK
+    ws.reset()
+    c.lens[1] = 16 * 13 + 1
+    pa.paged_attention(q, c.k, c.v, c.table, c.lens, 16, window=50, num_sinks=4, workspace=ws)
+    assert ws.read_status() & _native.PA_STATUS_BAD_SEQLEN
+
+
+def test_window_decode_through_ctypes_with_its_own_workspace():
+    import paged_attention as pa
+    from paged_attention import _native
+    lens, window, sinks, bs, hkv, d = [900, 3, 0], 128, 4, 16, 2, 128
+    c = PoisonedCache(lens, [1] * 3, hkv, d, bs, torch.bfloat16, window, sinks, 1)
+    q = torch.randn(3, 4 * hkv, d, device="cuda").bfloat16()
+    out = torch.empty_like(q)
+    p = pa.decode_params(q, c.k, c.v, c.table, c.lens, bs, out=out)
+    lib = _native.lib()
+    nb, nc = ctypes.c_size_t(), ctypes.c_size_t()
+    assert lib.pa_window_decode_workspace(ctypes.byref(p), window, sinks, ctypes.byref(nb),
+                                          ctypes.byref(nc)) == 0
+    buf = torch.empty(max(16, nb.value), dtype=torch.uint8, device="cuda")
+    cnt = torch.zeros(max(1, nc.value), dtype=torch.int32, device="cuda")
+    p.workspace, p.workspace_bytes = buf.data_ptr(), nb.value
+    p.counters, p.counter_count = cnt.data_ptr(), nc.value
+    stream = torch.cuda.current_stream().cuda_stream
+    for _ in range(2):
+        assert lib.pa_window_decode(ctypes.byref(p), window, sinks, stream) == 0
+        want, _, tol = reference(q, c.k, c.v, c.table, lens, bs, window, sinks)
+        assert_matches(out, want, tol, "ctypes")
+        out.zero_()
+        assert int(cnt.abs().sum()) == 0
