@@ -55,6 +55,8 @@ typedef enum pa_dtype { PA_F16 = 0, PA_BF16 = 1 } pa_dtype_t;
 #define PA_STATUS_BAD_BLOCK 1u    /* a block-table entry outside [0, num_blocks) */
 #define PA_STATUS_BAD_SEQLEN 2u   /* seq_lens[b] < 0 or > max_blocks * block_size (clamped) */
 #define PA_STATUS_TIMEOUT 4u      /* a bounded wait on a copy barrier gave up (2 s) */
+#define PA_STATUS_NO_PAGES 8u     /* the pool has too few free pages: a row stayed as it was */
+#define PA_STATUS_BAD_ROW 16u     /* a fork's row outside the table, or a child that is not empty */
 
 /* One decode step: O[b, h] = softmax(q[b, h] . K_b^T * scale) V_b, where token t
  * of sequence b lives at cache[block_table[b, t / block_size], t % block_size,
@@ -177,6 +179,79 @@ typedef struct pa_append_params {
 } pa_append_params;
 
 PA_API pa_status_t pa_cache_append(const pa_append_params* p, cudaStream_t stream);
+
+/* ---- Page accounting ------------------------------------------------------
+ *
+ * A pool of pages that the caches of `num_layers` layers share: page i is
+ * cache[i] of every layer's K and V cache. Counts, free bits, block tables and
+ * lengths are device memory that the calls below change on `stream`, without a
+ * host round trip; a captured graph replays them on the state it then finds.
+ * Free pages are taken in ascending order. Calls on one pool share its state
+ * and scratch, so they must be ordered (one stream, or events). No counterpart
+ * in the reference, whose tables are built by test code
+ * (tests/correctness.py:26-36).
+ *
+ * Block tables are int32 [rows, max_blocks], row stride bt_stride_b elements;
+ * entry -1: no page. seq_lens are int32 [rows]; a row of S tokens uses the
+ * entries j < ceil(S / block_size), of which a sliding window may have given
+ * some back (-1). */
+typedef struct pa_page_pool {
+  void* const* caches;         /* device array [2 * num_layers]: layer l's K cache at 2l, its V
+                                  cache at 2l + 1 (16-byte aligned); NULL when num_layers is 0 */
+  int32_t num_layers;
+  int64_t k_stride_block, k_stride_slot, k_stride_head;   /* elements, multiples of 8; the same */
+  int64_t v_stride_block, v_stride_slot, v_stride_head;   /* for every layer */
+  int32_t num_blocks, block_size, num_kv_heads, head_dim; /* 16-bit elements; head_dim % 8 == 0 */
+  int32_t* refs;               /* [num_blocks] users of each page, 0: free */
+  uint32_t* free_words;        /* [ceil(num_blocks / 32)] bit i % 32 of word i / 32: page i is free;
+                                  bits behind num_blocks are 0 */
+  int32_t* scratch;            /* pa_pages_scratch ints; the first 32 zeroed once by the caller */
+  size_t scratch_ints;
+  uint32_t* status;            /* optional device word, PA_STATUS_* bits OR-ed in */
+} pa_page_pool;
+
+/* int32s of scratch for tables of up to `rows` rows and forks of up to `pairs` pairs. */
+PA_API pa_status_t pa_pages_scratch(const pa_page_pool* pool, int32_t rows, int32_t pairs,
+                                    size_t* ints);
+
+/* Row r goes from seq_lens[r] to new_lens[r] tokens (negative: the row is left
+ * alone). First every row releases its pages behind the new length and, with a
+ * window (window > 0), the pages in which no token is visible to the next
+ * queries (positions >= min(old, new)) nor among the first num_sinks. Then, in
+ * row order, growing rows take the pages they miss, all of them or none
+ * (PA_STATUS_NO_PAGES: the row keeps its old length, and so does every later
+ * row that needs pages). A row that grows
+ * into a partly filled last page that has other users gets a copy of its own
+ * (the used slots, in every layer); when all users do so in one call, the page
+ * itself ends up free. A length outside the table leaves the row alone
+ * (PA_STATUS_BAD_SEQLEN); releasing a page that is free, or none of the pool's,
+ * changes no count (PA_STATUS_BAD_BLOCK). */
+PA_API pa_status_t pa_pages_resize(const pa_page_pool* pool, int32_t* block_table,
+                                   int64_t bt_stride_b, int32_t rows, int32_t max_blocks,
+                                   int32_t* seq_lens, const int32_t* new_lens, int32_t window,
+                                   int32_t num_sinks, cudaStream_t stream);
+
+/* Pair i: row children[i], which has to be empty (length 0), continues row
+ * parents[i]: full pages are shared, the partly filled last page is copied (its
+ * used slots, in every layer) to a new page, entries behind it become -1. A
+ * negative parent or child skips the pair. A parent may appear any number of
+ * times; of pairs with the same child the first goes through, the others are
+ * skipped (PA_STATUS_BAD_ROW, as for a child that is not empty or a row outside
+ * the table). A row that is a child of the call counts as empty where it is a
+ * parent. Without a free page the child stays empty (PA_STATUS_NO_PAGES). */
+PA_API pa_status_t pa_pages_fork(const pa_page_pool* pool, int32_t* block_table,
+                                 int64_t bt_stride_b, int32_t rows, int32_t max_blocks,
+                                 int32_t* seq_lens, const int32_t* parents,
+                                 const int32_t* children, int32_t num_pairs, cudaStream_t stream);
+
+/* Moves the live pages (refs > 0) into [0, *live), *live being their number:
+ * in ascending order, live pages at or behind *live go to the free pages before
+ * it, in every layer; the table entries follow. Other pages keep their places
+ * and contents. An entry that names a free page behind *live is left
+ * (PA_STATUS_BAD_BLOCK). The table must hold every row that uses the pool. */
+PA_API pa_status_t pa_pages_compact(const pa_page_pool* pool, int32_t* block_table,
+                                    int64_t bt_stride_b, int32_t rows, int32_t max_blocks,
+                                    int32_t* live, cudaStream_t stream);
 
 /* Allocation-free variant of pa_decode. It has no counterpart in the reference.
  *

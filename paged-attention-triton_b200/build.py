@@ -19,7 +19,8 @@ from concurrent.futures import ThreadPoolExecutor
 HERE = os.path.dirname(os.path.abspath(__file__))
 REPO = os.path.dirname(HERE)
 INCLUDE = os.path.join(REPO, "include")
-SOURCES = [os.path.join(HERE, "csrc", "pa_decode.cu")]
+SOURCES = [os.path.join(HERE, "csrc", "pa_decode.cu"),     # in parts, see PARTS
+           os.path.join(HERE, "csrc", "pa_pages.cu")]
 HEADERS = [os.path.join(INCLUDE, "pa_decode.h"), os.path.join(HERE, "csrc", "fastdiv.h")]
 OUTPUT = os.path.join(HERE, "paged_attention", "libpa_decode.so")
 EXT_SOURCE = os.path.join(HERE, "csrc", "torch_ext.cpp")
@@ -114,16 +115,27 @@ def _build_library(force: bool = False, verbose: bool = False) -> str:
     if not force and not _stale():
         return OUTPUT
     os.makedirs(BUILD_DIR, exist_ok=True)
-    src = SOURCES[0]
-    objs = [os.path.join(BUILD_DIR, f"pa_decode_part{k}.o") for k in PARTS]
-    cmds = []
-    for k, obj in zip(PARTS, objs):
-        cmd = [_nvcc(), *COMPILE_FLAGS, f"-DPA_PART={k}", f"-I{INCLUDE}", "-c", "-o", obj, src]
+    units = [(SOURCES[0], f"pa_decode_part{k}.o", [f"-DPA_PART={k}"]) for k in PARTS]
+    units += [(src, os.path.basename(src)[:-3] + ".o", []) for src in SOURCES[1:]]
+    objs, cmds = [], []
+    for src, name, defs in units:
+        obj = os.path.join(BUILD_DIR, name)
+        objs.append(obj)
+        # an object newer than its source, the headers and this file is kept
+        newest = max(os.path.getmtime(f) for f in [src, *HEADERS, __file__])
+        if not force and os.path.exists(obj) and os.path.getmtime(obj) > newest:
+            continue
+        cmd = [_nvcc(), *COMPILE_FLAGS, *defs, f"-I{INCLUDE}", "-c", "-o", obj + ".tmp", src]
         if verbose:
             cmd.insert(1, "-Xptxas=-v")
-        cmds.append(cmd)
-    with ThreadPoolExecutor(max_workers=min(len(cmds), os.cpu_count() or 1)) as pool:
-        list(pool.map(lambda c: _run(c, verbose), cmds))
+        cmds.append((cmd, obj))
+
+    def compile_one(unit):
+        _run(unit[0], verbose)
+        os.replace(unit[1] + ".tmp", unit[1])
+
+    with ThreadPoolExecutor(max_workers=max(1, min(len(cmds), os.cpu_count() or 1))) as pool:
+        list(pool.map(compile_one, cmds))
     _run([_nvcc(), *LINK_FLAGS, "-o", OUTPUT + ".tmp", *objs], verbose)
     os.replace(OUTPUT + ".tmp", OUTPUT)
     return OUTPUT

@@ -11,6 +11,7 @@
 #include <torch/extension.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 
 #include <cmath>
 #include <tuple>
@@ -221,10 +222,167 @@ void cache_append(const at::Tensor& key, const at::Tensor& value, const at::Tens
   TORCH_CHECK(rc == PA_OK, "pa_cache_append failed: ", pa_status_string(rc));
 }
 
+// A pool of pages (page_pool.py): the caches, the counts and free bits, and the
+// scratch of its calls.
+class PagePool {
+ public:
+  PagePool(std::vector<at::Tensor> k, std::vector<at::Tensor> v, int64_t num_blocks,
+           int64_t block_size, const at::Device& device)
+      : k_(std::move(k)), v_(std::move(v)), device_(device) {
+    check(k_.size() == v_.size(), "k_caches and v_caches differ in number");
+    check(device.is_cuda(), "the pool's caches must be CUDA tensors");
+    pool_.num_layers = static_cast<int32_t>(k_.size());
+    pool_.num_kv_heads = 1;
+    pool_.head_dim = 8;
+    std::vector<int64_t> ptrs;
+    for (size_t l = 0; l < k_.size(); ++l) {
+      for (const at::Tensor* t : {&k_[l], &v_[l]}) {
+        check(t->is_cuda() && t->device() == device, "caches on different devices");
+        dtype_code(*t);
+        check(t->scalar_type() == k_[0].scalar_type(), "caches must share one dtype");
+        check(t->dim() == 4 && t->sizes() == k_[0].sizes(),
+              "caches must all be [num_blocks, block_size, Hkv, D]");
+        check(t->stride(3) == 1, "head_dim must be contiguous");
+        check(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0 && t->stride(0) % 8 == 0 &&
+                  t->stride(1) % 8 == 0 && t->stride(2) % 8 == 0,
+              "caches must be 16-byte aligned, with strides that are multiples of 8");
+        const at::Tensor& first = (t == &k_[l]) ? k_[0] : v_[0];
+        check(t->strides() == first.strides(), "the layers' caches must have the same strides");
+        ptrs.push_back(reinterpret_cast<int64_t>(t->data_ptr()));
+      }
+    }
+    if (!k_.empty()) {
+      check(k_[0].size(0) == num_blocks && k_[0].size(1) == block_size,
+            "num_blocks or block_size differs from the caches'");
+      check(k_[0].size(3) % 8 == 0, "head_dim must be a multiple of 8");
+      pool_.num_kv_heads = static_cast<int32_t>(k_[0].size(2));
+      pool_.head_dim = static_cast<int32_t>(k_[0].size(3));
+      pool_.k_stride_block = k_[0].stride(0);
+      pool_.k_stride_slot = k_[0].stride(1);
+      pool_.k_stride_head = k_[0].stride(2);
+      pool_.v_stride_block = v_[0].stride(0);
+      pool_.v_stride_slot = v_[0].stride(1);
+      pool_.v_stride_head = v_[0].stride(2);
+    }
+    check(num_blocks > 0 && num_blocks <= (1 << 29) && block_size > 0 && block_size <= (1 << 20),
+          "num_blocks or block_size out of range");
+    pool_.num_blocks = static_cast<int32_t>(num_blocks);
+    pool_.block_size = static_cast<int32_t>(block_size);
+    c10::cuda::CUDAGuard guard(device);
+    const auto i32 = at::TensorOptions().dtype(at::kInt).device(device);
+    const int64_t words = (num_blocks + 31) / 32;
+    state_ = at::zeros({num_blocks + words}, i32);
+    refs_ = state_.narrow(0, 0, num_blocks);
+    words_ = state_.narrow(0, num_blocks, words);
+    status_ = at::zeros({1}, i32);
+    ptrs_ = at::tensor(ptrs, at::TensorOptions().dtype(at::kLong)).to(device);
+    pool_.caches = k_.empty() ? nullptr : reinterpret_cast<void* const*>(ptrs_.data_ptr());
+    pool_.refs = refs_.data_ptr<int32_t>();
+    pool_.free_words = reinterpret_cast<uint32_t*>(words_.data_ptr<int32_t>());
+    pool_.status = reinterpret_cast<uint32_t*>(status_.data_ptr<int32_t>());
+    ensure(1024, 1024);
+  }
+
+  void resize(const at::Tensor& bt, const at::Tensor& lens, const at::Tensor& new_lens,
+              int64_t window, int64_t num_sinks) {
+    table(bt);
+    rows(lens, bt, "seq_lens");
+    rows(new_lens, bt, "new_lens");
+    c10::cuda::CUDAGuard guard(device_);
+    ensure(bt.size(0), 0);
+    done(pa_pages_resize(&pool_, bt.data_ptr<int32_t>(), bt.stride(0), n(bt, 0), n(bt, 1),
+                         lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(),
+                         static_cast<int32_t>(window), static_cast<int32_t>(num_sinks), stream()),
+         "pa_pages_resize");
+  }
+
+  void fork(const at::Tensor& bt, const at::Tensor& lens, const at::Tensor& parents,
+            const at::Tensor& children) {
+    table(bt);
+    rows(lens, bt, "seq_lens");
+    for (const at::Tensor* t : {&parents, &children})
+      check(t->device() == device_ && t->scalar_type() == at::kInt && t->dim() == 1 &&
+                t->is_contiguous() && t->size(0) == parents.size(0),
+            "parents and children must be contiguous int32 [n] tensors on the pool's device");
+    c10::cuda::CUDAGuard guard(device_);
+    ensure(bt.size(0), parents.size(0));
+    done(pa_pages_fork(&pool_, bt.data_ptr<int32_t>(), bt.stride(0), n(bt, 0), n(bt, 1),
+                       lens.data_ptr<int32_t>(), parents.data_ptr<int32_t>(),
+                       children.data_ptr<int32_t>(), n(parents, 0), stream()),
+         "pa_pages_fork");
+  }
+
+  at::Tensor compact(const at::Tensor& bt) {
+    table(bt);
+    c10::cuda::CUDAGuard guard(device_);
+    ensure(bt.size(0), 0);
+    at::Tensor live = at::empty({1}, state_.options());
+    done(pa_pages_compact(&pool_, bt.data_ptr<int32_t>(), bt.stride(0), n(bt, 0), n(bt, 1),
+                          live.data_ptr<int32_t>(), stream()),
+         "pa_pages_compact");
+    return live;
+  }
+
+  at::Tensor state_, refs_, words_, status_;
+
+ private:
+  static int32_t n(const at::Tensor& t, int d) { return static_cast<int32_t>(t.size(d)); }
+  void table(const at::Tensor& bt) const {
+    check(bt.device() == device_ && bt.scalar_type() == at::kInt && bt.dim() == 2 &&
+              (bt.size(1) <= 1 || bt.stride(1) == 1) &&
+              (bt.size(0) <= 1 || bt.stride(0) >= bt.size(1)),
+          "Block_Table must be an int32 [rows, max_blocks] tensor on the pool's device, its rows "
+          "apart and contiguous");
+    check(bt.size(0) <= INT32_MAX && bt.size(1) <= INT32_MAX / 2, "Block_Table is too large");
+  }
+  void rows(const at::Tensor& t, const at::Tensor& bt, const char* name) const {
+    TORCH_CHECK_VALUE(t.device() == device_ && t.scalar_type() == at::kInt && t.dim() == 1 &&
+                          t.is_contiguous() && t.size(0) == bt.size(0),
+                      "paged_attention: ", name,
+                      " must be a contiguous int32 [rows] tensor on the pool's device");
+  }
+  cudaStream_t stream() const {
+    return c10::cuda::getCurrentCUDAStream(device_.index()).stream();
+  }
+  void done(pa_status_t rc, const char* what) const {
+    TORCH_CHECK(rc == PA_OK, what, " failed: ", pa_status_string(rc));
+  }
+  // Scratch for tables of `r` rows and forks of `p` pairs. It grows outside
+  // capture only: a graph that is replayed keeps the address it was captured with.
+  void ensure(int64_t r, int64_t p) {
+    size_t ints = 0;
+    done(pa_pages_scratch(&pool_, static_cast<int32_t>(r), static_cast<int32_t>(p), &ints),
+         "pa_pages_scratch");
+    if (ints <= pool_.scratch_ints) return;
+    TORCH_CHECK(c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None,
+                "paged_attention: the pool's scratch has to grow for this table; make one call with "
+                "it before capturing");
+    scratch_.push_back(at::zeros({static_cast<int64_t>(ints)}, state_.options()));
+    pool_.scratch = scratch_.back().data_ptr<int32_t>();
+    pool_.scratch_ints = ints;
+  }
+
+  std::vector<at::Tensor> k_, v_;
+  at::Device device_;
+  at::Tensor ptrs_;
+  std::vector<at::Tensor> scratch_;   // earlier ones stay: captured graphs may hold them
+  pa_page_pool pool_{};
+};
+
 }  // namespace
 
 PYBIND11_MODULE(_pa_ext, m) {
   m.def("cache_append", &cache_append, "write K/V rows into the paged caches by slot");
   m.doc() = "PyTorch binding of the sm_100a paged-attention decode C ABI";
+  py::class_<PagePool>(m, "PagePool")
+      .def(py::init<std::vector<at::Tensor>, std::vector<at::Tensor>, int64_t, int64_t,
+                    const at::Device&>())
+      .def("resize", &PagePool::resize)
+      .def("fork", &PagePool::fork)
+      .def("compact", &PagePool::compact)
+      .def_readonly("state", &PagePool::state_)
+      .def_readonly("refs", &PagePool::refs_)
+      .def_readonly("free_words", &PagePool::words_)
+      .def_readonly("status", &PagePool::status_);
   m.def("decode", &decode, "one paged-attention decode step (see torch_kernel.py)");
 }

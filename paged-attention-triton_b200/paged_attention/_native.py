@@ -24,6 +24,8 @@ PA_BF16 = 1
 PA_STATUS_BAD_BLOCK = 1
 PA_STATUS_BAD_SEQLEN = 2
 PA_STATUS_TIMEOUT = 4
+PA_STATUS_NO_PAGES = 8
+PA_STATUS_BAD_ROW = 16
 
 # size of the scratch array pa_decode_noalloc uses (PA_NOALLOC_SCRATCH_BYTES)
 PA_NOALLOC_SCRATCH_BYTES = 16 << 20
@@ -124,6 +126,30 @@ class PlanInfo(ctypes.Structure):
     ]
 
 
+class PagePoolParams(ctypes.Structure):
+    """Mirror of ``pa_page_pool``."""
+
+    _fields_ = [
+        ("caches", ctypes.c_void_p),
+        ("num_layers", ctypes.c_int32),
+        ("k_stride_block", ctypes.c_int64),
+        ("k_stride_slot", ctypes.c_int64),
+        ("k_stride_head", ctypes.c_int64),
+        ("v_stride_block", ctypes.c_int64),
+        ("v_stride_slot", ctypes.c_int64),
+        ("v_stride_head", ctypes.c_int64),
+        ("num_blocks", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("refs", ctypes.c_void_p),
+        ("free_words", ctypes.c_void_p),
+        ("scratch", ctypes.c_void_p),
+        ("scratch_ints", ctypes.c_size_t),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 # name -> (restype, argtypes); every function declared in include/pa_decode.h.
 _SIGNATURES = {
     "pa_decode_workspace": (ctypes.c_int, [ctypes.POINTER(DecodeParams),
@@ -139,6 +165,19 @@ _SIGNATURES = {
     "pa_window_decode": (ctypes.c_int, [ctypes.POINTER(DecodeParams), ctypes.c_int32,
                                         ctypes.c_int32, ctypes.c_void_p]),
     "pa_cache_append": (ctypes.c_int, [ctypes.POINTER(AppendParams), ctypes.c_void_p]),
+    "pa_pages_scratch": (ctypes.c_int, [ctypes.POINTER(PagePoolParams), ctypes.c_int32,
+                                        ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
+    "pa_pages_resize": (ctypes.c_int, [ctypes.POINTER(PagePoolParams), ctypes.c_void_p,
+                                       ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                       ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,
+                                       ctypes.c_int32, ctypes.c_void_p]),
+    "pa_pages_fork": (ctypes.c_int, [ctypes.POINTER(PagePoolParams), ctypes.c_void_p,
+                                     ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                     ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p,
+                                     ctypes.c_int32, ctypes.c_void_p]),
+    "pa_pages_compact": (ctypes.c_int, [ctypes.POINTER(PagePoolParams), ctypes.c_void_p,
+                                        ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                        ctypes.c_void_p, ctypes.c_void_p]),
     "pa_num_splits_heuristic": (ctypes.c_int32, [ctypes.c_int32] * 5),
     "pa_selftest_wait_timeout": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p,
                                                 ctypes.c_uint64, ctypes.c_void_p,
