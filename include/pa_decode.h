@@ -156,6 +156,50 @@ PA_API pa_status_t pa_window_decode_workspace(const pa_decode_params* p, int32_t
 PA_API pa_status_t pa_window_decode(const pa_decode_params* p, int32_t window, int32_t num_sinks,
                              cudaStream_t stream);
 
+/* Prompt attention: chunks of new tokens attend to their sequences' cached
+ * tokens, their own (already in the cache) among them. Sequence b has the query
+ * rows [query_starts[b], query_starts[b + 1]), which are its last tokens: row i
+ * of n sits at position seq_lens[b] - n + i and sees token t when t <= position
+ * and, with a window, t < num_sinks or t > position - window. Rows that see
+ * nothing (positions before 0) get O = 0 and LSE = -1e30; rows outside every
+ * sequence are not written. Pages with no visible token are not read; their
+ * table entries may be anything. Slots of visible pages behind the sequence's
+ * end may hold anything too; a NaN or infinity inside the sequence may reach
+ * the rows of the same chunk that do not see it. query_starts has to ascend within
+ * [0, num_tokens], else what does not is cut (PA_STATUS_BAD_SEQLEN); a visible
+ * page outside the pool leaves the rows that see it undefined
+ * (PA_STATUS_BAD_BLOCK). No counterpart in the reference, which attends from
+ * single new tokens only. */
+typedef struct pa_prompt_params {
+  /* query and output [num_tokens, num_heads, head_dim], strides in elements */
+  const void* q;
+  int64_t q_stride_t, q_stride_h;
+  const void* k_cache;           /* as in pa_decode_params */
+  int64_t k_stride_block, k_stride_slot, k_stride_head;
+  const void* v_cache;
+  int64_t v_stride_block, v_stride_slot, v_stride_head;
+  const int32_t* block_table;    /* [batch, max_blocks] */
+  int64_t bt_stride_b;
+  int32_t max_blocks;
+  const int32_t* query_starts;   /* [batch + 1], device */
+  const int32_t* seq_lens;       /* [batch], device: lengths with the chunk */
+  int32_t num_tokens, batch, num_heads, num_kv_heads, head_dim, block_size, num_blocks;
+  int32_t window;                /* 0: none */
+  int32_t num_sinks;             /* goes with a window */
+  float scale;
+  int32_t dtype;
+  void* out;
+  int64_t out_stride_t, out_stride_h;
+  float* lse;                    /* optional [num_tokens, num_heads] */
+  int32_t num_splits;            /* parts of a sequence's keys that separate CTAs take; 0: automatic */
+  void* workspace;               /* pa_prompt_workspace bytes, 16-byte aligned */
+  size_t workspace_bytes;
+  uint32_t* status;              /* optional device word */
+} pa_prompt_params;
+
+PA_API pa_status_t pa_prompt_workspace(const pa_prompt_params* p, size_t* workspace_bytes);
+PA_API pa_status_t pa_prompt(const pa_prompt_params* p, cudaStream_t stream);
+
 /* New tokens' K/V rows into the paged caches (the step before decode in a
  * serving loop; the reference fills its caches in test code,
  * tests/correctness.py:30-36). Row t of key/value ([num_tokens, num_kv_heads,

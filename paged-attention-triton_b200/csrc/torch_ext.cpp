@@ -169,6 +169,100 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> decode(
   return {0, std::move(res), 0, 0};
 }
 
+// Prompt attention (prompt.py): (status, [out[, lse]], bytes); status -1: the
+// workspace is too small for `bytes`, and nothing was launched.
+std::tuple<int64_t, std::vector<at::Tensor>, int64_t> prompt(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& bt,
+    const at::Tensor& query_starts, const at::Tensor& seq_lens, int64_t block_size, double scale,
+    bool return_lse, const at::Tensor& ws_buffer, const at::Tensor& ws_status,
+    const c10::optional<at::Tensor>& out_opt, int64_t window, int64_t num_sinks,
+    int64_t num_splits) {
+  const auto dev = q.device();
+  for (const at::Tensor* t : {&q, &k, &v, &bt, &query_starts, &seq_lens})
+    check(t->is_cuda() && t->device() == dev, "all tensors must be on one CUDA device");
+  check(q.dim() == 3, "Q must be [T, H, D]");
+  check(k.dim() == 4 && v.sizes() == k.sizes(),
+        "K_Cache and V_Cache must both be [num_blocks, block_size, Hkv, D]");
+  const int dt = dtype_code(q);
+  check(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+        "Q, K_Cache and V_Cache must share one dtype");
+  check(bt.scalar_type() == at::kInt && bt.dim() == 2,
+        "Block_Table must be an int32 [B, max_blocks] tensor");
+  const int64_t batch = bt.size(0), tokens = q.size(0), heads = q.size(1), dim = q.size(2);
+  check(k.size(3) == dim, "head_dim of Q and the caches differ");
+  check(dim == 32 || dim == 64 || dim == 128 || dim == 256,
+        "head_dim must be 32, 64, 128 or 256");
+  check(block_size == k.size(1) && block_size >= 1,
+        "block_size differs from the cache's block dimension");
+  check(k.size(2) > 0 && heads > 0 && heads % k.size(2) == 0, "Hq must be a multiple of Hkv");
+  for (const at::Tensor* t : {&query_starts, &seq_lens})
+    check(t->scalar_type() == at::kInt && t->dim() == 1 && t->is_contiguous(),
+          "query_starts and seq_lens must be contiguous int32 tensors");
+  check(query_starts.size(0) == batch + 1, "query_starts must have B + 1 entries");
+  check(seq_lens.size(0) == batch, "seq_lens must have B entries");
+  check(k.stride(3) == 1 && v.stride(3) == 1 && (bt.size(1) <= 1 || bt.stride(1) == 1),
+        "last dimensions must be contiguous");
+  check(tokens <= INT32_MAX && batch < INT32_MAX && bt.size(1) <= INT32_MAX, "sizes beyond int32");
+
+  c10::cuda::CUDAGuard guard(dev);
+  at::Tensor Q = q;
+  if (q.stride(2) != 1 || q.stride(0) % 8 || q.stride(1) % 8 ||
+      reinterpret_cast<uintptr_t>(q.data_ptr()) % 16)
+    Q = q.contiguous();
+  at::Tensor out = out_opt.has_value() ? *out_opt : at::empty({tokens, heads, dim}, Q.options());
+  check(out.device() == dev && out.sizes() == Q.sizes() && out.scalar_type() == Q.scalar_type() &&
+            out.stride(2) == 1,
+        "out must match Q's shape, dtype and device");
+  at::Tensor lse;
+  if (return_lse) lse = at::empty({tokens, heads}, Q.options().dtype(at::kFloat));
+
+  pa_prompt_params p{};
+  p.q = Q.data_ptr();
+  p.q_stride_t = Q.stride(0);
+  p.q_stride_h = Q.stride(1);
+  p.k_cache = k.data_ptr();
+  p.k_stride_block = k.stride(0);
+  p.k_stride_slot = k.stride(1);
+  p.k_stride_head = k.stride(2);
+  p.v_cache = v.data_ptr();
+  p.v_stride_block = v.stride(0);
+  p.v_stride_slot = v.stride(1);
+  p.v_stride_head = v.stride(2);
+  p.block_table = bt.data_ptr<int32_t>();
+  p.bt_stride_b = bt.stride(0);
+  p.max_blocks = static_cast<int32_t>(bt.size(1));
+  p.query_starts = query_starts.data_ptr<int32_t>();
+  p.seq_lens = seq_lens.data_ptr<int32_t>();
+  p.num_tokens = static_cast<int32_t>(tokens);
+  p.batch = static_cast<int32_t>(batch);
+  p.num_heads = static_cast<int32_t>(heads);
+  p.num_kv_heads = static_cast<int32_t>(k.size(2));
+  p.head_dim = static_cast<int32_t>(dim);
+  p.block_size = static_cast<int32_t>(block_size);
+  p.num_blocks = static_cast<int32_t>(k.size(0));
+  p.window = static_cast<int32_t>(window);
+  p.num_sinks = static_cast<int32_t>(num_sinks);
+  p.scale = static_cast<float>(scale > 0 ? scale : 1.0 / std::sqrt(static_cast<double>(dim)));
+  p.dtype = dt;
+  p.out = out.data_ptr();
+  p.out_stride_t = out.stride(0);
+  p.out_stride_h = out.stride(1);
+  p.lse = return_lse ? lse.data_ptr<float>() : nullptr;
+  p.num_splits = static_cast<int32_t>(num_splits);
+  size_t bytes = 0;
+  pa_status_t rc = pa_prompt_workspace(&p, &bytes);
+  TORCH_CHECK(rc == PA_OK, "pa_prompt_workspace failed: ", pa_status_string(rc));
+  if (bytes > static_cast<size_t>(ws_buffer.numel())) return {-1, {}, static_cast<int64_t>(bytes)};
+  p.workspace = bytes ? ws_buffer.data_ptr() : nullptr;
+  p.workspace_bytes = bytes;
+  p.status = reinterpret_cast<uint32_t*>(ws_status.data_ptr<int32_t>());
+  rc = pa_prompt(&p, c10::cuda::getCurrentCUDAStream(dev.index()).stream());
+  TORCH_CHECK(rc == PA_OK, "pa_prompt failed: ", pa_status_string(rc));
+  std::vector<at::Tensor> res{out};
+  if (return_lse) res.push_back(lse);
+  return {0, std::move(res), 0};
+}
+
 // Writes key/value rows [T, Hkv, D] into the paged caches at slot_mapping[t]
 // (negative: skipped) through pa_cache_append.
 void cache_append(const at::Tensor& key, const at::Tensor& value, const at::Tensor& k_cache,
@@ -384,5 +478,6 @@ PYBIND11_MODULE(_pa_ext, m) {
       .def_readonly("refs", &PagePool::refs_)
       .def_readonly("free_words", &PagePool::words_)
       .def_readonly("status", &PagePool::status_);
+  m.def("prompt", &prompt, "prompt attention over paged caches (see prompt.py)");
   m.def("decode", &decode, "one paged-attention decode step (see torch_kernel.py)");
 }

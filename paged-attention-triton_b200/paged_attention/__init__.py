@@ -15,6 +15,7 @@ from .torch_kernel import (  # noqa: F401
 )
 from .graph_runner import PagedAttnGraphRunner  # noqa: F401
 from .cache_ops import write_kv_cache, slots_for_positions  # noqa: F401
+from .prompt import paged_prompt_attention  # noqa: F401
 from .page_pool import PagePool  # noqa: F401
 from .split_kv_kernel import LSE_SENTINEL, LSE_VALID_THRESHOLD  # noqa: F401
 

@@ -126,6 +126,48 @@ class PlanInfo(ctypes.Structure):
     ]
 
 
+class PromptParams(ctypes.Structure):
+    """Mirror of ``pa_prompt_params``."""
+
+    _fields_ = [
+        ("q", ctypes.c_void_p),
+        ("q_stride_t", ctypes.c_int64),
+        ("q_stride_h", ctypes.c_int64),
+        ("k_cache", ctypes.c_void_p),
+        ("k_stride_block", ctypes.c_int64),
+        ("k_stride_slot", ctypes.c_int64),
+        ("k_stride_head", ctypes.c_int64),
+        ("v_cache", ctypes.c_void_p),
+        ("v_stride_block", ctypes.c_int64),
+        ("v_stride_slot", ctypes.c_int64),
+        ("v_stride_head", ctypes.c_int64),
+        ("block_table", ctypes.c_void_p),
+        ("bt_stride_b", ctypes.c_int64),
+        ("max_blocks", ctypes.c_int32),
+        ("query_starts", ctypes.c_void_p),
+        ("seq_lens", ctypes.c_void_p),
+        ("num_tokens", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("num_heads", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("block_size", ctypes.c_int32),
+        ("num_blocks", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("num_sinks", ctypes.c_int32),
+        ("scale", ctypes.c_float),
+        ("dtype", ctypes.c_int32),
+        ("out", ctypes.c_void_p),
+        ("out_stride_t", ctypes.c_int64),
+        ("out_stride_h", ctypes.c_int64),
+        ("lse", ctypes.c_void_p),
+        ("num_splits", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+        ("status", ctypes.c_void_p),
+    ]
+
+
 class PagePoolParams(ctypes.Structure):
     """Mirror of ``pa_page_pool``."""
 
@@ -165,6 +207,9 @@ _SIGNATURES = {
     "pa_window_decode": (ctypes.c_int, [ctypes.POINTER(DecodeParams), ctypes.c_int32,
                                         ctypes.c_int32, ctypes.c_void_p]),
     "pa_cache_append": (ctypes.c_int, [ctypes.POINTER(AppendParams), ctypes.c_void_p]),
+    "pa_prompt_workspace": (ctypes.c_int, [ctypes.POINTER(PromptParams),
+                                           ctypes.POINTER(ctypes.c_size_t)]),
+    "pa_prompt": (ctypes.c_int, [ctypes.POINTER(PromptParams), ctypes.c_void_p]),
     "pa_pages_scratch": (ctypes.c_int, [ctypes.POINTER(PagePoolParams), ctypes.c_int32,
                                         ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
     "pa_pages_resize": (ctypes.c_int, [ctypes.POINTER(PagePoolParams), ctypes.c_void_p,

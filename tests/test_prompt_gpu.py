@@ -1,0 +1,293 @@
+"""GPU tests of prompt attention (``paged_prompt_attention``) against the definition in
+64 bits, over caches whose invisible slots are NaN and whose invisible pages are not
+there."""
+import ctypes
+
+import pytest
+import torch
+
+from window_helpers import PoisonedCache, assert_lse, assert_matches, reference
+
+pytestmark = pytest.mark.gpu
+
+
+def _starts(qs):
+    out = [0]
+    for n in qs:
+        out.append(out[-1] + n)
+    return out
+
+
+def _tolerance(q, tol, want_abs_v):
+    """The definition's tolerance, with probabilities rounded once to the 16-bit type
+    (half a step, relative) before the product with V: at most that times max|v|."""
+    return tol + torch.finfo(q.dtype).eps / 2 * want_abs_v
+
+
+def _run(qs, lens, hq, hkv, d, bs, dtype, window, sinks, seed, pad=0, **kw):
+    import paged_attention as pa
+    full = window is None
+    win = 10 ** 9 if full else window
+    c = PoisonedCache(lens, qs, hkv, d, bs, dtype, win, sinks, seed)
+    g = torch.Generator().manual_seed(seed + 1)
+    starts = _starts(qs)
+    q = torch.randn(starts[-1] + pad, hq, d, generator=g).to(dtype).cuda()
+    ws = pa.DecodeWorkspace("cuda")
+    out = torch.full_like(q, 7.0)
+    st = torch.tensor(starts, dtype=torch.int32, device="cuda")
+    o, lse = pa.paged_prompt_attention(q, c.k, c.v, c.table, st, c.lens, bs, window=window,
+                                       num_sinks=sinks, return_lse=True, workspace=ws, out=out,
+                                       **kw)
+    torch.cuda.synchronize()
+    assert ws.read_status() == 0
+    want, wl, tol = reference(q, c.k, c.v, c.table, lens, bs, win, sinks, starts)
+    n = starts[-1]
+    vmax = c.v[~c.v.isnan()].abs().max().double().item() if (~c.v.isnan()).any() else 0.0
+    what = f"{dtype} q{qs} s{lens} w{window} k{sinks} d{d} bs{bs} hq{hq}/{hkv} {kw}"
+    assert_matches(o[:n], want[:n], _tolerance(q, tol, vmax)[:n], what)
+    assert_lse(lse[:n], wl[:n], d, what)
+    assert (o[n:] == 7).all(), "rows behind the last sequence"
+    return c, q, st, o, lse
+
+
+SHAPES = [(2, 4, 128, 16), (3, 1, 64, 32), (1, 8, 128, 16), (1, 3, 128, 8), (1, 2, 256, 16),
+          (2, 5, 64, 64), (1, 2, 32, 16), (1, 2, 64, 1), (1, 4, 128, 24), (1, 2, 256, 128),
+          (1, 1, 128, 12), (1, 16, 64, 8), (1, 2, 128, 256)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (1, 0), (1, 3), (37, 5), (128, 4), (200, 140)])
+@pytest.mark.parametrize("hkv,g,d,bs", SHAPES)
+def test_prompt_small(dtype, window, sinks, hkv, g, d, bs):
+    """Chunks of 0 to 100 tokens at the start, in the middle and at the end of sequences."""
+    qs = [1, 0, 5, 33, 17, 100, 0, 2]
+    lens = [1, 9, 300, 33, 146, 129, 0, 513]
+    _run(qs, lens, hkv * g, hkv, d, bs, dtype, window, sinks, seed=d + bs + g, pad=3)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hkv,g,d,bs", [(1, 4, 128, 16), (2, 1, 64, 32), (1, 2, 256, 16)])
+@pytest.mark.parametrize("qs,lens,window,sinks", [
+    ([300], [300], None, 0),
+    ([257, 128], [700, 128], 130, 4),
+    ([256, 64, 65], [256, 1000, 1025], 256, 1),
+    ([600], [900], 64, 300),
+])
+def test_prompt_several_tiles(dtype, hkv, g, d, bs, qs, lens, window, sinks):
+    _run(qs, lens, hkv * g, hkv, d, bs, dtype, window, sinks, seed=sum(qs))
+
+
+@pytest.mark.parametrize("splits", [1, 2, 3, 7, 40])
+@pytest.mark.parametrize("window,sinks", [(None, 0), (500, 4)])
+def test_prompt_splits(splits, window, sinks):
+    """The keys in parts that a second kernel joins; more parts than tiles too."""
+    _run([7, 1, 0, 40], [1500, 1, 30, 640], 8, 2, 128, 16, torch.bfloat16, window, sinks,
+         seed=splits, pad=2, num_splits=splits)
+    _run([3, 20], [999, 2000], 4, 4, 64, 16, torch.float16, window, sinks, seed=splits,
+         num_splits=splits)
+    _run([3], [400], 4, 2, 256, 32, torch.float16, window, sinks, seed=splits, num_splits=splits)
+
+
+def test_prompt_rows_before_the_sequence_see_nothing():
+    """A chunk longer than its sequence: its first rows sit before position 0."""
+    for d, bs in ((128, 16), (32, 16)):
+        c, q, st, o, lse = _run([40, 9], [25, 0], 4, 2, d, bs, torch.float16, 8, 2, seed=4)
+        assert (o[:15] == 0).all() and (lse[:15] == -1e30).all()
+        assert (o[40:49] == 0).all() and (lse[40:49] == -1e30).all()
+
+
+def test_prompt_of_one_token_is_decode():
+    import paged_attention as pa
+    lens, window, sinks = [1, 40, 700, 64], 100, 4
+    c, q, st, o, lse = _run([1] * 4, lens, 8, 2, 128, 16, torch.bfloat16, window, sinks, seed=2)
+    d, dl = pa.paged_attention(q, c.k, c.v, c.table, c.lens, 16, window=window, num_sinks=sinks,
+                               return_lse=True)
+    # probabilities rounded to 8 bits here and to 16 there
+    assert_matches(o, d.double().cpu(), 2 * 2.0 ** -8 * c.v[~c.v.isnan()].abs().max().double().cpu()
+                   * torch.ones(d.shape, dtype=torch.float64), "prompt against decode")
+    assert_lse(lse, dl.double().cpu(), 128, "prompt against decode")
+
+
+def test_prompt_strided_inputs():
+    """K and V as slices of one buffer, a q that is a slice of a fused projection."""
+    import paged_attention as pa
+    qs, lens, bs, hkv, g, d, window, sinks = [50, 9], [200, 77], 16, 2, 4, 128, 60, 4
+    c = PoisonedCache(lens, qs, hkv, d, bs, torch.float16, window, sinks, 3)
+    kv = torch.stack([c.k, c.v], 1)
+    fused = torch.randn(59, hkv * g + 2 * hkv, d, device="cuda").half()
+    q = fused[:, : hkv * g]
+    st = torch.tensor(_starts(qs), dtype=torch.int32, device="cuda")
+    out = torch.empty(hkv * g, 59, d, device="cuda").half().transpose(0, 1)
+    o = pa.paged_prompt_attention(q, kv[:, 0], kv[:, 1], c.table, st, c.lens, bs, window=window,
+                                  num_sinks=sinks, out=out)
+    want, _, tol = reference(q, c.k, c.v, c.table, lens, bs, window, sinks, _starts(qs))
+    vmax = c.v[~c.v.isnan()].abs().max().double().item()
+    assert o.data_ptr() == out.data_ptr()
+    assert_matches(o, want, _tolerance(q, tol, vmax), "strided")
+
+
+def test_prompt_large_scores_and_scale():
+    """Scores in the hundreds, a running maximum that keeps growing, a given scale."""
+    import paged_attention as pa
+    qs, lens, bs, d = [64], [1024], 16, 128
+    for dtype in (torch.float16, torch.bfloat16):
+        c = PoisonedCache(lens, qs, 1, d, bs, dtype, 10 ** 9, 0, 5)
+        ramp = torch.arange(1024, device="cuda") / 64.0
+        page, slot = c.table[0, torch.arange(1024) // bs].long(), torch.arange(1024, device="cuda") % bs
+        c.k[page, slot] = (c.k[page, slot].float() * ramp[:, None, None]).to(dtype)
+        q = torch.randn(64, 4, d, device="cuda").to(dtype)
+        st = torch.tensor([0, 64], dtype=torch.int32, device="cuda")
+        o, lse = pa.paged_prompt_attention(q, c.k, c.v, c.table, st, c.lens, bs, scale=0.5,
+                                           return_lse=True)
+        want, wl, tol = reference(q, c.k, c.v, c.table, lens, bs, 10 ** 9, 0, [0, 64], scale=0.5)
+        vmax = c.v[~c.v.isnan()].abs().max().double().item()
+        assert_matches(o, want, _tolerance(q, tol, vmax), f"ramp {dtype}")
+
+
+def test_prompt_captured_and_replayed_follows_lengths():
+    import paged_attention as pa
+    bs, hkv, g, d, window, sinks = 16, 2, 4, 128, 90, 4
+    ws = pa.DecodeWorkspace("cuda")
+    width, pool = 40, 128
+    kk = torch.full((pool, bs, hkv, d), float("nan"), device="cuda").half()
+    vv = kk.clone()
+    table = torch.full((3, width), -1, dtype=torch.int32, device="cuda")
+    st = torch.zeros(4, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(3, dtype=torch.int32, device="cuda")
+    q = torch.randn(64, hkv * g, d, device="cuda").half()
+    out = torch.zeros_like(q)
+
+    def call():
+        pa.paged_prompt_attention(q, kk, vv, table, st, lens, bs, window=window, num_sinks=sinks,
+                                  workspace=ws, out=out)
+
+    call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call()
+    for seed, (qs, ls) in enumerate([([20, 0, 44], [600, 3, 50]), ([1, 1, 1], [300, 640, 1]),
+                                     ([64, 0, 0], [64, 0, 10])]):
+        c = PoisonedCache(ls, qs, hkv, d, bs, torch.float16, window, sinks, seed, width=width)
+        kk.fill_(float("nan"))
+        vv.fill_(float("nan"))
+        kk[: c.k.shape[0]], vv[: c.v.shape[0]] = c.k, c.v
+        table.copy_(c.table)
+        lens.copy_(c.lens)
+        starts = _starts(qs)
+        st.copy_(torch.tensor(starts, dtype=torch.int32))
+        out.fill_(7)
+        graph.replay()
+        want, _, tol = reference(q, c.k, c.v, c.table, ls, bs, window, sinks, starts)
+        vmax = c.v[~c.v.isnan()].abs().max().double().item()
+        n = starts[-1]
+        assert_matches(out[:n], want[:n], _tolerance(q, tol, vmax)[:n], f"replay {seed}")
+        assert (out[n:] == 7).all()
+
+
+def test_prompt_same_bits_on_every_run_and_stream():
+    c, q, st, o, lse = _run([300, 20], [900, 40], 8, 2, 128, 16, torch.bfloat16, 500, 4, seed=8)
+    import paged_attention as pa
+    side = torch.cuda.Stream()
+    for _ in range(3):
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.default_stream())
+            o2, lse2 = pa.paged_prompt_attention(q, c.k, c.v, c.table, st, c.lens, 16, window=500,
+                                                 num_sinks=4, return_lse=True)
+        side.synchronize()
+        assert torch.equal(o, o2) and torch.equal(lse, lse2)
+
+
+def test_prompt_flags_bad_pages_lengths_and_starts():
+    import paged_attention as pa
+    from paged_attention import _native
+    for d, bs in ((64, 16), (32, 16)):
+        c = PoisonedCache([200, 100], [10, 10], 1, d, bs, torch.float16, 50, 4, 3)
+        q = torch.randn(20, 1, d, device="cuda").half()
+        st = torch.tensor([0, 10, 20], dtype=torch.int32, device="cuda")
+        ws = pa.DecodeWorkspace("cuda")
+
+        def call(starts=st):
+            pa.paged_prompt_attention(q, c.k, c.v, c.table, starts, c.lens, bs, window=50,
+                                      num_sinks=4, workspace=ws)
+            return ws.read_status()
+
+        c.table[0, 5] = 10 ** 6                  # tokens 80..95: no row sees them
+        assert call() == 0
+        c.table[0, 11] = 10 ** 6                 # tokens 176..191: visible
+        assert call() == _native.PA_STATUS_BAD_BLOCK
+        c.table[0, 11] = -5
+        ws.reset()
+        assert call() == _native.PA_STATUS_BAD_BLOCK
+        c.table[0, 11] = 0
+        ws.reset()
+        assert call(torch.tensor([0, 10, 21], dtype=torch.int32, device="cuda")) == \
+            _native.PA_STATUS_BAD_SEQLEN
+        ws.reset()
+        assert call(torch.tensor([5, 3, 20], dtype=torch.int32, device="cuda")) & \
+            _native.PA_STATUS_BAD_SEQLEN
+        ws.reset()
+        c.lens[1] = 10 ** 6
+        assert call() & _native.PA_STATUS_BAD_SEQLEN
+
+
+def test_prompt_empty_calls():
+    import paged_attention as pa
+    k = torch.zeros(4, 16, 2, 64, device="cuda", dtype=torch.float16)
+    q = torch.zeros(0, 4, 64, device="cuda", dtype=torch.float16)
+    bt = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    z = torch.zeros(3, dtype=torch.int32, device="cuda")
+    o, lse = pa.paged_prompt_attention(q, k, k, bt, z, z[:2], 16, return_lse=True)
+    assert o.shape == (0, 4, 64) and lse.shape == (0, 4)
+    q = torch.zeros(5, 4, 64, device="cuda", dtype=torch.float16)
+    out = torch.full_like(q, 3.0)
+    pa.paged_prompt_attention(q, k, k, bt, z, z[:2], 16, out=out)          # rows of no sequence
+    pa.paged_prompt_attention(q, k, k, bt[:0], z[:1], z[:0], 16, out=out)  # no sequence
+    assert (out == 3).all()
+
+
+def test_prompt_refusals_on_the_device():
+    import paged_attention as pa
+    k = torch.zeros(4, 16, 2, 64, device="cuda", dtype=torch.float16)
+    q = torch.zeros(5, 4, 64, device="cuda", dtype=torch.float16)
+    bt = torch.zeros(2, 3, dtype=torch.int32, device="cuda")
+    st = torch.zeros(3, dtype=torch.int32, device="cuda")
+    ok = dict(Q=q, K_Cache=k, V_Cache=k, Block_Table=bt, query_starts=st, seq_lens=st[:2], block_size=16)
+    for bad in (dict(K_Cache=k.bfloat16()), dict(V_Cache=k[:3]), dict(Q=q[..., :32]), dict(Q=q[:, :3]),
+                dict(Block_Table=bt.long()), dict(query_starts=st[:2]), dict(seq_lens=st),
+                dict(seq_lens=st[:2].long()), dict(block_size=8), dict(K_Cache=k.cpu()),
+                dict(Q=q.float(), K_Cache=k.float(), V_Cache=k.float()), dict(out=q[:4]),
+                dict(window=0), dict(num_sinks=1), dict(num_splits=0)):
+        with pytest.raises(ValueError):
+            pa.paged_prompt_attention(**{**ok, **bad})
+
+
+def test_prompt_through_ctypes():
+    from paged_attention import _native
+    qs, lens, bs, hkv, d, window, sinks = [30, 4], [200, 900], 16, 2, 128, 70, 4
+    c = PoisonedCache(lens, qs, hkv, d, bs, torch.bfloat16, window, sinks, 1)
+    q = torch.randn(34, 4 * hkv, d, device="cuda").bfloat16()
+    st = torch.tensor(_starts(qs), dtype=torch.int32, device="cuda")
+    out = torch.empty_like(q)
+    p = _native.PromptParams()
+    p.q, p.q_stride_t, p.q_stride_h = q.data_ptr(), q.stride(0), q.stride(1)
+    p.k_cache, p.v_cache = c.k.data_ptr(), c.v.data_ptr()
+    p.k_stride_block, p.k_stride_slot, p.k_stride_head = c.k.stride()[:3]
+    p.v_stride_block, p.v_stride_slot, p.v_stride_head = c.v.stride()[:3]
+    p.block_table, p.bt_stride_b, p.max_blocks = c.table.data_ptr(), c.table.stride(0), c.table.shape[1]
+    p.query_starts, p.seq_lens = st.data_ptr(), c.lens.data_ptr()
+    p.num_tokens, p.batch, p.num_heads, p.num_kv_heads, p.head_dim = 34, 2, 4 * hkv, hkv, d
+    p.block_size, p.num_blocks, p.window, p.num_sinks = bs, c.k.shape[0], window, sinks
+    p.scale, p.dtype = d ** -0.5, _native.PA_BF16
+    p.out, p.out_stride_t, p.out_stride_h = out.data_ptr(), out.stride(0), out.stride(1)
+    lib = _native.lib()
+    need = ctypes.c_size_t()
+    assert lib.pa_prompt_workspace(ctypes.byref(p), ctypes.byref(need)) == 0
+    if need.value:
+        assert lib.pa_prompt(ctypes.byref(p), None) == _native.PA_ERR_WORKSPACE
+    buf = torch.empty(max(16, need.value), dtype=torch.uint8, device="cuda")
+    p.workspace, p.workspace_bytes = buf.data_ptr(), need.value
+    assert lib.pa_prompt(ctypes.byref(p), torch.cuda.current_stream().cuda_stream) == 0
+    want, _, tol = reference(q, c.k, c.v, c.table, lens, bs, window, sinks, _starts(qs))
+    vmax = c.v[~c.v.isnan()].abs().max().double().item()
+    assert_matches(out, want, _tolerance(q, tol, vmax), "ctypes")
