@@ -19,7 +19,9 @@
 #include <string.h>
 
 #include <algorithm>
+#include <climits>
 #include <mutex>
+#include <type_traits>
 
 #include "pa_decode.h"
 #include "fastdiv.h"
@@ -197,6 +199,792 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
 }
 
 // ----------------------------------------------------------------------------
+// Tile path: tcgen05 over pages copied by TMA
+// ----------------------------------------------------------------------------
+// One CTA takes 128 * NQ packed query rows of one (sequence, KV head): row R is
+// token R / G, head R % G of the group, so that the G query heads that share the
+// keys share their tiles. It walks the tiles of kTN keys that any of its rows
+// sees: those that hold visible first tokens, then those from the window's
+// first token to the last row's position. Per tile and 128 rows:
+//
+//   S (128 x kTN, TMEM) = Q K^T       one tcgen05.mma per 16 dimensions
+//   P = 2^(c S - m), rounded to the 16-bit type, over S in TMEM
+//   O (128 x D, TMEM) += P V          one tcgen05.mma per 16 tokens
+//
+// Roles: a producer warp (lane = one TMA box of a page), a warp that issues the
+// matrix instructions, and four softmax warps per 128 rows, thread = row, so
+// that row maxima and sums need no exchange. With NQ = 2 the two row tiles
+// alternate on the matrix pipe: while one's S is turned into P, the other's
+// products run. With NQ = 1 (short chunks, head_dim 256) S has two buffers and
+// the next tile's S is computed during the current softmax.
+//
+// P is rounded to the operand type once (half a step, relative); its sum, the
+// maxima and O are kept in 32 bits. O is rescaled only when a row's maximum has
+// grown by more than 2^8: until then P and the sum are relative to an older
+// maximum, which changes neither's relative rounding (P <= 2^8).
+//
+// Masks: a tile that is not entirely visible to all rows of a warp compares
+// each score's token with the row's limits. Tokens that no row sees are cut off
+// in steps of 16 by the products' shape (N of the first, K of the second); the
+// V rows of such tokens inside the remaining steps are zeroed in
+// shared memory first, as 0 * NaN would reach O.
+template <int D, int NQ>
+struct TC {
+  static constexpr int kTN = D == 256 ? 64 : 128;      // keys per tile
+  static constexpr int kChunks = D / 64;               // 128-byte chunks of a row
+  static constexpr int kQTile = 128 * D * 2;
+  static constexpr int kKV = kTN * D * 2;              // one K or V tile
+  static constexpr int kSlots = D == 64 ? 8 : (D == 128 && NQ == 1) ? 6 : 5;
+  static constexpr int kSmem = NQ * kQTile + kSlots * kKV + 1024;
+  static constexpr int kSBufs = NQ == 2 ? 1 : 2;       // S buffers per row tile
+  static constexpr int kOCol = NQ * kSBufs * kTN;      // first TMEM column of O
+  static constexpr int kThreads = NQ * 128 + 64;
+  static_assert(kOCol + NQ * D <= 512, "tensor memory");
+  static_assert(kSmem <= 232448 - 1024, "shared memory");
+};
+constexpr int kTmemCols = 512;
+constexpr unsigned long long kWaitLimitNs = 2000000000ull;   // 2 s per barrier wait
+constexpr float kRescaleLog2 = 8.f;
+
+struct TileParams {
+  Params p;
+  int R, lR;                // token rows per TMA box: gcd(page, tile), and its log2
+  int bs_log2;              // log2 of the page size, or -1
+  FastDiv div_g, div_bs;
+  int splits;
+  float* o_part;            // [splits][T * Hq][D], splits > 1
+  float* lse_part;          // [splits][T * Hq]
+};
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+  return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
+  asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
+  asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok != 0;
+}
+__device__ __forceinline__ unsigned long long global_ns() {
+  unsigned long long t;
+  asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+  return t;
+}
+// Waits for the barrier's phase with a wall-clock bound; false on timeout.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = global_ns();
+  while (true) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (global_ns() - t0 > kWaitLimitNs) return false;
+  }
+}
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int c0, int c1,
+                                            int c2, int c3, int c4, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void fence_async_smem() {
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_before() {
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+// Arrival on the barrier once every matrix instruction issued so far is done.
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+               : "memory");
+}
+// D[tmem] (+)= A[smem] B[smem], and with A in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
+      : "memory");
+}
+// Shared-memory matrix descriptor, 128-byte swizzle: 8-row groups 1024 bytes
+// apart; `lead`: bytes between the 64-element blocks of an operand whose
+// contiguous dimension is not the summed one (V), unused otherwise.
+__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
+  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | static_cast<uint64_t>(lead >> 4) << 16 |
+         static_cast<uint64_t>(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+}
+// Instruction descriptor: 32-bit accumulator, A and B of type T, M = 128;
+// `b_mn`: B's contiguous dimension is N (V), else K.
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t instr_desc(int n, bool b_mn) {
+  const uint32_t ty = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return 1u << 4 | ty << 7 | ty << 10 | (b_mn ? 1u : 0u) << 16 |
+         static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 32 rows (lanes of the warp's quarter) x N columns of tensor memory, thread = row.
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(addr + 0)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[64]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%64];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%65];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]),
+        "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+        "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
+      : "r"(addr + 0), "r"(addr + 32)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld(uint32_t addr, uint32_t (&r)[128]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%128];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%32, %33, %34, %35, %36, %37, %38, %39, %40, %41, %42, %43, %44, %45, %46, %47, %48, %49, %50, %51, %52, %53, %54, %55, %56, %57, %58, %59, %60, %61, %62, %63}, [%129];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%64, %65, %66, %67, %68, %69, %70, %71, %72, %73, %74, %75, %76, %77, %78, %79, %80, %81, %82, %83, %84, %85, %86, %87, %88, %89, %90, %91, %92, %93, %94, %95}, [%130];\n\t"
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%96, %97, %98, %99, %100, %101, %102, %103, %104, %105, %106, %107, %108, %109, %110, %111, %112, %113, %114, %115, %116, %117, %118, %119, %120, %121, %122, %123, %124, %125, %126, %127}, [%131];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+        "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]),
+        "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]),
+        "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
+        "=r"(r[29]), "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]),
+        "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]), "=r"(r[40]), "=r"(r[41]), "=r"(r[42]),
+        "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+        "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]),
+        "=r"(r[57]), "=r"(r[58]), "=r"(r[59]), "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]),
+        "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]), "=r"(r[70]),
+        "=r"(r[71]), "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]),
+        "=r"(r[78]), "=r"(r[79]), "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]),
+        "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]), "=r"(r[90]), "=r"(r[91]),
+        "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]),
+        "=r"(r[99]), "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]),
+        "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]), "=r"(r[110]),
+        "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]),
+        "=r"(r[117]), "=r"(r[118]), "=r"(r[119]), "=r"(r[120]), "=r"(r[121]), "=r"(r[122]),
+        "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+      : "r"(addr + 0), "r"(addr + 32), "r"(addr + 64), "r"(addr + 96)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
+      :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+        "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+        "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+// A CTA's work: its rows and the key tiles they see.
+struct Job {
+  int b, kvh, split;
+  Seq s;
+  int r0, rows;             // first packed row, packed rows of the sequence
+  int low, hi;              // window: tokens [low, hi) are seen by some row
+  int first, nsink, sink_end;   // first window tile; sink tiles, of tokens [0, sink_end)
+  int sinks;
+  int k0, k1;               // tiles of this CTA
+};
+// First token; some row sees the tokens [from, to) of the tile. `gap`: except
+// [sinks, low), where the window's first tile holds the last sinks too.
+struct KeyTile { int base, from, to, gap; };
+template <int kTN>
+__device__ __forceinline__ KeyTile key_tile(const Job& j, int k) {
+  KeyTile t;
+  const bool sink = k < j.nsink;
+  t.base = (sink ? k : j.first + k - j.nsink) * kTN;
+  t.gap = !sink && t.base < j.sinks && t.base < j.low;
+  t.from = sink || t.gap ? t.base : max(t.base, j.low);
+  t.to = min(t.base + kTN, sink ? j.sink_end : j.hi);
+  return t;
+}
+
+// Whether some row sees a token of the box of R tokens from `tok` on (else its
+// page is not read).
+__device__ __forceinline__ bool box_seen(const Job& j, const KeyTile& t, int tok, int R) {
+  return tok < t.to && tok + R > t.from && !(t.gap && tok >= j.sinks && tok + R <= j.low);
+}
+
+// The job of block x, or false. Tiles are numbered from the last sequence's last
+// rows, which see the most keys under a causal mask, to the first ones.
+template <int D, int NQ>
+__device__ __forceinline__ bool find_job(const TileParams& a, Job& j, int* sh) {
+  constexpr int kRows = 128 * NQ, kTN = TC<D, NQ>::kTN;
+  const Params& p = a.p;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  const int per = p.Hkv * a.splits;
+  const int x = blockIdx.x / per;
+  const int rest = blockIdx.x - x * per;
+  // running sums over the sequences, from the last to the first
+  int before = 0;
+  if (threadIdx.x == 0) sh[32] = -1;
+  for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
+    const int b = p.B - 1 - (b0 + static_cast<int>(threadIdx.x));
+    int nt = 0;
+    bool bad = false;
+    if (b >= 0) nt = (load_seq(p, b, bad).n * p.G + kRows - 1) / kRows;
+    if (bad && blockIdx.x == 0) flag(p, PA_STATUS_BAD_SEQLEN);
+    int v = nt;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(kFull, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) sh[warp] = v;
+    __syncthreads();
+    int base = before, all = 0;
+    for (int w = 0; w < nw; ++w) {
+      if (w < warp) base += sh[w];
+      all += sh[w];
+    }
+    const int lo = base + v - nt;
+    if (x >= lo && x < lo + nt) {
+      sh[32] = b;
+      sh[33] = lo + nt - 1 - x;
+    }
+    before += all;
+    __syncthreads();
+    if (before > x && blockIdx.x) break;   // block 0 checks every sequence
+  }
+  const int b = sh[32];
+  if (b < 0) return false;
+  bool bad;
+  j.b = b;
+  j.s = load_seq(p, b, bad);
+  j.r0 = sh[33] * kRows;
+  j.rows = j.s.n * p.G;
+  j.kvh = rest / a.splits;
+  j.split = rest - j.kvh * a.splits;
+  const int pos0 = j.s.S - j.s.n;
+  const int last = min(j.r0 + kRows, j.rows) - 1;
+  const int pmin = pos0 + static_cast<int>(fast_div(j.r0, a.div_g));
+  j.hi = max(0, pos0 + static_cast<int>(fast_div(last, a.div_g)) + 1);
+  j.low = pmin >= p.window ? pmin - p.window + 1 : 0;
+  j.sinks = p.sinks;
+  j.first = j.low / kTN;
+  j.sink_end = min(p.sinks, j.first * kTN);
+  j.nsink = (j.sink_end + kTN - 1) / kTN;
+  const int tiles = j.hi > 0 ? j.nsink + (j.hi - 1) / kTN - j.first + 1 : 0;
+  j.k0 = static_cast<int>(static_cast<long long>(tiles) * j.split / a.splits);
+  j.k1 = static_cast<int>(static_cast<long long>(tiles) * (j.split + 1) / a.splits);
+  return true;
+}
+
+template <typename T, int D, int NQ>
+__global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
+    prompt_tile_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
+                       const TileParams a) {
+  using C = TC<D, NQ>;
+  constexpr int kTN = C::kTN;
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t bars[2 * C::kSlots + NQ * (3 + C::kSBufs) + 1];
+  __shared__ uint32_t s_tmem;
+  __shared__ int s_find[34];
+  const Params& p = a.p;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  Job j;
+  if (!find_job<D, NQ>(a, j, s_find)) return;   // the same answer in every thread
+
+  unsigned char* smem = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t sq = smem_u32(smem);
+  const uint32_t skv = sq + NQ * C::kQTile;
+  const uint32_t bar0 = smem_u32(bars);
+  auto kv_full = [&](int s) { return bar0 + s * 8; };
+  auto kv_empty = [&](int s) { return bar0 + (C::kSlots + s) * 8; };
+  auto q_full = [&](int t) { return bar0 + (2 * C::kSlots + t) * 8; };
+  auto p_full = [&](int t) { return bar0 + (2 * C::kSlots + NQ + t) * 8; };
+  auto o_done = [&](int t) { return bar0 + (2 * C::kSlots + 2 * NQ + t) * 8; };
+  auto s_full = [&](int i) { return bar0 + (2 * C::kSlots + 3 * NQ + i) * 8; };
+  const uint32_t drained = bar0 + (2 * C::kSlots + NQ * (3 + C::kSBufs)) * 8;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 2 * C::kSlots; ++s) mbar_init(bar0 + s * 8, 1);
+    for (int t = 0; t < NQ; ++t) {
+      mbar_init(q_full(t), 128);
+      mbar_init(p_full(t), 128);
+      mbar_init(o_done(t), 1);
+    }
+    for (int i = 0; i < NQ * C::kSBufs; ++i) mbar_init(s_full(i), 1);
+    mbar_init(drained, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == NQ * 4) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(&s_tmem)),
+                 "n"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem;
+  bool ok = true;
+
+  if (warp == NQ * 4 + 1) {
+    // ---------------------------------------------------------------- producer
+    // Lane = one box: R token rows of one 64-dim chunk.
+    const int box = lane / C::kChunks, chunk = lane - box * C::kChunks;
+    auto lookup = [&](int k, int& phys, int& slot) {
+      phys = INT_MIN;
+      slot = 0;
+      const KeyTile t = key_tile<kTN>(j, k);
+      const int tok = t.base + (box << a.lR);
+      if (box < (kTN >> a.lR) && box_seen(j, t, tok, a.R)) {
+        const int pg = a.bs_log2 >= 0 ? tok >> a.bs_log2 : static_cast<int>(fast_div(tok, a.div_bs));
+        slot = tok - pg * p.bs;
+        phys = __ldg(p.bt + j.b * p.bt_sb + pg);
+      }
+    };
+    int phys, slot, nphys = INT_MIN, nslot = 0, s = 0;
+    uint32_t phase = 0;
+    if (j.k0 < j.k1) lookup(j.k0, nphys, nslot);
+    for (int k = j.k0; k < j.k1 && ok; ++k) {
+      phys = nphys;
+      slot = nslot;
+      if (k + 1 < j.k1) lookup(k + 1, nphys, nslot);
+      bool valid = phys != INT_MIN;
+      if (valid && (phys < 0 || phys >= p.NB)) {
+        flag(p, PA_STATUS_BAD_BLOCK);
+        valid = false;
+      }
+      const uint32_t bytes = __popc(__ballot_sync(kFull, valid)) * a.R * 128;
+      for (int kv = 0; kv < 2; ++kv) {
+        ok = mbar_wait(kv_empty(s), phase ^ 1);
+        if (!__all_sync(kFull, ok)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) mbar_expect_tx(kv_full(s), bytes);
+        __syncwarp();
+        if (valid)
+          tma_load_5d(skv + s * C::kKV + chunk * kTN * 128 + (box << a.lR) * 128, kv ? &mv : &mk, 0,
+                      slot, chunk, j.kvh, phys, kv_full(s));
+        if (++s == C::kSlots) {
+          s = 0;
+          phase ^= 1;
+        }
+      }
+    }
+    if (!ok) {
+      // leave no copy in flight: every slot's last fill (a slot that was never
+      // filled passes as the phase before its first)
+      for (int i = 0; i < C::kSlots; ++i) mbar_wait(kv_full(i), i < s ? phase : phase ^ 1);
+    }
+  } else if (warp == NQ * 4) {
+    // ------------------------------------------------------- matrix instructions
+    int s = 0;
+    uint32_t phase = 0;
+    const int n = j.k1 - j.k0;
+    const bool lead = lane == 0;
+    constexpr uint32_t kDescPV = instr_desc<T>(D, true);
+    auto next_slot = [&]() {
+      if (++s == C::kSlots) {
+        s = 0;
+        phase ^= 1;
+      }
+    };
+    // S of row tile t, keys in slot ks, for tile k
+    auto issue_s = [&](int t, int buf, int ks, const KeyTile& kt) {
+      const uint32_t d = tmem + (t * C::kSBufs + buf) * kTN;
+      const uint32_t idesc = instr_desc<T>((kt.to - kt.base + 15) & ~15, false);
+      const uint32_t qa = sq + t * C::kQTile, kb = skv + ks * C::kKV;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint32_t in = (i & 3) * 32;
+        mma_ss(d, smem_desc(qa + (i >> 2) * 128 * 128 + in, 16),
+               smem_desc(kb + (i >> 2) * kTN * 128 + in, 16), idesc, i > 0);
+      }
+      tc_commit(s_full(t * C::kSBufs + buf));
+    };
+    // O of row tile t += P V, values in slot vs
+    auto issue_o = [&](int t, int buf, int vs, const KeyTile& kt, bool add) {
+      const uint32_t d = tmem + C::kOCol + t * D;
+      const uint32_t pa = tmem + (t * C::kSBufs + buf) * kTN;
+      const uint32_t vb = skv + vs * C::kKV;
+      const int i1 = (kt.to - kt.base + 15) >> 4;
+      for (int i = (kt.from - kt.base) >> 4; i < i1; ++i) {
+        mma_ts(d, pa + i * 8, smem_desc(vb + i * 16 * 128, kTN * 128), kDescPV, add);
+        add = true;
+      }
+    };
+    // V rows of the multiplied 16-token steps whose tokens no row sees become zero.
+    auto clean_v = [&](int vs, const KeyTile& kt) {
+      const int v0 = kt.from - kt.base, v1 = kt.to - kt.base;
+      const int c0 = v0 & ~15, c1 = (v1 + 15) & ~15;
+      if (!kt.gap && v0 == c0 && v1 == c1) return;
+      const int g0 = kt.gap ? j.sinks - kt.base : c1, g1 = kt.gap ? j.low - kt.base : c1;
+      for (int r = c0 + lane / (D / 8 < 32 ? D / 8 : 32); r < c1; r += D / 8 < 32 ? 32 / (D / 8) : 1) {
+        if (r >= v0 && r < v1 && !(r >= g0 && r < g1)) continue;
+        const int c = lane % (D / 8);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                         skv + vs * C::kKV + (c >> 3) * kTN * 128 + r * 128 + (c & 7) * 16),
+                     "r"(0)
+                     : "memory");
+      }
+      fence_async_smem();
+      __syncwarp();
+    };
+    auto wait = [&](uint32_t bar, uint32_t parity) {
+      if (ok) ok = __all_sync(kFull, mbar_wait(bar, parity));
+    };
+
+    if (n > 0) {
+      for (int t = 0; t < NQ; ++t) wait(q_full(t), 0);
+      wait(kv_full(s), phase);
+      tc_fence_after();
+      KeyTile cur = key_tile<kTN>(j, j.k0);
+      if (ok && lead) {
+        for (int t = 0; t < NQ; ++t) issue_s(t, 0, s, cur);
+        if (n > 1) tc_commit(kv_empty(s));
+      }
+      next_slot();
+      for (int i = 0; i < n && ok; ++i) {
+        const bool more = i + 1 < n;
+        const KeyTile nxt = key_tile<kTN>(j, j.k0 + i + (more ? 1 : 0));
+        const int vs = s;
+        const uint32_t vph = phase;
+        next_slot();
+        const int ks = s;
+        const uint32_t kph = phase;
+        if (more) next_slot();
+        if constexpr (NQ == 1) {
+          if (more) {   // the next tile's S, into the other buffer, during this softmax
+            wait(kv_full(ks), kph);
+            tc_fence_after();
+            if (ok && lead) {
+              issue_s(0, (i + 1) & 1, ks, nxt);
+              if (i + 2 < n) tc_commit(kv_empty(ks));
+            }
+          }
+          wait(kv_full(vs), vph);
+          if (!ok) break;
+          clean_v(vs, cur);
+          wait(p_full(0), i & 1);
+          tc_fence_after();
+          if (ok && lead) {
+            issue_o(0, i & 1, vs, cur, i > 0);
+            tc_commit(o_done(0));
+            if (more) tc_commit(kv_empty(vs));
+          }
+        } else {
+          wait(kv_full(vs), vph);
+          if (!ok) break;
+          clean_v(vs, cur);
+#pragma unroll
+          for (int t = 0; t < NQ; ++t) {
+            wait(p_full(t), i & 1);
+            tc_fence_after();
+            if (ok && lead) {
+              issue_o(t, 0, vs, cur, i > 0);
+              if (t == NQ - 1 && more) tc_commit(kv_empty(vs));
+              if (!more) tc_commit(o_done(t));
+            }
+            if (more) {
+              if (t == 0) {
+                wait(kv_full(ks), kph);
+                tc_fence_after();
+              }
+              if (ok && lead) {
+                issue_s(t, 0, ks, nxt);
+                if (t == NQ - 1 && i + 2 < n) tc_commit(kv_empty(ks));
+              }
+            }
+          }
+        }
+        cur = nxt;
+        __syncwarp();
+      }
+      if (!ok) {
+        if (lane == 0) {
+          flag(p, PA_STATUS_TIMEOUT);
+          tc_commit(drained);
+        }
+        mbar_wait(drained, 0);
+      }
+    }
+  } else {
+    // ----------------------------------------------------------------- softmax
+    const int t = warp >> 2;
+    const int tid = threadIdx.x & 127;
+    const int r0 = j.r0 + t * 128;
+    {
+      // the row tile into shared memory: 16-byte pieces, D/8 threads a row
+      constexpr int kPer = D / 8;
+      const int c = tid % kPer;
+#pragma unroll 4
+      for (int i = 0; i < kPer; ++i) {
+        const int r = i * (128 / kPer) + tid / kPer;
+        const int pr = r0 + r;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (pr < j.rows) {
+          const int tok = static_cast<int>(fast_div(pr, a.div_g));
+          v = __ldg(reinterpret_cast<const uint4*>(p.q + (j.s.start + tok) * p.q_st +
+                                                   (j.kvh * p.G + pr - tok * p.G) * p.q_sh) + c);
+        }
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                         sq + t * C::kQTile + (c >> 3) * 128 * 128 + r * 128 +
+                         (((c & 7) ^ (r & 7)) << 4)),
+                     "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                     : "memory");
+      }
+      fence_async_smem();
+      mbar_arrive(q_full(t));
+    }
+    const int pr = r0 + tid;
+    const bool live = pr < j.rows;
+    const int tok = live ? static_cast<int>(fast_div(pr, a.div_g)) : 0;
+    const int pos = j.s.S - j.s.n + tok;
+    // the row sees tokens t < hi with t >= low or t < sinks
+    const int hi = live ? max(pos + 1, 0) : 0;
+    const int low = pos >= p.window ? pos - p.window + 1 : 0;
+    const float scl = p.scale_log2;
+    const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;   // TMEM lane 32 * (warp % 4)
+    const uint32_t o_at = tmem + lanes + C::kOCol + t * D;
+    float m = -INFINITY, l = 0.f;
+    const int n = j.k1 - j.k0;
+    // NQ = 1: waits for the product of tile i - 1, once per tile and before tile i's
+    // P is handed over, so that no barrier here gets a phase ahead of its reader.
+    int waited = 0;
+    auto o_free = [&](int i) {
+      if (NQ == 2 || waited == i) return true;
+      ok = mbar_wait(o_done(t), (i - 1) & 1);
+      ok = __all_sync(kFull, ok);
+      tc_fence_after();
+      waited = i;
+      return ok;
+    };
+    for (int i = 0; i < n; ++i) {
+      const int buf = NQ == 1 ? (i & 1) : 0;
+      const uint32_t s_at = tmem + lanes + (t * C::kSBufs + buf) * kTN;
+      ok = mbar_wait(s_full(t * C::kSBufs + buf), NQ == 1 ? (i >> 1) & 1 : i & 1);
+      if (!__all_sync(kFull, ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int base = key_tile<kTN>(j, j.k0 + i).base;
+      uint32_t raw[kTN];
+      tmem_ld(s_at, raw);
+      float s[kTN];
+#pragma unroll
+      for (int c = 0; c < kTN; ++c) s[c] = __uint_as_float(raw[c]);
+      if (__any_sync(kFull, hi < base + kTN || low > base)) {
+        const int h = hi - base, lo = low - base, sk = p.sinks - base;
+#pragma unroll
+        for (int c = 0; c < kTN; ++c)
+          if (!(c < h && (c >= lo || c < sk))) s[c] = -INFINITY;
+      }
+      float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+      for (int c = 4; c < kTN; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
+      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      if (i == 0) {
+        m = top;
+      } else if (__any_sync(kFull, (top - m) * scl > kRescaleLog2)) {
+        // (the difference is NaN, not greater, while the row has seen nothing)
+        const float mn = fmaxf(m, top);
+        const float f = mn == -INFINITY ? 1.f : ex2((m - mn) * scl);
+        m = mn;
+        l *= f;
+        // O is free once the previous tile's product is done (with NQ = 2 the
+        // commit behind this tile's S covers it)
+        if (!o_free(i)) break;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          tmem_ld(o_at + c, o);
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st(o_at + c, o);
+        }
+      }
+      const float off = m == -INFINITY ? 0.f : -m * scl;
+      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int c0 = 0; c0 < kTN; c0 += 32) {
+        uint32_t pk[16];
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) {
+          const float x = ex2(fmaf(s[c0 + c], scl, off));
+          const float y = ex2(fmaf(s[c0 + c + 1], scl, off));
+          sum[c & 2] += x;
+          sum[(c & 2) + 1] += y;
+          pk[c / 2] = pack2<T>(x, y);
+        }
+        tmem_st(s_at + c0 / 2, pk);
+      }
+      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+      if (!o_free(i)) break;
+      tc_fence_before();
+      mbar_arrive(p_full(t));
+    }
+    if (n > 0 && ok) {
+      ok = mbar_wait(o_done(t), NQ == 1 ? (n - 1) & 1 : 0);
+      ok = __all_sync(kFull, ok);
+      tc_fence_after();
+    }
+    if (!ok) {
+      if (lane == 0) flag(p, PA_STATUS_TIMEOUT);
+    } else {
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float lse = l > 0.f ? (m * scl + log2f(l)) * kLn2 : kSentinel;
+      const int hq = j.kvh * p.G + pr - tok * p.G;
+      const long long at = static_cast<long long>(j.s.start + tok) * p.Hq + hq;
+      if (a.splits == 1) {
+        char* dst = p.out + (j.s.start + tok) * p.o_st + hq * p.o_sh;
+#pragma unroll 1
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          if (n > 0) {
+            tmem_ld(o_at + c, o);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0;
+          }
+          if (live) {
+#pragma unroll
+            for (int e = 0; e < 32; e += 8) {
+              uint32_t w[4];
+#pragma unroll
+              for (int x = 0; x < 4; ++x) {
+                // a row that saw nothing has zero products, and P = 0
+                w[x] = pack2<T>(__uint_as_float(o[e + 2 * x]) * inv,
+                                __uint_as_float(o[e + 2 * x + 1]) * inv);
+              }
+              *reinterpret_cast<uint4*>(dst + (c + e) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+        if (live && p.lse) p.lse[at] = lse;
+      } else {
+        const long long row = static_cast<long long>(j.split) * p.T * p.Hq + at;
+        if (n > 0) {
+          float* dst = a.o_part + row * D;
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            tmem_ld(o_at + c, o);
+            if (live) {
+#pragma unroll
+              for (int e = 0; e < 32; e += 4)
+                *reinterpret_cast<float4*>(dst + c + e) =
+                    make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                                __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+            }
+          }
+        }
+        if (live) a.lse_part[row] = n > 0 ? lse : kSentinel;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == NQ * 4)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemCols)
+                 : "memory");
+}
+
+// Joins the splits of a row: one warp per (row, query head), weights
+// 2^(lse - max) over the splits that saw a token.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) prompt_join_kernel(const TileParams a) {
+  constexpr int N = D / 32;
+  const Params& p = a.p;
+  const int lane = threadIdx.x & 31;
+  const long long w = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const long long rows = static_cast<long long>(p.T) * p.Hq;
+  if (w >= rows) return;
+  const int row = static_cast<int>(w / p.Hq);
+  const int hq = static_cast<int>(w - static_cast<long long>(row) * p.Hq);
+  int lo = 0, hi = p.B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (__ldg(p.starts + mid) <= row) lo = mid; else hi = mid - 1;
+  }
+  bool bad;
+  const Seq s = load_seq(p, lo, bad);
+  if (row < s.start || row >= s.start + s.n) return;
+  float top = kSentinel;
+  for (int k = lane; k < a.splits; k += 32) top = fmaxf(top, a.lse_part[k * rows + w]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
+  float sum = 0.f, acc[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) acc[i] = 0.f;
+  for (int k = 0; k < a.splits; ++k) {
+    const float l = a.lse_part[k * rows + w];
+    if (l <= -1e29f) continue;
+    const float f = exp2f((l - top) * kLog2e);
+    sum += f;
+    const float* src = a.o_part + (k * rows + w) * D + lane * N;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] = fmaf(f, src[i], acc[i]);
+  }
+  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + row * p.o_st + hq * p.o_sh + lane * N * 2);
+#pragma unroll
+  for (int i = 0; i < N / 2; ++i) dst[i] = pack2<T>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  if (lane == 0 && p.lse) p.lse[w] = sum > 0.f ? top + logf(sum) : kSentinel;
+}
+
+// ----------------------------------------------------------------------------
 // Host side
 // ----------------------------------------------------------------------------
 static bool aligned16(const void* ptr) { return (reinterpret_cast<uintptr_t>(ptr) & 15) == 0; }
@@ -285,6 +1073,124 @@ static cudaError_t launch_rows(const Params& a, int D, cudaStream_t stream) {
   return cudaGetLastError();
 }
 
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  return fn;
+}
+
+// A paged cache as (64 dims, slot, 64-dim chunk, head, page); a box is R token
+// rows of one chunk, 128-byte swizzled.
+static bool encode_map(CUtensorMap* map, const pa_prompt_params* p, const void* base,
+                       int64_t s_block, int64_t s_slot, int64_t s_head, int R) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const CUtensorMapDataType dt =
+      p->dtype == PA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(p->block_size),
+                              static_cast<cuuint64_t>(p->head_dim / 64),
+                              static_cast<cuuint64_t>(p->num_kv_heads),
+                              static_cast<cuuint64_t>(p->num_blocks)};
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(s_slot) * 2, 128,
+                                 static_cast<cuuint64_t>(s_head) * 2,
+                                 static_cast<cuuint64_t>(s_block) * 2};
+  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(R), 1, 1, 1};
+  const cuuint32_t step[5] = {1, 1, 1, 1, 1};
+  return fn(map, dt, 5, const_cast<void*>(base), dims, strides, box, step,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// How a call runs: the CUDA-core path, or row tiles of 128 * nq with the keys
+// in `splits` parts.
+struct Plan {
+  bool rows_path;
+  int nq, splits;
+  long long tiles;          // bound on the row tiles of a KV head
+  size_t ws_bytes;
+};
+static Plan make_plan(const pa_prompt_params* p, int sms) {
+  Plan pl = {};
+  pl.splits = 1;
+  pl.rows_path = p->head_dim == 32 || p->block_size % 8 != 0;
+  if (pl.rows_path) return pl;
+  const int g = p->num_heads / p->num_kv_heads;
+  const long long packed = static_cast<long long>(p->num_tokens) * g;   // rows of a KV head
+  // Two row tiles per CTA keep the matrix pipe busy; a batch whose sequences
+  // bring no more than one tile each would leave the second empty.
+  pl.nq = p->head_dim == 256 || packed <= 128ll * p->batch ? 1 : 2;
+  // sum over the sequences of ceil(rows / tile), whatever their shares are
+  pl.tiles = packed / (128 * pl.nq) + std::min<long long>(p->batch, p->num_tokens);
+  const long long ctas = pl.tiles * p->num_kv_heads;
+  if (p->num_splits > 0) {
+    pl.splits = p->num_splits;
+  } else {
+    // Few row tiles: as many parts as fill the SMs once, each of two or more key
+    // tiles (each part's partial costs a write, a read and the joining kernel).
+    const int tn = p->head_dim == 256 ? 64 : 128;
+    const long long cap = static_cast<long long>(p->max_blocks) * p->block_size;
+    const long long span = 128ll * pl.nq / g + 1;
+    const long long seen =
+        p->window ? std::min(cap, static_cast<long long>(p->window) + span + p->num_sinks + tn) : cap;
+    const long long by_keys = (seen + tn - 1) / tn / 2;
+    pl.splits = static_cast<int>(std::max(1ll, std::min({static_cast<long long>(sms) / ctas, by_keys, 64ll})));
+  }
+  if (pl.splits > 1)
+    pl.ws_bytes = static_cast<size_t>(pl.splits) * p->num_tokens * p->num_heads *
+                  (p->head_dim + 1) * sizeof(float);
+  return pl;
+}
+
+template <typename T, int D, int NQ>
+static cudaError_t launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams& a,
+                                const Plan& pl, cudaStream_t stream) {
+  using C = TC<D, NQ>;
+  static std::mutex mu;
+  static bool set[64] = {false};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || dev >= 64) return cudaErrorInvalidDevice;
+  {
+    std::lock_guard<std::mutex> lk(mu);
+    if (!set[dev]) {
+      e = cudaFuncSetAttribute(prompt_tile_kernel<T, D, NQ>,
+                               cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+      if (e != cudaSuccess) return e;
+      set[dev] = true;
+    }
+  }
+  const long long grid = pl.tiles * a.p.Hkv * pl.splits;
+  if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
+  prompt_tile_kernel<T, D, NQ>
+      <<<static_cast<unsigned>(grid), C::kThreads, C::kSmem, stream>>>(mk, mv, a);
+  e = cudaGetLastError();
+  if (e == cudaSuccess && pl.splits > 1) {
+    const long long warps = static_cast<long long>(a.p.T) * a.p.Hq;
+    prompt_join_kernel<T, D><<<static_cast<unsigned>((warps + 3) / 4), 128, 0, stream>>>(a);
+    e = cudaGetLastError();
+  }
+  return e;
+}
+
+template <typename T>
+static cudaError_t launch_tiles_d(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams& a,
+                                  const Plan& pl, int D, cudaStream_t stream) {
+  if (D == 256) return launch_tiles<T, 256, 1>(mk, mv, a, pl, stream);
+  if (D == 128)
+    return pl.nq == 2 ? launch_tiles<T, 128, 2>(mk, mv, a, pl, stream)
+                      : launch_tiles<T, 128, 1>(mk, mv, a, pl, stream);
+  return pl.nq == 2 ? launch_tiles<T, 64, 2>(mk, mv, a, pl, stream)
+                    : launch_tiles<T, 64, 1>(mk, mv, a, pl, stream);
+}
+
 }  // namespace pp
 
 using namespace pp;
@@ -294,7 +1200,13 @@ extern "C" {
 pa_status_t pa_prompt_workspace(const pa_prompt_params* p, size_t* workspace_bytes) {
   const pa_status_t v = validate(p);
   if (v != PA_OK) return v;
-  if (workspace_bytes) *workspace_bytes = 0;
+  size_t bytes = 0;
+  if (p->num_tokens > 0 && p->batch > 0) {
+    const int sms = pa_device_sm_count();
+    if (sms <= 0) return PA_ERR_LAUNCH;
+    bytes = make_plan(p, sms).ws_bytes;
+  }
+  if (workspace_bytes) *workspace_bytes = bytes;
   return PA_OK;
 }
 
@@ -304,9 +1216,40 @@ pa_status_t pa_prompt(const pa_prompt_params* p, cudaStream_t stream) {
   if (p->num_tokens == 0 || p->batch == 0) return PA_OK;
   v = validate_launch(p);
   if (v != PA_OK) return v;
-  const Params a = make_params(p);
-  const cudaError_t e = p->dtype == PA_F16 ? launch_rows<__half>(a, p->head_dim, stream)
-                                           : launch_rows<__nv_bfloat16>(a, p->head_dim, stream);
+  const int sms = pa_device_sm_count();
+  if (sms <= 0) return PA_ERR_LAUNCH;
+  const Plan pl = make_plan(p, sms);
+  if (pl.ws_bytes && (pl.ws_bytes > p->workspace_bytes || !p->workspace)) return PA_ERR_WORKSPACE;
+  if (!aligned16(p->workspace)) return PA_ERR_ARG;
+  const bool half = p->dtype == PA_F16;
+  TileParams a;
+  memset(&a, 0, sizeof(a));
+  a.p = make_params(p);
+  cudaError_t e;
+  if (pl.rows_path) {
+    e = half ? launch_rows<__half>(a.p, p->head_dim, stream)
+             : launch_rows<__nv_bfloat16>(a.p, p->head_dim, stream);
+    return e == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
+  }
+  const int tn = p->head_dim == 256 ? 64 : 128;
+  a.R = 8;                                   // the largest power of two in both
+  while (a.R < tn && p->block_size % (2 * a.R) == 0) a.R *= 2;
+  a.lR = 0;
+  while ((1 << a.lR) < a.R) ++a.lR;
+  a.bs_log2 = -1;
+  for (int k = 0; k < 31; ++k)
+    if ((1 << k) == p->block_size) a.bs_log2 = k;
+  a.div_g = make_fastdiv(static_cast<uint32_t>(a.p.G));
+  a.div_bs = make_fastdiv(static_cast<uint32_t>(p->block_size));
+  a.splits = pl.splits;
+  a.o_part = static_cast<float*>(p->workspace);
+  a.lse_part = a.o_part + static_cast<size_t>(pl.splits) * p->num_tokens * p->num_heads * p->head_dim;
+  CUtensorMap mk, mv;
+  if (!encode_map(&mk, p, p->k_cache, p->k_stride_block, p->k_stride_slot, p->k_stride_head, a.R) ||
+      !encode_map(&mv, p, p->v_cache, p->v_stride_block, p->v_stride_slot, p->v_stride_head, a.R))
+    return PA_ERR_ARG;
+  e = half ? launch_tiles_d<__half>(mk, mv, a, pl, p->head_dim, stream)
+           : launch_tiles_d<__nv_bfloat16>(mk, mv, a, pl, p->head_dim, stream);
   return e == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 }
 
