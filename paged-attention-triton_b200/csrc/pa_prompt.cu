@@ -238,13 +238,28 @@ struct TC {
   static constexpr int kSmem = NQ * kQTile + kSlots * kKV + 1024;
   static constexpr int kSBufs = NQ == 2 ? 1 : 2;       // S buffers per row tile
   static constexpr int kOCol = NQ * kSBufs * kTN;      // first TMEM column of O
-  static constexpr int kThreads = NQ * 128 + 64;
+  // NQ = 2: three full warpgroups, whose registers are split unevenly
+  static constexpr int kThreads = NQ == 2 ? 384 : NQ * 128 + 64;
   static_assert(kOCol + NQ * D <= 512, "tensor memory");
   static_assert(kSmem <= 232448 - 1024, "shared memory");
 };
 constexpr int kTmemCols = 512;
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;   // 2 s per barrier wait
 constexpr float kRescaleLog2 = 8.f;
+// Registers per thread of a 384-thread CTA: 168 at launch; the softmax
+// warpgroups take kSoftmaxRegs once the third has gone down to kIssueRegs. (At
+// 168 the softmax spills, and with shared memory full of tiles the spills miss
+// the first-level cache.)
+constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kIssueRegs = 72;
+static_assert(2 * kSoftmaxRegs + kIssueRegs <= 3 * kLaunchRegs, "register split");
+template <int N>
+__device__ __forceinline__ void regs_up() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_down() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
 
 struct TileParams {
   Params p;
@@ -304,6 +319,18 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
       : "memory");
 }
+// One lane of a converged warp. (A lane elected this way is known to be alone,
+// so that the matrix instructions behind the branch take their operands from
+// uniform registers directly.)
+__device__ __forceinline__ bool elect_one() {
+  uint32_t is;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(is));
+  return is != 0;
+}
 __device__ __forceinline__ void fence_async_smem() {
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
 }
@@ -316,6 +343,10 @@ __device__ __forceinline__ void tc_fence_after() {
 // Arrival on the barrier once every matrix instruction issued so far is done.
 __device__ __forceinline__ void tc_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+               : "memory");
+}
+__device__ __forceinline__ void tmem_free(uint32_t tmem) {
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemCols)
                : "memory");
 }
 // D[tmem] (+)= A[smem] B[smem], and with A in tensor memory.
@@ -347,6 +378,60 @@ __device__ __forceinline__ constexpr uint32_t instr_desc(int n, bool b_mn) {
   const uint32_t ty = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
   return 1u << 4 | ty << 7 | ty << 10 | (b_mn ? 1u : 0u) << 16 |
          static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
+}
+// Pairs of 32-bit floats in one register pair: one instruction for two elements.
+__device__ __forceinline__ uint64_t f2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void f2_split(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// (2^x, 2^y) on the FMA pipe, for a share of the exponentials (the special
+// function unit does 4 a cycle and quarter SM, the bound of the softmax): n =
+// the integer nearest to x, from the low bits of x + 1.5 * 2^23; 2^(x - n) by a
+// polynomial of degree 4 fitted to the least largest relative error on [-1/2,
+// 1/2] with its constant term held at 1 (2.9e-6 in 32-bit arithmetic; P is
+// rounded to 2^-9 or 2^-12 of it); n added to the exponent. x < 128. Arguments
+// up to -127 give 0 exactly, NaN gives infinity or NaN.
+__device__ __forceinline__ void ex2_pair_fma(uint64_t v, float& x, float& y) {
+  f2_split(v, x, y);
+  v = f2(max_nan(x, -127.f), max_nan(y, -127.f));
+  const float kRound = 12582912.f;
+  const uint64_t t = f2_add(v, f2(kRound, kRound));
+  const uint64_t n = f2_add(t, f2(-kRound, -kRound));
+  const uint64_t f = f2_fma(n, f2(-1.f, -1.f), v);
+  uint64_t r = f2(0.009582852013409138f, 0.009582852013409138f);
+  r = f2_fma(r, f, f2(0.055906426161527634f, 0.055906426161527634f));
+  r = f2_fma(r, f, f2(0.24024099111557007f, 0.24024099111557007f));
+  r = f2_fma(r, f, f2(0.6931241750717163f, 0.6931241750717163f));
+  r = f2_fma(r, f, f2(1.f, 1.f));
+  float tx, ty;
+  f2_split(t, tx, ty);
+  f2_split(r, x, y);
+  x = __uint_as_float(__float_as_uint(x) + (__float_as_uint(tx) << 23));
+  y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -530,14 +615,11 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
   using C = TC<D, NQ>;
   constexpr int kTN = C::kTN;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * C::kSlots + NQ * (3 + C::kSBufs) + 1];
+  __shared__ __align__(8) uint64_t bars[2 * C::kSlots + NQ * (4 + C::kSBufs) + 1];
   __shared__ uint32_t s_tmem;
   __shared__ int s_find[34];
   const Params& p = a.p;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-
-  Job j;
-  if (!find_job<D, NQ>(a, j, s_find)) return;   // the same answer in every thread
 
   unsigned char* smem = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -547,15 +629,16 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
   auto kv_full = [&](int s) { return bar0 + s * 8; };
   auto kv_empty = [&](int s) { return bar0 + (C::kSlots + s) * 8; };
   auto q_full = [&](int t) { return bar0 + (2 * C::kSlots + t) * 8; };
-  auto p_full = [&](int t) { return bar0 + (2 * C::kSlots + NQ + t) * 8; };
-  auto o_done = [&](int t) { return bar0 + (2 * C::kSlots + 2 * NQ + t) * 8; };
-  auto s_full = [&](int i) { return bar0 + (2 * C::kSlots + 3 * NQ + i) * 8; };
-  const uint32_t drained = bar0 + (2 * C::kSlots + NQ * (3 + C::kSBufs)) * 8;
+  auto p_full = [&](int t, int half) { return bar0 + (2 * C::kSlots + NQ + 2 * t + half) * 8; };
+  auto o_done = [&](int t) { return bar0 + (2 * C::kSlots + 3 * NQ + t) * 8; };
+  auto s_full = [&](int i) { return bar0 + (2 * C::kSlots + 4 * NQ + i) * 8; };
+  const uint32_t drained = bar0 + (2 * C::kSlots + NQ * (4 + C::kSBufs)) * 8;
   if (threadIdx.x == 0) {
     for (int s = 0; s < 2 * C::kSlots; ++s) mbar_init(bar0 + s * 8, 1);
     for (int t = 0; t < NQ; ++t) {
       mbar_init(q_full(t), 128);
-      mbar_init(p_full(t), 128);
+      mbar_init(p_full(t, 0), 128);
+      mbar_init(p_full(t, 1), 128);
       mbar_init(o_done(t), 1);
     }
     for (int i = 0; i < NQ * C::kSBufs; ++i) mbar_init(s_full(i), 1);
@@ -570,11 +653,19 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
+  Job j;
+  const bool found = find_job<D, NQ>(a, j, s_find);   // the same answer in every thread
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
+  if (!found) {
+    if (warp == NQ * 4) tmem_free(tmem);
+    return;
+  }
   bool ok = true;
 
+  if (warp >= NQ * 4) {
+    if constexpr (NQ == 2) regs_down<kIssueRegs>();
   if (warp == NQ * 4 + 1) {
     // ---------------------------------------------------------------- producer
     // Lane = one box: R token rows of one 64-dim chunk.
@@ -625,12 +716,12 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       // filled passes as the phase before its first)
       for (int i = 0; i < C::kSlots; ++i) mbar_wait(kv_full(i), i < s ? phase : phase ^ 1);
     }
-  } else if (warp == NQ * 4) {
+  }
+  if (warp == NQ * 4) {
     // ------------------------------------------------------- matrix instructions
     int s = 0;
     uint32_t phase = 0;
     const int n = j.k1 - j.k0;
-    const bool lead = lane == 0;
     constexpr uint32_t kDescPV = instr_desc<T>(D, true);
     auto next_slot = [&]() {
       if (++s == C::kSlots) {
@@ -638,28 +729,39 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
         phase ^= 1;
       }
     };
-    // S of row tile t, keys in slot ks, for tile k
+    // Descriptors advance by adding to their address field (16-byte units): one
+    // thread issues 16 matrix instructions per 2 x 64 x 16 cycles of their work,
+    // so few instructions may stand between them (with descriptors rebuilt for
+    // each in a loop, a tile's pair of products took 2180 cycles instead of ~1100).
+    const uint64_t q_desc = smem_desc(sq, 16), k_desc = smem_desc(skv, 16);
+    const uint64_t v_desc = smem_desc(skv, kTN * 128);
+    // S of row tile t, keys in slot ks
     auto issue_s = [&](int t, int buf, int ks, const KeyTile& kt) {
       const uint32_t d = tmem + (t * C::kSBufs + buf) * kTN;
       const uint32_t idesc = instr_desc<T>((kt.to - kt.base + 15) & ~15, false);
-      const uint32_t qa = sq + t * C::kQTile, kb = skv + ks * C::kKV;
+      const uint64_t qa = q_desc + t * (C::kQTile >> 4), kb = k_desc + ks * (C::kKV >> 4);
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint32_t in = (i & 3) * 32;
-        mma_ss(d, smem_desc(qa + (i >> 2) * 128 * 128 + in, 16),
-               smem_desc(kb + (i >> 2) * kTN * 128 + in, 16), idesc, i > 0);
-      }
+      for (int i = 0; i < D / 16; ++i)
+        mma_ss(d, qa + ((i >> 2) * 128 * 128 + (i & 3) * 32) / 16,
+               kb + ((i >> 2) * kTN * 128 + (i & 3) * 32) / 16, idesc, i > 0);
       tc_commit(s_full(t * C::kSBufs + buf));
     };
-    // O of row tile t += P V, values in slot vs
-    auto issue_o = [&](int t, int buf, int vs, const KeyTile& kt, bool add) {
+    // O of row tile t += P V over one half of the tile's 16-token steps
+    auto issue_o = [&](int t, int buf, int vs, const KeyTile& kt, int half, bool add) {
+      constexpr int kHalf = kTN / 32;
       const uint32_t d = tmem + C::kOCol + t * D;
       const uint32_t pa = tmem + (t * C::kSBufs + buf) * kTN;
-      const uint32_t vb = skv + vs * C::kKV;
-      const int i1 = (kt.to - kt.base + 15) >> 4;
-      for (int i = (kt.from - kt.base) >> 4; i < i1; ++i) {
-        mma_ts(d, pa + i * 8, smem_desc(vb + i * 16 * 128, kTN * 128), kDescPV, add);
-        add = true;
+      const uint64_t vb = v_desc + vs * (C::kKV >> 4);
+      const int i0 = (kt.from - kt.base) >> 4, i1 = (kt.to - kt.base + 15) >> 4;
+      if (i0 == 0 && i1 == kTN / 16) {
+#pragma unroll
+        for (int i = 0; i < kHalf; ++i)
+          mma_ts(d, pa + (half * kHalf + i) * 8, vb + (half * kHalf + i) * (16 * 128 / 16), kDescPV,
+                 i > 0 || half || add);
+      } else {
+        const int e = min(i1, (half + 1) * kHalf);
+        for (int i = max(i0, half * kHalf); i < e; ++i)
+          mma_ts(d, pa + i * 8, vb + i * (16 * 128 / 16), kDescPV, i > i0 || add);
       }
     };
     // V rows of the multiplied 16-token steps whose tokens no row sees become zero.
@@ -688,7 +790,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       wait(kv_full(s), phase);
       tc_fence_after();
       KeyTile cur = key_tile<kTN>(j, j.k0);
-      if (ok && lead) {
+      if (ok && elect_one()) {
         for (int t = 0; t < NQ; ++t) issue_s(t, 0, s, cur);
         if (n > 1) tc_commit(kv_empty(s));
       }
@@ -706,7 +808,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
           if (more) {   // the next tile's S, into the other buffer, during this softmax
             wait(kv_full(ks), kph);
             tc_fence_after();
-            if (ok && lead) {
+            if (ok && elect_one()) {
               issue_s(0, (i + 1) & 1, ks, nxt);
               if (i + 2 < n) tc_commit(kv_empty(ks));
             }
@@ -714,10 +816,13 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
           wait(kv_full(vs), vph);
           if (!ok) break;
           clean_v(vs, cur);
-          wait(p_full(0), i & 1);
+          wait(p_full(0, 0), i & 1);
           tc_fence_after();
-          if (ok && lead) {
-            issue_o(0, i & 1, vs, cur, i > 0);
+          if (ok && elect_one()) issue_o(0, i & 1, vs, cur, 0, i > 0);
+          wait(p_full(0, 1), i & 1);
+          tc_fence_after();
+          if (ok && elect_one()) {
+            issue_o(0, i & 1, vs, cur, 1, i > 0);
             tc_commit(o_done(0));
             if (more) tc_commit(kv_empty(vs));
           }
@@ -727,10 +832,13 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
           clean_v(vs, cur);
 #pragma unroll
           for (int t = 0; t < NQ; ++t) {
-            wait(p_full(t), i & 1);
+            wait(p_full(t, 0), i & 1);
             tc_fence_after();
-            if (ok && lead) {
-              issue_o(t, 0, vs, cur, i > 0);
+            if (ok && elect_one()) issue_o(t, 0, vs, cur, 0, i > 0);
+            wait(p_full(t, 1), i & 1);
+            tc_fence_after();
+            if (ok && elect_one()) {
+              issue_o(t, 0, vs, cur, 1, i > 0);
               if (t == NQ - 1 && more) tc_commit(kv_empty(vs));
               if (!more) tc_commit(o_done(t));
             }
@@ -739,7 +847,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
                 wait(kv_full(ks), kph);
                 tc_fence_after();
               }
-              if (ok && lead) {
+              if (ok && elect_one()) {
                 issue_s(t, 0, ks, nxt);
                 if (t == NQ - 1 && i + 2 < n) tc_commit(kv_empty(ks));
               }
@@ -750,15 +858,17 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
         __syncwarp();
       }
       if (!ok) {
-        if (lane == 0) {
+        if (elect_one()) {
           flag(p, PA_STATUS_TIMEOUT);
           tc_commit(drained);
         }
         mbar_wait(drained, 0);
       }
     }
+  }
   } else {
     // ----------------------------------------------------------------- softmax
+    if constexpr (NQ == 2) regs_up<kSoftmaxRegs>();
     const int t = warp >> 2;
     const int tid = threadIdx.x & 127;
     const int r0 = j.r0 + t * 128;
@@ -766,21 +876,29 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       // the row tile into shared memory: 16-byte pieces, D/8 threads a row
       constexpr int kPer = D / 8;
       const int c = tid % kPer;
-#pragma unroll 4
-      for (int i = 0; i < kPer; ++i) {
-        const int r = i * (128 / kPer) + tid / kPer;
-        const int pr = r0 + r;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (pr < j.rows) {
-          const int tok = static_cast<int>(fast_div(pr, a.div_g));
-          v = __ldg(reinterpret_cast<const uint4*>(p.q + (j.s.start + tok) * p.q_st +
-                                                   (j.kvh * p.G + pr - tok * p.G) * p.q_sh) + c);
+#pragma unroll
+      for (int i0 = 0; i0 < kPer; i0 += 16) {
+        constexpr int kFly = kPer < 16 ? kPer : 16;     // loads in flight per thread
+        uint4 v[kFly];
+#pragma unroll
+        for (int i = 0; i < kFly; ++i) {
+          const int pr = r0 + (i0 + i) * (128 / kPer) + tid / kPer;
+          v[i] = make_uint4(0, 0, 0, 0);
+          if (pr < j.rows) {
+            const int tok = static_cast<int>(fast_div(pr, a.div_g));
+            v[i] = __ldg(reinterpret_cast<const uint4*>(p.q + (j.s.start + tok) * p.q_st +
+                                                        (j.kvh * p.G + pr - tok * p.G) * p.q_sh) + c);
+          }
         }
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                         sq + t * C::kQTile + (c >> 3) * 128 * 128 + r * 128 +
-                         (((c & 7) ^ (r & 7)) << 4)),
-                     "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
-                     : "memory");
+#pragma unroll
+        for (int i = 0; i < kFly; ++i) {
+          const int r = (i0 + i) * (128 / kPer) + tid / kPer;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                           sq + t * C::kQTile + (c >> 3) * 128 * 128 + r * 128 +
+                           (((c & 7) ^ (r & 7)) << 4)),
+                       "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
+                       : "memory");
+        }
       }
       fence_async_smem();
       mbar_arrive(q_full(t));
@@ -831,8 +949,12 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       }
       float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-      for (int c = 4; c < kTN; ++c) mx[c & 3] = fmaxf(mx[c & 3], s[c]);
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+      for (int c = 4; c + 7 < kTN; c += 8) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + 2 * e], s[c + 2 * e + 1]);
+      }
+      const float top = max3(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]),
+                             max3(fmaxf(s[kTN - 4], s[kTN - 3]), s[kTN - 2], s[kTN - 1]));
       if (i == 0) {
         m = top;
       } else if (__any_sync(kFull, (top - m) * scl > kRescaleLog2)) {
@@ -854,25 +976,45 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
         }
       }
       const float off = m == -INFINITY ? 0.f : -m * scl;
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t scl2 = f2(scl, scl), off2 = f2(off, off);
+      uint64_t sum[2] = {f2(0.f, 0.f), f2(0.f, 0.f)};
+      bool stop = false;
 #pragma unroll
-      for (int c0 = 0; c0 < kTN; c0 += 32) {
-        uint32_t pk[16];
+      for (int half = 0; half < 2; ++half) {
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) {
-          const float x = ex2(fmaf(s[c0 + c], scl, off));
-          const float y = ex2(fmaf(s[c0 + c + 1], scl, off));
-          sum[c & 2] += x;
-          sum[(c & 2) + 1] += y;
-          pk[c / 2] = pack2<T>(x, y);
+        for (int c0 = half * (kTN / 2); c0 < (half + 1) * (kTN / 2); c0 += 32) {
+          uint32_t pk[16];
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            const uint64_t v = f2_fma(f2(s[c0 + c], s[c0 + c + 1]), scl2, off2);
+            float x, y;
+            // 3 of 8 pairs on the FMA pipe
+            if ((c & 15) == 4 || (c & 15) == 10 || (c & 15) == 14) {
+              ex2_pair_fma(v, x, y);
+            } else {
+              f2_split(v, x, y);
+              x = ex2(x);
+              y = ex2(y);
+            }
+            sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2(x, y));
+            pk[c / 2] = pack2<T>(x, y);
+          }
+          tmem_st(s_at + c0 / 2, pk);
         }
-        tmem_st(s_at + c0 / 2, pk);
+        asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+        if (half == 0 && !o_free(i)) {
+          stop = true;
+          break;
+        }
+        // the first half's product may start while the second half is formed
+        tc_fence_before();
+        mbar_arrive(p_full(t, half));
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-      if (!o_free(i)) break;
-      tc_fence_before();
-      mbar_arrive(p_full(t));
+      if (stop) break;
+      float x0, x1, x2, x3;
+      f2_split(sum[0], x0, x1);
+      f2_split(sum[1], x2, x3);
+      l += (x0 + x1) + (x2 + x3);
     }
     if (n > 0 && ok) {
       ok = mbar_wait(o_done(t), NQ == 1 ? (n - 1) & 1 : 0);
@@ -887,7 +1029,10 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       const int hq = j.kvh * p.G + pr - tok * p.G;
       const long long at = static_cast<long long>(j.s.start + tok) * p.Hq + hq;
       if (a.splits == 1) {
-        char* dst = p.out + (j.s.start + tok) * p.o_st + hq * p.o_sh;
+        // Through shared memory (the row tile's queries are no longer needed), so that
+        // whole rows leave in one piece: 16-byte pieces, XOR-spread over the banks.
+        constexpr int kPer = D / 8;
+        const uint32_t so = sq + t * C::kQTile;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
           uint32_t o[32];
@@ -897,18 +1042,33 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = 0;
           }
-          if (live) {
 #pragma unroll
-            for (int e = 0; e < 32; e += 8) {
-              uint32_t w[4];
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t w[4];
 #pragma unroll
-              for (int x = 0; x < 4; ++x) {
-                // a row that saw nothing has zero products, and P = 0
-                w[x] = pack2<T>(__uint_as_float(o[e + 2 * x]) * inv,
-                                __uint_as_float(o[e + 2 * x + 1]) * inv);
-              }
-              *reinterpret_cast<uint4*>(dst + (c + e) * 2) = make_uint4(w[0], w[1], w[2], w[3]);
-            }
+            for (int x = 0; x < 4; ++x)
+              w[x] = pack2<T>(__uint_as_float(o[e + 2 * x]) * inv,
+                              __uint_as_float(o[e + 2 * x + 1]) * inv);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
+                             so + tid * (D * 2) + ((((c + e) >> 3) ^ (tid & 7)) << 4)),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+          }
+        }
+        asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
+        const int c = tid % kPer;
+#pragma unroll 4
+        for (int i = 0; i < kPer; ++i) {
+          const int r = i * (128 / kPer) + tid / kPer;
+          const int q = r0 + r;
+          if (q < j.rows) {
+            const int qt = static_cast<int>(fast_div(q, a.div_g));
+            uint4 v;
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                         : "r"(so + r * (D * 2) + ((c ^ (r & 7)) << 4)));
+            *(reinterpret_cast<uint4*>(p.out + (j.s.start + qt) * p.o_st +
+                                       (j.kvh * p.G + q - qt * p.G) * p.o_sh) + c) = v;
           }
         }
         if (live && p.lse) p.lse[at] = lse;
@@ -936,9 +1096,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == NQ * 4)
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemCols)
-                 : "memory");
+  if (warp == NQ * 4) tmem_free(tmem);
 }
 
 // Joins the splits of a row: one warp per (row, query head), weights
