@@ -877,29 +877,22 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       constexpr int kPer = D / 8;
       const int c = tid % kPer;
 #pragma unroll
-      for (int i0 = 0; i0 < kPer; i0 += 16) {
-        constexpr int kFly = kPer < 16 ? kPer : 16;     // loads in flight per thread
-        uint4 v[kFly];
-#pragma unroll
-        for (int i = 0; i < kFly; ++i) {
-          const int pr = r0 + (i0 + i) * (128 / kPer) + tid / kPer;
-          v[i] = make_uint4(0, 0, 0, 0);
-          if (pr < j.rows) {
-            const int tok = static_cast<int>(fast_div(pr, a.div_g));
-            v[i] = __ldg(reinterpret_cast<const uint4*>(p.q + (j.s.start + tok) * p.q_st +
-                                                        (j.kvh * p.G + pr - tok * p.G) * p.q_sh) + c);
-          }
-        }
-#pragma unroll
-        for (int i = 0; i < kFly; ++i) {
-          const int r = (i0 + i) * (128 / kPer) + tid / kPer;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(
-                           sq + t * C::kQTile + (c >> 3) * 128 * 128 + r * 128 +
-                           (((c & 7) ^ (r & 7)) << 4)),
-                       "r"(v[i].x), "r"(v[i].y), "r"(v[i].z), "r"(v[i].w)
-                       : "memory");
-        }
+      for (int i = 0; i < kPer; ++i) {
+        const int r = i * (128 / kPer) + tid / kPer;
+        const int pr = r0 + r;
+        const bool in = pr < j.rows;
+        const int tok = in ? static_cast<int>(fast_div(pr, a.div_g)) : 0;
+        const char* src = in ? p.q + (j.s.start + tok) * p.q_st + (j.kvh * p.G + pr - tok * p.G) * p.q_sh + c * 16
+                             : p.q;
+        // asynchronous, past the first-level cache (which shared memory leaves
+        // smaller than the tile); rows behind the sequence become zero
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                         sq + t * C::kQTile + (c >> 3) * 128 * 128 + r * 128 +
+                         (((c & 7) ^ (r & 7)) << 4)),
+                     "l"(src), "r"(in ? 16 : 0)
+                     : "memory");
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
       fence_async_smem();
       mbar_arrive(q_full(t));
     }
