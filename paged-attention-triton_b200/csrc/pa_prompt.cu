@@ -211,9 +211,10 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
 //   P = 2^(c S - m), rounded to the 16-bit type, over S in TMEM
 //   O (128 x D, TMEM) += P V          one tcgen05.mma per 16 tokens
 //
-// Roles: a producer warp (lane = one TMA box of a page), a warp that issues the
-// matrix instructions, and four softmax warps per 128 rows, thread = row, so
-// that row maxima and sums need no exchange. With NQ = 2 the two row tiles
+// Roles: a producer warp (lane = one TMA box of a page), a warp that cleans V
+// tiles at the edges of what is visible, one issuing warp per 128 rows, and four
+// softmax warps per 128 rows, thread = row, so that row maxima and sums need no
+// exchange. With NQ = 2 the two row tiles
 // alternate on the matrix pipe: while one's S is turned into P, the other's
 // products run. With NQ = 1 (short chunks, head_dim 256) S has two buffers and
 // the next tile's S is computed during the current softmax.
@@ -238,8 +239,13 @@ struct TC {
   static constexpr int kSmem = NQ * kQTile + kSlots * kKV + 1024;
   static constexpr int kSBufs = NQ == 2 ? 1 : 2;       // S buffers per row tile
   static constexpr int kOCol = NQ * kSBufs * kTN;      // first TMEM column of O
-  // NQ = 2: three full warpgroups, whose registers are split unevenly
-  static constexpr int kThreads = NQ == 2 ? 384 : NQ * 128 + 64;
+  // softmax warps, NQ issuing warps, the producer and the cleaner; NQ = 2: three
+  // full warpgroups, whose registers are split unevenly
+  static constexpr int kThreads = NQ * 128 + (NQ + 2) * 32;
+  // V tiles handed on by the cleaner, at most one ring of them ahead
+  static constexpr int kVBars = 4;
+  static_assert(2 * kVBars >= kSlots, "V barriers");
+  static constexpr int kBars = 2 * kSlots + kVBars + NQ * (5 + kSBufs);
   static_assert(kOCol + NQ * D <= 512, "tensor memory");
   static_assert(kSmem <= 232448 - 1024, "shared memory");
 };
@@ -349,27 +355,31 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemCols)
                : "memory");
 }
-// D[tmem] (+)= A[smem] B[smem], and with A in tensor memory.
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(static_cast<uint32_t>(add))
-      : "memory");
-}
 // Shared-memory matrix descriptor, 128-byte swizzle: 8-row groups 1024 bytes
 // apart; `lead`: bytes between the 64-element blocks of an operand whose
-// contiguous dimension is not the summed one (V), unused otherwise.
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lead) {
-  return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | static_cast<uint64_t>(lead >> 4) << 16 |
-         static_cast<uint64_t>(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
+// contiguous dimension is not the summed one (V), unused otherwise. The high
+// word is the same for every operand here; advancing by b bytes adds b / 16 to
+// the low one.
+constexpr uint32_t kDescHigh = 1024 >> 4 | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint32_t smem_desc(uint32_t addr, uint32_t lead) {
+  return (addr & 0x3ffff) >> 4 | (lead >> 4) << 16;
+}
+// D[tmem] (+)= A[smem] B[smem], and with A in tensor memory.
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 x, y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 x, {%1, %5};\n\tmov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], x, y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)), "n"(kDescHigh)
+      : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc, bool add) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 y;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "mov.b64 y, {%2, %5};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], y, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b), "r"(idesc), "r"(static_cast<uint32_t>(add)), "n"(kDescHigh)
+      : "memory");
 }
 // Instruction descriptor: 32-bit accumulator, A and B of type T, M = 128;
 // `b_mn`: B's contiguous dimension is N (V), else K.
@@ -615,7 +625,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
   using C = TC<D, NQ>;
   constexpr int kTN = C::kTN;
   extern __shared__ unsigned char smem_raw[];
-  __shared__ __align__(8) uint64_t bars[2 * C::kSlots + NQ * (4 + C::kSBufs) + 1];
+  __shared__ __align__(8) uint64_t bars[C::kBars];
   __shared__ uint32_t s_tmem;
   __shared__ int s_find[34];
   const Params& p = a.p;
@@ -628,21 +638,27 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
   const uint32_t bar0 = smem_u32(bars);
   auto kv_full = [&](int s) { return bar0 + s * 8; };
   auto kv_empty = [&](int s) { return bar0 + (C::kSlots + s) * 8; };
-  auto q_full = [&](int t) { return bar0 + (2 * C::kSlots + t) * 8; };
-  auto p_full = [&](int t, int half) { return bar0 + (2 * C::kSlots + NQ + 2 * t + half) * 8; };
-  auto o_done = [&](int t) { return bar0 + (2 * C::kSlots + 3 * NQ + t) * 8; };
-  auto s_full = [&](int i) { return bar0 + (2 * C::kSlots + 4 * NQ + i) * 8; };
-  const uint32_t drained = bar0 + (2 * C::kSlots + NQ * (4 + C::kSBufs)) * 8;
+  auto v_ready = [&](int i) { return bar0 + (2 * C::kSlots + i % C::kVBars) * 8; };   // i-th tile's
+  const uint32_t bar1 = bar0 + (2 * C::kSlots + C::kVBars) * 8;
+  auto q_full = [&](int t) { return bar1 + t * 8; };
+  auto o_done = [&](int t) { return bar1 + (NQ + t) * 8; };
+  auto drained = [&](int t) { return bar1 + (2 * NQ + t) * 8; };
+  auto p_full = [&](int t, int half) { return bar1 + (3 * NQ + 2 * t + half) * 8; };
+  auto s_full = [&](int i) { return bar1 + (5 * NQ + i) * 8; };
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 2 * C::kSlots; ++s) mbar_init(bar0 + s * 8, 1);
+    for (int s = 0; s < C::kSlots; ++s) {
+      mbar_init(kv_full(s), 1);
+      mbar_init(kv_empty(s), NQ);
+    }
+    for (int i = 0; i < C::kVBars; ++i) mbar_init(v_ready(i), 32);
     for (int t = 0; t < NQ; ++t) {
       mbar_init(q_full(t), 128);
       mbar_init(p_full(t, 0), 128);
       mbar_init(p_full(t, 1), 128);
       mbar_init(o_done(t), 1);
+      mbar_init(drained(t), 1);
     }
     for (int i = 0; i < NQ * C::kSBufs; ++i) mbar_init(s_full(i), 1);
-    mbar_init(drained, 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == NQ * 4) {
@@ -666,7 +682,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
 
   if (warp >= NQ * 4) {
     if constexpr (NQ == 2) regs_down<kIssueRegs>();
-  if (warp == NQ * 4 + 1) {
+  if (warp == NQ * 4 + NQ) {
     // ---------------------------------------------------------------- producer
     // Lane = one box: R token rows of one 64-dim chunk.
     const int box = lane / C::kChunks, chunk = lane - box * C::kChunks;
@@ -717,154 +733,139 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       for (int i = 0; i < C::kSlots; ++i) mbar_wait(kv_full(i), i < s ? phase : phase ^ 1);
     }
   }
-  if (warp == NQ * 4) {
-    // ------------------------------------------------------- matrix instructions
+  if (warp == NQ * 4 + NQ + 1) {
+    // ----------------------------------------------------------------- cleaner
+    // Hands each V tile on to the issuing warps, after zeroing the rows of its
+    // multiplied 16-token steps whose tokens no row sees.
     int s = 0;
     uint32_t phase = 0;
-    const int n = j.k1 - j.k0;
-    constexpr uint32_t kDescPV = instr_desc<T>(D, true);
-    auto next_slot = [&]() {
+    for (int k = j.k0; k < j.k1; ++k) {
+      if (++s == C::kSlots) {      // past the K tile
+        s = 0;
+        phase ^= 1;
+      }
+      ok = __all_sync(kFull, mbar_wait(kv_full(s), phase));
+      if (!ok) break;
+      const KeyTile kt = key_tile<kTN>(j, k);
+      const int v0 = kt.from - kt.base, v1 = kt.to - kt.base;
+      const int c0 = v0 & ~15, c1 = (v1 + 15) & ~15;
+      if (kt.gap || v0 != c0 || v1 != c1) {
+        constexpr int kRowsAtOnce = D / 8 < 32 ? 32 / (D / 8) : 1;
+        const int g0 = kt.gap ? j.sinks - kt.base : c1, g1 = kt.gap ? j.low - kt.base : c1;
+        const int c = lane % (D / 8);
+        for (int r = c0 + lane / (D / 8); r < c1; r += kRowsAtOnce) {
+          if (r >= v0 && r < v1 && !(r >= g0 && r < g1)) continue;
+          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                           skv + s * C::kKV + (c >> 3) * kTN * 128 + r * 128 + (c & 7) * 16),
+                       "r"(0)
+                       : "memory");
+        }
+        fence_async_smem();
+      }
+      mbar_arrive(v_ready(k - j.k0));
       if (++s == C::kSlots) {
         s = 0;
         phase ^= 1;
       }
-    };
-    // Descriptors advance by adding to their address field (16-byte units): one
-    // thread issues 16 matrix instructions per 2 x 64 x 16 cycles of their work,
-    // so few instructions may stand between them (with descriptors rebuilt for
-    // each in a loop, a tile's pair of products took 2180 cycles instead of ~1100).
-    const uint64_t q_desc = smem_desc(sq, 16), k_desc = smem_desc(skv, 16);
-    const uint64_t v_desc = smem_desc(skv, kTN * 128);
-    // S of row tile t, keys in slot ks
-    auto issue_s = [&](int t, int buf, int ks, const KeyTile& kt) {
-      const uint32_t d = tmem + (t * C::kSBufs + buf) * kTN;
-      const uint32_t idesc = instr_desc<T>((kt.to - kt.base + 15) & ~15, false);
-      const uint64_t qa = q_desc + t * (C::kQTile >> 4), kb = k_desc + ks * (C::kKV >> 4);
+    }
+    if (!ok && lane == 0) flag(p, PA_STATUS_TIMEOUT);
+  }
+  if (warp < NQ * 4 + NQ) {
+    // -------------------------------------------------------------- issuing warps
+    // One lane per row tile issues its products. What it runs between them
+    // bounds the kernel (the softmax warps take most issue slots: a wait on a
+    // barrier that is already complete costs ~100-200 cycles, a matrix
+    // instruction of 64 cycles' work ~70): with one warp for both row tiles, whole-
+    // warp waits and descriptors rebuilt per instruction, 8192 tokens, window
+    // 4096, Hq32/Hkv8 took 417 us. So: a warp per row tile, a single lane, the
+    // next keys' wait ahead of P's, no wait between the two products.
+    if (elect_one()) {
+      const int t = warp - NQ * 4;
+      const int n = j.k1 - j.k0;
+      constexpr uint32_t kDescPV = instr_desc<T>(D, true);
+      constexpr uint32_t kStep = C::kKV >> 4;
+      const uint32_t q_desc = smem_desc(sq + t * C::kQTile, 16);
+      const uint32_t k_desc = smem_desc(skv, 16);
+      const uint32_t v_desc = smem_desc(skv, kTN * 128);
+      const uint32_t o_col = tmem + C::kOCol + t * D;
+      const uint32_t s_col = tmem + t * C::kSBufs * kTN;
+      // S from the keys in slot ks
+      auto issue_s = [&](int buf, int ks, const KeyTile& kt) {
+        const uint32_t idesc = instr_desc<T>((kt.to - kt.base + 15) & ~15, false);
+        const uint32_t kb = k_desc + ks * kStep;
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i)
-        mma_ss(d, qa + ((i >> 2) * 128 * 128 + (i & 3) * 32) / 16,
-               kb + ((i >> 2) * kTN * 128 + (i & 3) * 32) / 16, idesc, i > 0);
-      tc_commit(s_full(t * C::kSBufs + buf));
-    };
-    // O of row tile t += P V over one half of the tile's 16-token steps
-    auto issue_o = [&](int t, int buf, int vs, const KeyTile& kt, int half, bool add) {
-      constexpr int kHalf = kTN / 32;
-      const uint32_t d = tmem + C::kOCol + t * D;
-      const uint32_t pa = tmem + (t * C::kSBufs + buf) * kTN;
-      const uint64_t vb = v_desc + vs * (C::kKV >> 4);
-      const int i0 = (kt.from - kt.base) >> 4, i1 = (kt.to - kt.base + 15) >> 4;
-      if (i0 == 0 && i1 == kTN / 16) {
+        for (int i = 0; i < D / 16; ++i)
+          mma_ss(s_col + buf * kTN, q_desc + ((i >> 2) * 128 * 128 + (i & 3) * 32) / 16,
+                 kb + ((i >> 2) * kTN * 128 + (i & 3) * 32) / 16, idesc, i > 0);
+        tc_commit(s_full(t * C::kSBufs + buf));
+      };
+      // O += P V over one half of the tile's 16-token steps, values in slot vs
+      auto issue_o = [&](int buf, int vs, const KeyTile& kt, int half, bool add) {
+        constexpr int kHalf = kTN / 32;
+        const uint32_t pa = s_col + buf * kTN;
+        const uint32_t vb = v_desc + vs * kStep;
+        const int i0 = (kt.from - kt.base) >> 4, i1 = (kt.to - kt.base + 15) >> 4;
+        if (i0 == 0 && i1 == kTN / 16) {
 #pragma unroll
-        for (int i = 0; i < kHalf; ++i)
-          mma_ts(d, pa + (half * kHalf + i) * 8, vb + (half * kHalf + i) * (16 * 128 / 16), kDescPV,
-                 i > 0 || half || add);
-      } else {
-        const int e = min(i1, (half + 1) * kHalf);
-        for (int i = max(i0, half * kHalf); i < e; ++i)
-          mma_ts(d, pa + i * 8, vb + i * (16 * 128 / 16), kDescPV, i > i0 || add);
-      }
-    };
-    // V rows of the multiplied 16-token steps whose tokens no row sees become zero.
-    auto clean_v = [&](int vs, const KeyTile& kt) {
-      const int v0 = kt.from - kt.base, v1 = kt.to - kt.base;
-      const int c0 = v0 & ~15, c1 = (v1 + 15) & ~15;
-      if (!kt.gap && v0 == c0 && v1 == c1) return;
-      const int g0 = kt.gap ? j.sinks - kt.base : c1, g1 = kt.gap ? j.low - kt.base : c1;
-      for (int r = c0 + lane / (D / 8 < 32 ? D / 8 : 32); r < c1; r += D / 8 < 32 ? 32 / (D / 8) : 1) {
-        if (r >= v0 && r < v1 && !(r >= g0 && r < g1)) continue;
-        const int c = lane % (D / 8);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                         skv + vs * C::kKV + (c >> 3) * kTN * 128 + r * 128 + (c & 7) * 16),
-                     "r"(0)
-                     : "memory");
-      }
-      fence_async_smem();
-      __syncwarp();
-    };
-    auto wait = [&](uint32_t bar, uint32_t parity) {
-      if (ok) ok = __all_sync(kFull, mbar_wait(bar, parity));
-    };
-
-    if (n > 0) {
-      for (int t = 0; t < NQ; ++t) wait(q_full(t), 0);
-      wait(kv_full(s), phase);
-      tc_fence_after();
+          for (int i = 0; i < kHalf; ++i)
+            mma_ts(o_col, pa + (half * kHalf + i) * 8, vb + (half * kHalf + i) * (16 * 128 / 16),
+                   kDescPV, i > 0 || half || add);
+        } else {
+          const int e = min(i1, (half + 1) * kHalf);
+          for (int i = max(i0, half * kHalf); i < e; ++i)
+            mma_ts(o_col, pa + i * 8, vb + i * (16 * 128 / 16), kDescPV, i > i0 || add);
+        }
+      };
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (ok) ok = mbar_wait(bar, parity);
+        return ok;
+      };
+      // Tile i's keys are fill 2 i of the ring, its values fill 2 i + 1.
+      int ks = 0, vs = 1;
+      uint32_t kph = 0;
       KeyTile cur = key_tile<kTN>(j, j.k0);
-      if (ok && elect_one()) {
-        for (int t = 0; t < NQ; ++t) issue_s(t, 0, s, cur);
-        if (n > 1) tc_commit(kv_empty(s));
+      if (n > 0 && wait(q_full(t), 0) && wait(kv_full(0), 0)) {
+        issue_s(0, 0, cur);
+        if (n > 1) tc_commit(kv_empty(0));
       }
-      next_slot();
       for (int i = 0; i < n && ok; ++i) {
         const bool more = i + 1 < n;
         const KeyTile nxt = key_tile<kTN>(j, j.k0 + i + (more ? 1 : 0));
-        const int vs = s;
-        const uint32_t vph = phase;
-        next_slot();
-        const int ks = s;
-        const uint32_t kph = phase;
-        if (more) next_slot();
-        if constexpr (NQ == 1) {
-          if (more) {   // the next tile's S, into the other buffer, during this softmax
-            wait(kv_full(ks), kph);
-            tc_fence_after();
-            if (ok && elect_one()) {
-              issue_s(0, (i + 1) & 1, ks, nxt);
-              if (i + 2 < n) tc_commit(kv_empty(ks));
-            }
-          }
-          wait(kv_full(vs), vph);
-          if (!ok) break;
-          clean_v(vs, cur);
-          wait(p_full(0, 0), i & 1);
-          tc_fence_after();
-          if (ok && elect_one()) issue_o(0, i & 1, vs, cur, 0, i > 0);
-          wait(p_full(0, 1), i & 1);
-          tc_fence_after();
-          if (ok && elect_one()) {
-            issue_o(0, i & 1, vs, cur, 1, i > 0);
-            tc_commit(o_done(0));
-            if (more) tc_commit(kv_empty(vs));
-          }
-        } else {
-          wait(kv_full(vs), vph);
-          if (!ok) break;
-          clean_v(vs, cur);
-#pragma unroll
-          for (int t = 0; t < NQ; ++t) {
-            wait(p_full(t, 0), i & 1);
-            tc_fence_after();
-            if (ok && elect_one()) issue_o(t, 0, vs, cur, 0, i > 0);
-            wait(p_full(t, 1), i & 1);
-            tc_fence_after();
-            if (ok && elect_one()) {
-              issue_o(t, 0, vs, cur, 1, i > 0);
-              if (t == NQ - 1 && more) tc_commit(kv_empty(vs));
-              if (!more) tc_commit(o_done(t));
-            }
-            if (more) {
-              if (t == 0) {
-                wait(kv_full(ks), kph);
-                tc_fence_after();
-              }
-              if (ok && elect_one()) {
-                issue_s(t, 0, ks, nxt);
-                if (t == NQ - 1 && i + 2 < n) tc_commit(kv_empty(ks));
-              }
-            }
-          }
+        ks += 2;
+        if (ks >= C::kSlots) {
+          ks -= C::kSlots;
+          kph ^= 1;
         }
+        if (more && !wait(kv_full(ks), kph)) break;
+        if (NQ == 1 && more) {
+          // the next tile's S, into the other buffer, during this tile's softmax
+          issue_s((i + 1) & 1, ks, nxt);
+          if (i + 2 < n) tc_commit(kv_empty(ks));
+        }
+        const int buf = NQ == 1 ? i & 1 : 0;
+        if (!wait(v_ready(i), i / C::kVBars & 1) || !wait(p_full(t, 0), i & 1)) break;
+        tc_fence_after();
+        issue_o(buf, vs, cur, 0, i > 0);
+        if (!wait(p_full(t, 1), i & 1)) break;
+        tc_fence_after();
+        issue_o(buf, vs, cur, 1, i > 0);
+        if (NQ == 1 || !more) tc_commit(o_done(t));
+        if (NQ == 2 && more) {
+          issue_s(0, ks, nxt);
+          if (i + 2 < n) tc_commit(kv_empty(ks));
+        }
+        if (more) tc_commit(kv_empty(vs));
+        vs += 2;
+        if (vs >= C::kSlots) vs -= C::kSlots;
         cur = nxt;
-        __syncwarp();
       }
       if (!ok) {
-        if (elect_one()) {
-          flag(p, PA_STATUS_TIMEOUT);
-          tc_commit(drained);
-        }
-        mbar_wait(drained, 0);
+        flag(p, PA_STATUS_TIMEOUT);
+        tc_commit(drained(t));
+        mbar_wait(drained(t), 0);
       }
     }
+    __syncwarp();
   }
   } else {
     // ----------------------------------------------------------------- softmax
