@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
 //   P = 2^(c S - m), rounded to the 16-bit type, over S in TMEM
 //   O (128 x D, TMEM) += P V          one tcgen05.mma per 16 tokens
 //
-// Roles: a producer warp (lane = one TMA box of a page), a warp that cleans V
+// Roles: producer warps (lane = one TMA box of a page), a warp that cleans V
 // tiles at the edges of what is visible, one issuing warp per 128 rows, and four
 // softmax warps per 128 rows, thread = row, so that row maxima and sums need no
 // exchange. With NQ = 2 the two row tiles
@@ -239,25 +239,26 @@ struct TC {
   static constexpr int kSmem = NQ * kQTile + kSlots * kKV + 1024;
   static constexpr int kSBufs = NQ == 2 ? 1 : 2;       // S buffers per row tile
   static constexpr int kOCol = NQ * kSBufs * kTN;      // first TMEM column of O
-  // softmax warps, NQ issuing warps, the producer and the cleaner; NQ = 2: three
-  // full warpgroups, whose registers are split unevenly
-  static constexpr int kThreads = NQ * 128 + (NQ + 2) * 32;
+  // warps: 4 softmax and one issuing warp per row tile, the producers, the cleaner;
+  // NQ = 2: four full warpgroups, whose registers are split unevenly
+  static constexpr int kProducers = NQ == 2 ? 4 : 2;
+  static constexpr int kThreads = NQ == 2 ? 512 : 128 + (1 + kProducers + 1) * 32;
   // V tiles handed on by the cleaner, at most one ring of them ahead
   static constexpr int kVBars = 4;
   static_assert(2 * kVBars >= kSlots, "V barriers");
-  static constexpr int kBars = 2 * kSlots + kVBars + NQ * (5 + kSBufs);
+  static constexpr int kBars = 2 * kSlots + kVBars + NQ * (7 + kSBufs);
   static_assert(kOCol + NQ * D <= 512, "tensor memory");
   static_assert(kSmem <= 232448 - 1024, "shared memory");
 };
 constexpr int kTmemCols = 512;
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;   // 2 s per barrier wait
 constexpr float kRescaleLog2 = 8.f;
-// Registers per thread of a 384-thread CTA: 168 at launch; the softmax
-// warpgroups take kSoftmaxRegs once the third has gone down to kIssueRegs. (At
-// 168 the softmax spills, and with shared memory full of tiles the spills miss
-// the first-level cache.)
-constexpr int kLaunchRegs = 168, kSoftmaxRegs = 216, kIssueRegs = 72;
-static_assert(2 * kSoftmaxRegs + kIssueRegs <= 3 * kLaunchRegs, "register split");
+// Registers per thread of a 512-thread CTA: 128 at launch; the two softmax
+// warpgroups take kSoftmaxRegs once the two others have gone down to kOtherRegs.
+// (At the launch's share the softmax spills, and with shared memory full of tiles
+// the spills miss the first-level cache.)
+constexpr int kLaunchRegs = 128, kSoftmaxRegs = 200, kOtherRegs = 56;
+static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * kLaunchRegs, "register split");
 template <int N>
 __device__ __forceinline__ void regs_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -389,7 +390,7 @@ __device__ __forceinline__ constexpr uint32_t instr_desc(int n, bool b_mn) {
   return 1u << 4 | ty << 7 | ty << 10 | (b_mn ? 1u : 0u) << 16 |
          static_cast<uint32_t>(n >> 3) << 17 | (128u >> 4) << 24;
 }
-// Pairs of 32-bit floats in one register pair: one instruction for two elements.
+// Pairs of 32-bit floats: one issue slot for two elements.
 __device__ __forceinline__ uint64_t f2(float x, float y) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
@@ -412,36 +413,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-// (2^x, 2^y) on the FMA pipe, for a share of the exponentials (the special
-// function unit does 4 a cycle and quarter SM, the bound of the softmax): n =
-// the integer nearest to x, from the low bits of x + 1.5 * 2^23; 2^(x - n) by a
-// polynomial of degree 4 fitted to the least largest relative error on [-1/2,
-// 1/2] with its constant term held at 1 (2.9e-6 in 32-bit arithmetic; P is
-// rounded to 2^-9 or 2^-12 of it); n added to the exponent. x < 128. Arguments
-// up to -127 give 0 exactly, NaN gives infinity or NaN.
-__device__ __forceinline__ void ex2_pair_fma(uint64_t v, float& x, float& y) {
-  f2_split(v, x, y);
-  v = f2(max_nan(x, -127.f), max_nan(y, -127.f));
-  const float kRound = 12582912.f;
-  const uint64_t t = f2_add(v, f2(kRound, kRound));
-  const uint64_t n = f2_add(t, f2(-kRound, -kRound));
-  const uint64_t f = f2_fma(n, f2(-1.f, -1.f), v);
-  uint64_t r = f2(0.009582852013409138f, 0.009582852013409138f);
-  r = f2_fma(r, f, f2(0.055906426161527634f, 0.055906426161527634f));
-  r = f2_fma(r, f, f2(0.24024099111557007f, 0.24024099111557007f));
-  r = f2_fma(r, f, f2(0.6931241750717163f, 0.6931241750717163f));
-  r = f2_fma(r, f, f2(1.f, 1.f));
-  float tx, ty;
-  f2_split(t, tx, ty);
-  f2_split(r, x, y);
-  x = __uint_as_float(__float_as_uint(x) + (__float_as_uint(tx) << 23));
-  y = __uint_as_float(__float_as_uint(y) + (__float_as_uint(ty) << 23));
 }
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -522,6 +493,10 @@ __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[32]) 
         "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
         "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
+}
+// The lowest n bits (none for n <= 0, all for n >= 32).
+__device__ __forceinline__ uint32_t ones_below(int n) {
+  return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
 }
 // A CTA's work: its rows and the key tiles they see.
 struct Job {
@@ -644,10 +619,12 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
   auto o_done = [&](int t) { return bar1 + (NQ + t) * 8; };
   auto drained = [&](int t) { return bar1 + (2 * NQ + t) * 8; };
   auto p_full = [&](int t, int half) { return bar1 + (3 * NQ + 2 * t + half) * 8; };
-  auto s_full = [&](int i) { return bar1 + (5 * NQ + i) * 8; };
+  auto turn = [&](int t) { return bar1 + (5 * NQ + t) * 8; };
+  auto staged = [&](int t) { return bar1 + (6 * NQ + t) * 8; };
+  auto s_full = [&](int i) { return bar1 + (7 * NQ + i) * 8; };
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kSlots; ++s) {
-      mbar_init(kv_full(s), 1);
+      mbar_init(kv_full(s), C::kProducers);
       mbar_init(kv_empty(s), NQ);
     }
     for (int i = 0; i < C::kVBars; ++i) mbar_init(v_ready(i), 32);
@@ -657,6 +634,8 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       mbar_init(p_full(t, 1), 128);
       mbar_init(o_done(t), 1);
       mbar_init(drained(t), 1);
+      mbar_init(turn(t), 1);
+      mbar_init(staged(t), 128);
     }
     for (int i = 0; i < NQ * C::kSBufs; ++i) mbar_init(s_full(i), 1);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -681,11 +660,15 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
   bool ok = true;
 
   if (warp >= NQ * 4) {
-    if constexpr (NQ == 2) regs_down<kIssueRegs>();
-  if (warp == NQ * 4 + NQ) {
+    if constexpr (NQ == 2) regs_down<kOtherRegs>();
+  if (warp >= NQ * 4 + NQ && warp < NQ * 4 + NQ + C::kProducers) {
     // ---------------------------------------------------------------- producer
-    // Lane = one box: R token rows of one 64-dim chunk.
-    const int box = lane / C::kChunks, chunk = lane - box * C::kChunks;
+    // A box is R token rows of one 64-dim chunk; lane l of producer w has box
+    // l * kProducers + w. (A box takes ~60 cycles to set off, whichever lane does
+    // it: one warp for all 64 boxes of a tile with pages of 16 tokens kept the
+    // products waiting, 434 us where pages of 32 took 393.)
+    const int f = lane * C::kProducers + warp - (NQ * 4 + NQ);
+    const int box = f / C::kChunks, chunk = f - box * C::kChunks;
     auto lookup = [&](int k, int& phys, int& slot) {
       phys = INT_MIN;
       slot = 0;
@@ -733,7 +716,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       for (int i = 0; i < C::kSlots; ++i) mbar_wait(kv_full(i), i < s ? phase : phase ^ 1);
     }
   }
-  if (warp == NQ * 4 + NQ + 1) {
+  if (warp == NQ * 4 + NQ + C::kProducers) {
     // ----------------------------------------------------------------- cleaner
     // Hands each V tile on to the issuing warps, after zeroing the rows of its
     // multiplied 16-token steps whose tokens no row sees.
@@ -824,9 +807,19 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       int ks = 0, vs = 1;
       uint32_t kph = 0;
       KeyTile cur = key_tile<kTN>(j, j.k0);
-      if (n > 0 && wait(q_full(t), 0) && wait(kv_full(0), 0)) {
+      // The two row tiles' (P V, next S) blocks alternate on the pipe: mixed, both
+      // would be ready late, and the softmax warps of both would first wait and
+      // then run at the same time.
+      auto my_turn = [&](int block) {
+        return NQ == 1 || (t == 0 && block == 0) || wait(turn(t), (t == 0 ? block - 1 : block) & 1);
+      };
+      auto pass_turn = [&]() {
+        if (NQ == 2) mbar_arrive(turn(1 - t));
+      };
+      if (n > 0 && wait(q_full(t), 0) && wait(kv_full(0), 0) && my_turn(0)) {
         issue_s(0, 0, cur);
         if (n > 1) tc_commit(kv_empty(0));
+        pass_turn();
       }
       for (int i = 0; i < n && ok; ++i) {
         const bool more = i + 1 < n;
@@ -846,7 +839,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
         if (!wait(v_ready(i), i / C::kVBars & 1) || !wait(p_full(t, 0), i & 1)) break;
         tc_fence_after();
         issue_o(buf, vs, cur, 0, i > 0);
-        if (!wait(p_full(t, 1), i & 1)) break;
+        if (!my_turn(i + 1) || !wait(p_full(t, 1), i & 1)) break;
         tc_fence_after();
         issue_o(buf, vs, cur, 1, i > 0);
         if (NQ == 1 || !more) tc_commit(o_done(t));
@@ -854,6 +847,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
           issue_s(0, ks, nxt);
           if (i + 2 < n) tc_commit(kv_empty(ks));
         }
+        pass_turn();
         if (more) tc_commit(kv_empty(vs));
         vs += 2;
         if (vs >= C::kSlots) vs -= C::kSlots;
@@ -938,8 +932,13 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       if (__any_sync(kFull, hi < base + kTN || low > base)) {
         const int h = hi - base, lo = low - base, sk = p.sinks - base;
 #pragma unroll
-        for (int c = 0; c < kTN; ++c)
-          if (!(c < h && (c >= lo || c < sk))) s[c] = -INFINITY;
+        for (int c0 = 0; c0 < kTN; c0 += 32) {
+          // 32 columns' visibility as one word
+          const uint32_t seen = ones_below(h - c0) & (~ones_below(lo - c0) | ones_below(sk - c0));
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            s[c0 + c] = seen & 1u << c ? s[c0 + c] : -INFINITY;
+        }
       }
       float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
@@ -980,16 +979,10 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
           uint32_t pk[16];
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            const uint64_t v = f2_fma(f2(s[c0 + c], s[c0 + c + 1]), scl2, off2);
             float x, y;
-            // 3 of 8 pairs on the FMA pipe
-            if ((c & 15) == 4 || (c & 15) == 10 || (c & 15) == 14) {
-              ex2_pair_fma(v, x, y);
-            } else {
-              f2_split(v, x, y);
-              x = ex2(x);
-              y = ex2(y);
-            }
+            f2_split(f2_fma(f2(s[c0 + c], s[c0 + c + 1]), scl2, off2), x, y);
+            x = ex2(x);
+            y = ex2(y);
             sum[(c >> 1) & 1] = f2_add(sum[(c >> 1) & 1], f2(x, y));
             pk[c / 2] = pack2<T>(x, y);
           }
@@ -1049,13 +1042,15 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
                          : "memory");
           }
         }
-        asm volatile("bar.sync %0, 128;" ::"r"(t + 1) : "memory");
+        mbar_arrive(staged(t));
+        ok = __all_sync(kFull, mbar_wait(staged(t), 0));   // bounded, unlike a named barrier
+        if (!ok && lane == 0) flag(p, PA_STATUS_TIMEOUT);
         const int c = tid % kPer;
 #pragma unroll 4
         for (int i = 0; i < kPer; ++i) {
           const int r = i * (128 / kPer) + tid / kPer;
           const int q = r0 + r;
-          if (q < j.rows) {
+          if (ok && q < j.rows) {
             const int qt = static_cast<int>(fast_div(q, a.div_g));
             uint4 v;
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
