@@ -34,9 +34,14 @@ constexpr int kPlanThreads = 1024;
 constexpr int kReleaseSpan = 512;
 // Taken pages listed in shared memory; longer lists go through the scratch.
 constexpr int kListSmem = 4096;
-// Copy kernel: 256 threads x 4 x 16 bytes per unit.
+// Copy kernel: 256 threads x 8 x 16 bytes per unit.
 constexpr int kCopyThreads = 256;
-constexpr int kCopyUnroll = 4;
+constexpr int kCopyUnroll = 8;
+// Three blocks an SM (96 KB of loads in flight): compacting 4096 pages of 16 layers
+// (2.06 GB moved) 349 us, with four blocks 378, two 357, four loads a thread 361;
+// grids of 8 to 64 blocks an SM differ by 5 %.
+constexpr int kCopyBlocks = 3;
+constexpr int kCopyGrid = 16;
 constexpr int kCopyChunks = kCopyThreads * kCopyUnroll;   // 16-byte chunks of one unit
 
 // Scratch header (int32): zero between launches except kHCopies, which the plan
@@ -123,18 +128,19 @@ __device__ __forceinline__ int count_free(const Pool& p, const Share& s) {
   for (int w = s.lo; w < s.hi; ++w) n += __popc(__ldcg(p.words + w));
   return n;
 }
-// Takes the `total` lowest free pages: list[k] = the k-th, its bit cleared and
-// its count set to 1. `before`: free pages in lower shares.
-__device__ __forceinline__ void take_free(const Pool& p, const Share& s, int before, int total,
+// Takes the free pages of rank [from, to) in ascending order: list[k] = the one
+// of rank from + k, its bit cleared and its count set to 1. `rank`: the rank of
+// this thread's lowest free page that has not been taken, advanced past those
+// taken here.
+__device__ __forceinline__ void take_free(const Pool& p, const Share& s, int& rank, int from, int to,
                                           int* list) {
-  int k = before;
-  for (int w = s.lo; w < s.hi && k < total; ++w) {
+  for (int w = s.lo; w < s.hi && rank < to; ++w) {
     unsigned bits = __ldcg(p.words + w);
     if (!bits) continue;
-    while (bits && k < total) {
+    while (bits && rank < to) {
       const int page = w * 32 + __ffs(bits) - 1;
       bits &= bits - 1;
-      list[k++] = page;
+      list[rank++ - from] = page;
       p.refs[page] = 1;
     }
     p.words[w] = bits;
@@ -183,7 +189,7 @@ __device__ __forceinline__ RowChange row_change(const Resize& a, int r, bool& ba
 __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Resize a) {
   __shared__ int s_scan[32];
   __shared__ int s_list[kListSmem];
-  __shared__ int s_last;
+  __shared__ int s_last, s_copies;
   const Pool& p = a.p;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   grid_wait();
@@ -243,138 +249,171 @@ __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Resize a) {
   const Share sh = word_share(p);
   const int mine = count_free(p, sh);
   int avail;
-  const int before = block_scan(mine, s_scan, avail) - mine;
+  int rank = block_scan(mine, s_scan, avail) - mine;
+  if (threadIdx.x == 0) {
+    p.scratch[kHArrive] = 0;
+    s_copies = 0;
+  }
 
-  // Which rows get their pages: in row order, a row all of them or none.
-  long long carry = 0;
-  int granted = 0;
-  int* plan = p.plan();
+  // In row order, a row all of its pages or none; 1024 rows at a time, one
+  // thread each (a step's rows miss a page or two: with a warp per row, eight
+  // rows in turn per warp and their lengths read again, this phase took 10 of
+  // the call's 18 us for 256 rows).
+  long long carry = 0;        // pages asked for so far, refused rows' among them
+  int given = 0;              // pages given out so far
   for (int r0 = 0; r0 < a.t.rows; r0 += blockDim.x) {
     const int r = r0 + threadIdx.x;
-    int need = 0, cow = 0;
-    bool active = false;
-    if (r < a.t.rows) {
-      bool bad;
-      const RowChange c = row_change(a, r, bad);
-      active = c.active;
-      if (active && c.n > c.S) {
-        need = c.want - c.used;
-        if (c.S % p.bs) {                   // grows into its partly filled last page
-          const int e = __ldcg(a.t.bt + r * a.t.sb + c.S / p.bs);
-          if (!in_pool(p, e))
-            flag(p, PA_STATUS_BAD_BLOCK);
-          else
-            cow = __ldcg(p.refs + e) > 1;   // others use it too: a copy of its own
-        }
-      }
-      need += cow;
-    }
-    int total;
-    const int end = block_scan(need, s_scan, total);
-    const long long all = carry + end;
-    const bool ok = need == 0 || all <= avail;
-    if (r < a.t.rows) {
-      plan[r] = !active ? -2 : ok ? (static_cast<int>(all - need) << 1 | cow) : -1;
-      if (active && !ok) flag(p, PA_STATUS_NO_PAGES);
-    }
-    // pages given out: the largest end of a row that gets its pages
-    const int give = need > 0 && ok ? static_cast<int>(all) : 0;
-    const int top = __reduce_max_sync(kFull, static_cast<unsigned>(give));
-    if (lane == 0) s_scan[warp] = top;
-    __syncthreads();
-    for (int w = 0; w < nw; ++w) granted = max(granted, s_scan[w]);
-    __syncthreads();
-    carry += total;
-  }
-  int* list = granted <= kListSmem ? s_list : p.list();
-  take_free(p, sh, before, granted, list);
-  if (threadIdx.x == 0) p.scratch[kHArrive] = 0;
-  __shared__ int s_copies;
-  if (threadIdx.x == 0) s_copies = 0;
-  __syncthreads();
-
-  // Entries, lengths, and the copy list (its order changes nothing).
-  for (int r = warp; r < a.t.rows; r += nw) {
-    const int pl = __ldcg(plan + r);
-    if (pl < 0) continue;
+    int need = 0, cow = 0, tail = 0;
     bool bad;
-    const RowChange c = row_change(a, r, bad);
+    RowChange c;
+    c.active = false;
     int* row = a.t.bt + r * a.t.sb;
-    const int begin = pl >> 1, cow = pl & 1;
-    for (int j = c.used + lane; j < c.want; j += 32) row[j] = list[begin + cow + j - c.used];
-    __syncwarp();
-    if (lane == 0) {
+    if (r < a.t.rows) c = row_change(a, r, bad);
+    if (c.active && c.n > c.S) {
+      need = c.want - c.used;
+      if (c.S % p.bs) {                     // grows into its partly filled last page
+        tail = __ldcg(row + c.S / p.bs);
+        if (!in_pool(p, tail))
+          flag(p, PA_STATUS_BAD_BLOCK);
+        else
+          cow = __ldcg(p.refs + tail) > 1;  // others use it too: a copy of its own
+      }
+    }
+    need += cow;
+    int total;
+    const long long all = carry + block_scan(need, s_scan, total);
+    const bool ok = need == 0 || all <= avail;
+    if (c.active && !ok) flag(p, PA_STATUS_NO_PAGES);
+    // the pages of this round: up to the largest end of a row that gets its pages
+    const unsigned top = __reduce_max_sync(kFull, need > 0 && ok ? static_cast<unsigned>(all) : 0u);
+    if (lane == 0) s_scan[warp] = static_cast<int>(top);
+    __syncthreads();
+    int end = given;
+    for (int w = 0; w < nw; ++w) end = max(end, s_scan[w]);
+    int* list = end - given <= kListSmem ? s_list : p.list();
+    take_free(p, sh, rank, given, end, list);
+    __syncthreads();
+    int at = static_cast<int>(all - need) - given;     // the row's place in the list
+    if (c.active && ok) {
       if (cow) {
-        const int at = c.S / p.bs;
-        const int src = row[at], dst = list[begin];
-        row[at] = dst;
-        if (atomicSub(p.refs + src, 1) == 1)
-          atomicOr(p.words + (src >> 5), 1u << (src & 31));
-        int* e = p.copies() + 3 * atomicAdd(&s_copies, 1);
-        e[0] = src;
+        const int dst = list[at];
+        row[c.S / p.bs] = dst;
+        if (atomicSub(p.refs + tail, 1) == 1)
+          atomicOr(p.words + (tail >> 5), 1u << (tail & 31));
+        int* e = p.copies() + 3 * atomicAdd(&s_copies, 1);   // (in any order)
+        e[0] = tail;
         e[1] = dst;
         e[2] = c.S % p.bs;
+        ++at;
       }
       a.t.lens[r] = c.n;
     }
+    // New entries: a few by the row's own thread, many by its warp.
+    const int fresh = c.active && ok ? max(0, c.want - c.used) : 0;
+    if (fresh <= 4)
+      for (int i = 0; i < fresh; ++i) row[c.used + i] = list[at + i];
+    for (unsigned big = __ballot_sync(kFull, fresh > 4); big; big &= big - 1) {
+      const int src = __ffs(big) - 1;
+      const int cnt = __shfl_sync(kFull, fresh, src), first = __shfl_sync(kFull, c.used, src);
+      const int from = __shfl_sync(kFull, at, src);
+      int* to = a.t.bt + (r - lane + src) * a.t.sb + first;
+      for (int i = lane; i < cnt; i += 32) to[i] = list[from + i];
+    }
+    carry += total;
+    given = end;
+    __syncthreads();
   }
-  __syncthreads();
   if (threadIdx.x == 0) p.scratch[kHCopies] = s_copies;
 }
 
 // ----------------------------------------------------------------------------
 // Copies
 // ----------------------------------------------------------------------------
-// Unit u of the copy list: entry, cache, 16 KB part of the page's used slots.
-// All loads of a unit are issued before its stores (16 KB per block in flight,
-// 8 blocks an SM).
-__device__ __forceinline__ void copy_unit(const Pool& p, long long u, int parts) {
-  const int part = static_cast<int>(u % parts);
-  const long long ec = u / parts;
-  const int ncache = 2 * p.layers;
-  const int cache = static_cast<int>(ec % ncache);
-  const int* e = p.copies() + 3 * (ec / ncache);
-  const int src = __ldcg(e), dst = __ldcg(e + 1), slots = __ldcg(e + 2);
-  const int row = p.Hkv * p.chunks;                 // chunks of one slot
-  const int n = slots * row;
-  const int c0 = part * kCopyChunks + threadIdx.x;
-  if (part * kCopyChunks >= n) return;
-  const int kv = cache & 1;
-  char* base = p.caches[cache];
-  const char* from = base + src * p.sb[kv];
-  char* to = base + dst * p.sb[kv];
-  uint4 v[kCopyUnroll];
-  long long off[kCopyUnroll];
-#pragma unroll
-  for (int i = 0; i < kCopyUnroll; ++i) {
-    const int c = c0 + i * kCopyThreads;
-    if (p.dense) {
-      off[i] = c * 16ll;
-    } else {
-      const int slot = c / row;
-      const int h = (c - slot * row) / p.chunks;
-      off[i] = slot * p.ss[kv] + h * p.sh[kv] + (c - slot * row - h * p.chunks) * 16ll;
-    }
-    if (c < n) v[i] = __ldcs(reinterpret_cast<const uint4*>(from + off[i]));
+// A unit is one 32 KB part of the used slots of one page in one cache: all eight
+// loads of a thread are issued before its stores. A block runs several units in
+// turn and reads the next one's list entry during the current one, so that the
+// list's latency stays off the path of the data.
+struct CopyUnit { int src, dst, slots, cache, part; };
+__device__ __forceinline__ CopyUnit load_unit(const Pool& p, long long u, int parts) {
+  CopyUnit c;
+  const int per_entry = 2 * p.layers * parts;
+  long long entry;
+  int rest;
+  if (u <= 0xffffffffll) {                          // 32-bit divisions nearly always
+    const unsigned q = static_cast<unsigned>(u) / static_cast<unsigned>(per_entry);
+    entry = q;
+    rest = static_cast<int>(static_cast<unsigned>(u) - q * per_entry);
+  } else {
+    entry = u / per_entry;
+    rest = static_cast<int>(u - entry * per_entry);
   }
+  c.cache = rest / parts;
+  c.part = rest - c.cache * parts;
+  const int* e = p.copies() + 3 * entry;
+  c.src = __ldcg(e);
+  c.dst = __ldcg(e + 1);
+  c.slots = __ldcg(e + 2);
+  return c;
+}
+__device__ __forceinline__ void copy_unit(const Pool& p, const CopyUnit& u) {
+  const int row = p.Hkv * p.chunks;                 // chunks of one slot
+  const int n = u.slots * row;
+  if (u.part * kCopyChunks >= n) return;
+  const int c0 = u.part * kCopyChunks + threadIdx.x;
+  const bool v_cache = u.cache & 1;
+  const long long sb = v_cache ? p.sb[1] : p.sb[0];
+  char* base = p.caches[u.cache];
+  const char* from = base + u.src * sb;
+  char* to = base + u.dst * sb;
+  uint4 v[kCopyUnroll];
+  if (p.dense) {
+    from += c0 * 16ll;
+    to += c0 * 16ll;
+#pragma unroll
+    for (int i = 0; i < kCopyUnroll; ++i)
+      if (c0 + i * kCopyThreads < n)
+        v[i] = __ldcs(reinterpret_cast<const uint4*>(from) + i * kCopyThreads);
+#pragma unroll
+    for (int i = 0; i < kCopyUnroll; ++i)
+      if (c0 + i * kCopyThreads < n) reinterpret_cast<uint4*>(to)[i * kCopyThreads] = v[i];
+    return;
+  }
+  const long long ss = v_cache ? p.ss[1] : p.ss[0], sh = v_cache ? p.sh[1] : p.sh[0];
+  auto off = [&](int c) {
+    const int slot = c / row;
+    const int h = (c - slot * row) / p.chunks;
+    return slot * ss + h * sh + (c - slot * row - h * p.chunks) * 16ll;
+  };
 #pragma unroll
   for (int i = 0; i < kCopyUnroll; ++i)
-    if (c0 + i * kCopyThreads < n) *reinterpret_cast<uint4*>(to + off[i]) = v[i];
+    if (c0 + i * kCopyThreads < n)
+      v[i] = __ldcs(reinterpret_cast<const uint4*>(from + off(c0 + i * kCopyThreads)));
+#pragma unroll
+  for (int i = 0; i < kCopyUnroll; ++i)
+    if (c0 + i * kCopyThreads < n)
+      *reinterpret_cast<uint4*>(to + off(c0 + i * kCopyThreads)) = v[i];
 }
 
 __device__ __forceinline__ int page_parts(const Pool& p) {
   return (p.bs * p.Hkv * p.chunks + kCopyChunks - 1) / kCopyChunks;
 }
 
-__device__ __forceinline__ void copy_all(const Pool& p) {
+// The copy list's units from `first` on, `step` apart.
+__device__ __forceinline__ void copy_all(const Pool& p, long long first, long long step) {
   const int parts = page_parts(p);
   const long long units = static_cast<long long>(__ldcg(p.scratch + kHCopies)) * 2 * p.layers * parts;
-  for (long long u = blockIdx.x; u < units; u += gridDim.x) copy_unit(p, u, parts);
+  if (first >= units) return;
+  CopyUnit next = load_unit(p, first, parts);
+  for (long long u = first; u < units; u += step) {
+    const CopyUnit cur = next;
+    if (u + step < units) next = load_unit(p, u + step, parts);
+    copy_unit(p, cur);
+  }
 }
 
-__global__ void __launch_bounds__(kCopyThreads) copy_kernel(const Pool p) {
+__global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) copy_kernel(const Pool p) {
   grid_wait();
-  copy_all(p);
+  copy_all(p, blockIdx.x, gridDim.x);
 }
 
 // ----------------------------------------------------------------------------
@@ -399,7 +438,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const Fork a) {
   const Share sh = word_share(p);
   const int mine = count_free(p, sh);
   int avail;
-  const int before = block_scan(mine, s_scan, avail) - mine;
+  int rank = block_scan(mine, s_scan, avail) - mine;
   int* plan = p.plan();
 
   // A child row has to be empty. Pairs that name the same child: the first one
@@ -464,7 +503,7 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const Fork a) {
   }
   granted = static_cast<int>(min(carry, static_cast<long long>(avail)));
   int* list = granted <= kListSmem ? s_list : p.list();
-  take_free(p, sh, before, granted, list);
+  take_free(p, sh, rank, 0, granted, list);
   __syncthreads();
   for (int i = threadIdx.x; i < a.n; i += blockDim.x) {
     const int S = plan[2 * i];
@@ -486,19 +525,13 @@ __global__ void __launch_bounds__(kPlanThreads) fork_plan_kernel(const Fork a) {
 }
 
 // The children's table rows (each shared page counted once more), and the copies.
-__global__ void __launch_bounds__(kCopyThreads) fork_apply_kernel(const Fork a) {
+__global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) fork_apply_kernel(const Fork a) {
   const Pool& p = a.p;
   grid_wait();
   const int* plan = p.plan();
   const int spans = (a.t.width + kCopyThreads - 1) / kCopyThreads;
   const long long rows = static_cast<long long>(a.n) * spans;
-  const int parts = page_parts(p);
-  const long long units = static_cast<long long>(__ldcg(p.scratch + kHCopies)) * 2 * p.layers * parts;
-  for (long long u = blockIdx.x; u < rows + units; u += gridDim.x) {
-    if (u >= rows) {
-      copy_unit(p, u - rows, parts);
-      continue;
-    }
+  for (long long u = blockIdx.x; u < rows; u += gridDim.x) {
     const int i = static_cast<int>(u / spans);
     const int S = __ldcg(plan + 2 * i);
     const int j = static_cast<int>(u - static_cast<long long>(i) * spans) * kCopyThreads + threadIdx.x;
@@ -513,6 +546,7 @@ __global__ void __launch_bounds__(kCopyThreads) fork_apply_kernel(const Fork a) 
     }
     a.t.bt[__ldg(a.children + i) * a.t.sb + j] = e;
   }
+  copy_all(p, (blockIdx.x + gridDim.x - rows % gridDim.x) % gridDim.x, gridDim.x);
 }
 
 // ----------------------------------------------------------------------------
@@ -585,20 +619,14 @@ __global__ void __launch_bounds__(kPlanThreads) compact_plan_kernel(const Compac
   }
 }
 
-__global__ void __launch_bounds__(kCopyThreads) compact_apply_kernel(const Compact a) {
+__global__ void __launch_bounds__(kCopyThreads, kCopyBlocks) compact_apply_kernel(const Compact a) {
   const Pool& p = a.p;
   grid_wait();
   const int live = __ldcg(p.scratch + kHLive);
   const int* map = p.list();
   const int spans = (a.t.width + kCopyThreads - 1) / kCopyThreads;
   const long long rows = static_cast<long long>(a.t.rows) * spans;
-  const int parts = page_parts(p);
-  const long long units = static_cast<long long>(__ldcg(p.scratch + kHCopies)) * 2 * p.layers * parts;
-  for (long long u = blockIdx.x; u < rows + units; u += gridDim.x) {
-    if (u >= rows) {
-      copy_unit(p, u - rows, parts);
-      continue;
-    }
+  for (long long u = blockIdx.x; u < rows; u += gridDim.x) {
     const int r = static_cast<int>(u / spans);
     const int j = static_cast<int>(u - static_cast<long long>(r) * spans) * kCopyThreads + threadIdx.x;
     if (j >= a.t.width) continue;
@@ -611,6 +639,7 @@ __global__ void __launch_bounds__(kCopyThreads) compact_apply_kernel(const Compa
     else
       *at = to;
   }
+  copy_all(p, (blockIdx.x + gridDim.x - rows % gridDim.x) % gridDim.x, gridDim.x);
 }
 
 // ----------------------------------------------------------------------------
@@ -693,11 +722,11 @@ static cudaError_t launch(void (*kernel)(const Arg), long long grid, int threads
 }
 
 // Blocks of a kernel that copies up to `entries` pages and walks `row_units`
-// table parts: one per unit, at most eight per SM.
+// table parts: one per unit, at most kCopyGrid per SM.
 static long long copy_grid(const Pool& p, long long entries, long long row_units, int sms) {
   const long long parts =
       (static_cast<long long>(p.bs) * p.Hkv * p.chunks + kCopyChunks - 1) / kCopyChunks;
-  return std::min(8ll * sms, entries * 2 * p.layers * parts + row_units);
+  return std::min<long long>(static_cast<long long>(kCopyGrid) * sms, entries * 2 * p.layers * parts + row_units);
 }
 
 }  // namespace pa_pages
