@@ -99,6 +99,24 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// The sequence that holds a query row (warp-uniform), -1 for a row of none.
+__device__ __forceinline__ int seq_of_row(const Params& p, int row) {
+  const int lane = threadIdx.x & 31;
+  if (p.B < 32) {                        // one load per lane, no search
+    const int s = lane <= p.B ? __ldg(p.starts + lane) : 0;
+    const unsigned at = __ballot_sync(kFull, lane < p.B && s <= row);
+    const int b = at ? 31 - __clz(at) : 0;
+    const int s0 = __shfl_sync(kFull, s, b), s1 = __shfl_sync(kFull, s, b + 1);
+    return row >= s0 && row < s1 ? b : -1;
+  }
+  int lo = 0, hi = p.B - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (__ldg(p.starts + mid) <= row) lo = mid; else hi = mid - 1;
+  }
+  return row >= __ldg(p.starts + lo) && row < __ldg(p.starts + lo + 1) ? lo : -1;
+}
+
 // ----------------------------------------------------------------------------
 // CUDA-core path: every shape
 // ----------------------------------------------------------------------------
@@ -115,17 +133,18 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
   if (w >= static_cast<long long>(p.T) * p.Hq) return;
   const int row = static_cast<int>(w / p.Hq);
   const int hq = static_cast<int>(w - static_cast<long long>(row) * p.Hq);
-  // the last sequence that starts at or before the row
-  int lo = 0, hi = p.B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(p.starts + mid) <= row) lo = mid; else hi = mid - 1;
-  }
   bool bad;
-  const Seq s = load_seq(p, lo, bad);
-  if (bad && lane == 0) flag(p, PA_STATUS_BAD_SEQLEN);
-  if (row < s.start || row >= s.start + s.n) return;   // behind the last sequence
-  const int b = lo, kvh = hq / p.G;
+  if (w == 0) {                    // every sequence is checked once
+    for (int b = lane; b < p.B; b += 32) {
+      load_seq(p, b, bad);
+      if (bad) flag(p, PA_STATUS_BAD_SEQLEN);
+    }
+    __syncwarp();
+  }
+  const int b = seq_of_row(p, row);
+  if (b < 0) return;               // a row of no sequence
+  const Seq s = load_seq(p, b, bad);
+  const int kvh = hq / p.G;
   const int pos = s.S - s.n + row - s.start;
   const int first = pos >= p.window ? pos - p.window + 1 : 0;   // of the window
   const int a = min(p.sinks, first);                            // visible sinks
@@ -214,10 +233,21 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
 // Roles: producer warps (lane = one TMA box of a page), a warp that cleans V
 // tiles at the edges of what is visible, one issuing warp per 128 rows, and four
 // softmax warps per 128 rows, thread = row, so that row maxima and sums need no
-// exchange. With NQ = 2 the two row tiles
-// alternate on the matrix pipe: while one's S is turned into P, the other's
-// products run. With NQ = 1 (short chunks, head_dim 256) S has two buffers and
-// the next tile's S is computed during the current softmax.
+// exchange. With NQ = 2 the two row tiles alternate on the matrix pipe: while
+// one's S is turned into P, the other's products run. With NQ = 1 (short chunks,
+// head_dim 256) S has two buffers and the next tile's S is computed during the
+// current softmax.
+//
+// What bounds it (8192 tokens, Hq32/Hkv8, D 128, window 4096 / none: 368 / 457 us,
+// 1.12 / 1.20 PFLOP/s): the chain from a tile's S to its P. 256 rows x 128 keys
+// take the matrix pipe 2048 cycles, the special function units as many, and the
+// tile's turn ~3000: load of S 250, maximum 300-400, exponentials 1400 (1024 if no
+// other warp ran), then the rest of P V and the next S 1000. Tried and slower:
+// two threads per row (twice the warps; a meeting for each maximum, registers
+// spill: 481 us where one thread took 425), tiles of 64 keys with two S buffers
+// (S is no longer waited for, but every tile's fixed costs double and the row
+// tile is read twice as often: 418 against 388), P formed against the previous
+// maximum while the new one is taken (430 against 388).
 //
 // P is rounded to the operand type once (half a step, relative); its sum, the
 // maxima and O are kept in 32 bits. O is rescaled only when a row's maximum has
@@ -226,9 +256,9 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
 //
 // Masks: a tile that is not entirely visible to all rows of a warp compares
 // each score's token with the row's limits. Tokens that no row sees are cut off
-// in steps of 16 by the products' shape (N of the first, K of the second); the
-// V rows of such tokens inside the remaining steps are zeroed in
-// shared memory first, as 0 * NaN would reach O.
+// in steps of 16 by the products' shape (N of the first, K of the second); the V
+// rows of such tokens inside the remaining steps are zeroed in shared memory
+// first, as 0 * NaN would reach O.
 template <int D, int NQ>
 struct TC {
   static constexpr int kTN = D == 256 ? 64 : 128;      // keys per tile
@@ -569,43 +599,67 @@ __device__ __forceinline__ bool find_job(const TileParams& a, Job& j, int* sh) {
   const int per = p.Hkv * a.splits;
   const int x = blockIdx.x / per;
   const int rest = blockIdx.x - x * per;
-  // running sums over the sequences, from the last to the first
-  int before = 0;
-  if (threadIdx.x == 0) sh[32] = -1;
-  for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
-    const int b = p.B - 1 - (b0 + static_cast<int>(threadIdx.x));
-    int nt = 0;
-    bool bad = false;
-    if (b >= 0) nt = (load_seq(p, b, bad).n * p.G + kRows - 1) / kRows;
-    if (bad && blockIdx.x == 0) flag(p, PA_STATUS_BAD_SEQLEN);
+  bool bad = false;
+  int tile = 0;
+  if (p.B <= 32) {
+    // few sequences: every warp finds the job by itself
+    const int b = p.B - 1 - lane;
+    Seq s = {0, 0, 0};
+    if (b >= 0) s = load_seq(p, b, bad);
+    if (bad && blockIdx.x == 0 && warp == 0) flag(p, PA_STATUS_BAD_SEQLEN);
+    const int nt = (s.n * p.G + kRows - 1) / kRows;
     int v = nt;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int u = __shfl_up_sync(kFull, v, o);
       if (lane >= o) v += u;
     }
-    if (lane == 31) sh[warp] = v;
-    __syncthreads();
-    int base = before, all = 0;
-    for (int w = 0; w < nw; ++w) {
-      if (w < warp) base += sh[w];
-      all += sh[w];
+    const unsigned reach = __ballot_sync(kFull, x < v);
+    if (!reach) return false;
+    const int src = __ffs(reach) - 1;
+    tile = __shfl_sync(kFull, v, src) - 1 - x;
+    j.b = p.B - 1 - src;
+    j.s.start = __shfl_sync(kFull, s.start, src);
+    j.s.n = __shfl_sync(kFull, s.n, src);
+    j.s.S = __shfl_sync(kFull, s.S, src);
+  } else {
+    // running sums over the sequences, from the last to the first
+    int before = 0;
+    if (threadIdx.x == 0) sh[32] = -1;
+    for (int b0 = 0; b0 < p.B; b0 += blockDim.x) {
+      const int b = p.B - 1 - (b0 + static_cast<int>(threadIdx.x));
+      int nt = 0;
+      bad = false;
+      if (b >= 0) nt = (load_seq(p, b, bad).n * p.G + kRows - 1) / kRows;
+      if (bad && blockIdx.x == 0) flag(p, PA_STATUS_BAD_SEQLEN);
+      int v = nt;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(kFull, v, o);
+        if (lane >= o) v += u;
+      }
+      if (lane == 31) sh[warp] = v;
+      __syncthreads();
+      int base = before, all = 0;
+      for (int w = 0; w < nw; ++w) {
+        if (w < warp) base += sh[w];
+        all += sh[w];
+      }
+      const int lo = base + v - nt;
+      if (x >= lo && x < lo + nt) {
+        sh[32] = b;
+        sh[33] = lo + nt - 1 - x;
+      }
+      before += all;
+      __syncthreads();
+      if (before > x && blockIdx.x) break;   // block 0 checks every sequence
     }
-    const int lo = base + v - nt;
-    if (x >= lo && x < lo + nt) {
-      sh[32] = b;
-      sh[33] = lo + nt - 1 - x;
-    }
-    before += all;
-    __syncthreads();
-    if (before > x && blockIdx.x) break;   // block 0 checks every sequence
+    j.b = sh[32];
+    if (j.b < 0) return false;
+    j.s = load_seq(p, j.b, bad);
+    tile = sh[33];
   }
-  const int b = sh[32];
-  if (b < 0) return false;
-  bool bad;
-  j.b = b;
-  j.s = load_seq(p, b, bad);
-  j.r0 = sh[33] * kRows;
+  j.r0 = tile * kRows;
   j.rows = j.s.n * p.G;
   j.kvh = rest / a.splits;
   j.split = rest - j.kvh * a.splits;
@@ -679,6 +733,9 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   tc_fence_before();
+  // Dependent launch: from here on global memory is read.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   Job j;
   const bool found = find_job<D, NQ>(a, j, s_find);   // the same answer in every thread
   __syncthreads();
@@ -692,206 +749,206 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
 
   if (warp >= NQ * 4) {
     if constexpr (NQ == 2) regs_down<kOtherRegs>();
-  if (warp >= NQ * 4 + NQ && warp < NQ * 4 + NQ + C::kProducers) {
-    // ---------------------------------------------------------------- producer
-    // A box is R token rows of one 64-dim chunk; lane l of producer w has box
-    // l * kProducers + w. (A box takes ~60 cycles to set off, whichever lane does
-    // it: one warp for all 64 boxes of a tile with pages of 16 tokens kept the
-    // products waiting, 434 us where pages of 32 took 393.)
-    const int f = lane * C::kProducers + warp - (NQ * 4 + NQ);
-    const int box = f / C::kChunks, chunk = f - box * C::kChunks;
-    auto lookup = [&](int k, int& phys, int& slot) {
-      phys = INT_MIN;
-      slot = 0;
-      const KeyTile t = key_tile<kTN>(j, k);
-      const int tok = t.base + (box << a.lR);
-      if (box < (kTN >> a.lR) && box_seen(j, t, tok, a.R)) {
-        const int pg = a.bs_log2 >= 0 ? tok >> a.bs_log2 : static_cast<int>(fast_div(tok, a.div_bs));
-        slot = tok - pg * p.bs;
-        phys = __ldg(p.bt + j.b * p.bt_sb + pg);
-      }
-    };
-    int phys, slot, nphys = INT_MIN, nslot = 0, s = 0;
-    uint32_t phase = 0;
-    if (j.k0 < j.k1) lookup(j.k0, nphys, nslot);
-    for (int k = j.k0; k < j.k1 && ok; ++k) {
-      phys = nphys;
-      slot = nslot;
-      if (k + 1 < j.k1) lookup(k + 1, nphys, nslot);
-      bool valid = phys != INT_MIN;
-      if (valid && (phys < 0 || phys >= p.NB)) {
-        flag(p, PA_STATUS_BAD_BLOCK);
-        valid = false;
-      }
-      const uint32_t bytes = __popc(__ballot_sync(kFull, valid)) * a.R * 128;
-      for (int kv = 0; kv < 2; ++kv) {
-        ok = mbar_wait(kv_empty(s), phase ^ 1);
-        if (!__all_sync(kFull, ok)) {
-          ok = false;
-          break;
+    if (warp >= NQ * 4 + NQ && warp < NQ * 4 + NQ + C::kProducers) {
+      // ---------------------------------------------------------------- producer
+      // A box is R token rows of one 64-dim chunk; lane l of producer w has box
+      // l * kProducers + w. (A box takes ~60 cycles to set off, whichever lane does
+      // it: one warp for all 64 boxes of a tile with pages of 16 tokens kept the
+      // products waiting, 434 us where pages of 32 took 393.)
+      const int f = lane * C::kProducers + warp - (NQ * 4 + NQ);
+      const int box = f / C::kChunks, chunk = f - box * C::kChunks;
+      auto lookup = [&](int k, int& phys, int& slot) {
+        phys = INT_MIN;
+        slot = 0;
+        const KeyTile t = key_tile<kTN>(j, k);
+        const int tok = t.base + (box << a.lR);
+        if (box < (kTN >> a.lR) && box_seen(j, t, tok, a.R)) {
+          const int pg = a.bs_log2 >= 0 ? tok >> a.bs_log2 : static_cast<int>(fast_div(tok, a.div_bs));
+          slot = tok - pg * p.bs;
+          phys = __ldg(p.bt + j.b * p.bt_sb + pg);
         }
-        if (lane == 0) mbar_expect_tx(kv_full(s), bytes);
-        __syncwarp();
-        if (valid)
-          tma_load_5d(skv + s * C::kKV + chunk * kTN * 128 + (box << a.lR) * 128, kv ? &mv : &mk, 0,
-                      slot, chunk, j.kvh, phys, kv_full(s));
+      };
+      int phys, slot, nphys = INT_MIN, nslot = 0, s = 0;
+      uint32_t phase = 0;
+      if (j.k0 < j.k1) lookup(j.k0, nphys, nslot);
+      for (int k = j.k0; k < j.k1 && ok; ++k) {
+        phys = nphys;
+        slot = nslot;
+        if (k + 1 < j.k1) lookup(k + 1, nphys, nslot);
+        bool valid = phys != INT_MIN;
+        if (valid && (phys < 0 || phys >= p.NB)) {
+          flag(p, PA_STATUS_BAD_BLOCK);
+          valid = false;
+        }
+        const uint32_t bytes = __popc(__ballot_sync(kFull, valid)) * a.R * 128;
+        for (int kv = 0; kv < 2; ++kv) {
+          ok = mbar_wait(kv_empty(s), phase ^ 1);
+          if (!__all_sync(kFull, ok)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_expect_tx(kv_full(s), bytes);
+          __syncwarp();
+          if (valid)
+            tma_load_5d(skv + s * C::kKV + chunk * kTN * 128 + (box << a.lR) * 128, kv ? &mv : &mk, 0,
+                        slot, chunk, j.kvh, phys, kv_full(s));
+          if (++s == C::kSlots) {
+            s = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      if (!ok) {
+        // leave no copy in flight: every slot's last fill (a slot that was never
+        // filled passes as the phase before its first)
+        for (int i = 0; i < C::kSlots; ++i) mbar_wait(kv_full(i), i < s ? phase : phase ^ 1);
+      }
+    }
+    if (warp == NQ * 4 + NQ + C::kProducers) {
+      // ----------------------------------------------------------------- cleaner
+      // Hands each V tile on to the issuing warps, after zeroing the rows of its
+      // multiplied 16-token steps whose tokens no row sees.
+      int s = 0;
+      uint32_t phase = 0;
+      for (int k = j.k0; k < j.k1; ++k) {
+        if (++s == C::kSlots) {      // past the K tile
+          s = 0;
+          phase ^= 1;
+        }
+        ok = __all_sync(kFull, mbar_wait(kv_full(s), phase));
+        if (!ok) break;
+        const KeyTile kt = key_tile<kTN>(j, k);
+        const int v0 = kt.from - kt.base, v1 = kt.to - kt.base;
+        const int c0 = v0 & ~15, c1 = (v1 + 15) & ~15;
+        if (kt.gap || v0 != c0 || v1 != c1) {
+          constexpr int kRowsAtOnce = D / 8 < 32 ? 32 / (D / 8) : 1;
+          const int g0 = kt.gap ? j.sinks - kt.base : c1, g1 = kt.gap ? j.low - kt.base : c1;
+          const int c = lane % (D / 8);
+          for (int r = c0 + lane / (D / 8); r < c1; r += kRowsAtOnce) {
+            if (r >= v0 && r < v1 && !(r >= g0 && r < g1)) continue;
+            asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
+                             skv + s * C::kKV + (c >> 3) * kTN * 128 + r * 128 + (c & 7) * 16),
+                         "r"(0)
+                         : "memory");
+          }
+          fence_async_smem();
+        }
+        mbar_arrive(v_ready(k - j.k0));
         if (++s == C::kSlots) {
           s = 0;
           phase ^= 1;
         }
       }
+      if (!ok && lane == 0) flag(p, PA_STATUS_TIMEOUT);
     }
-    if (!ok) {
-      // leave no copy in flight: every slot's last fill (a slot that was never
-      // filled passes as the phase before its first)
-      for (int i = 0; i < C::kSlots; ++i) mbar_wait(kv_full(i), i < s ? phase : phase ^ 1);
-    }
-  }
-  if (warp == NQ * 4 + NQ + C::kProducers) {
-    // ----------------------------------------------------------------- cleaner
-    // Hands each V tile on to the issuing warps, after zeroing the rows of its
-    // multiplied 16-token steps whose tokens no row sees.
-    int s = 0;
-    uint32_t phase = 0;
-    for (int k = j.k0; k < j.k1; ++k) {
-      if (++s == C::kSlots) {      // past the K tile
-        s = 0;
-        phase ^= 1;
-      }
-      ok = __all_sync(kFull, mbar_wait(kv_full(s), phase));
-      if (!ok) break;
-      const KeyTile kt = key_tile<kTN>(j, k);
-      const int v0 = kt.from - kt.base, v1 = kt.to - kt.base;
-      const int c0 = v0 & ~15, c1 = (v1 + 15) & ~15;
-      if (kt.gap || v0 != c0 || v1 != c1) {
-        constexpr int kRowsAtOnce = D / 8 < 32 ? 32 / (D / 8) : 1;
-        const int g0 = kt.gap ? j.sinks - kt.base : c1, g1 = kt.gap ? j.low - kt.base : c1;
-        const int c = lane % (D / 8);
-        for (int r = c0 + lane / (D / 8); r < c1; r += kRowsAtOnce) {
-          if (r >= v0 && r < v1 && !(r >= g0 && r < g1)) continue;
-          asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(
-                           skv + s * C::kKV + (c >> 3) * kTN * 128 + r * 128 + (c & 7) * 16),
-                       "r"(0)
-                       : "memory");
-        }
-        fence_async_smem();
-      }
-      mbar_arrive(v_ready(k - j.k0));
-      if (++s == C::kSlots) {
-        s = 0;
-        phase ^= 1;
-      }
-    }
-    if (!ok && lane == 0) flag(p, PA_STATUS_TIMEOUT);
-  }
-  if (warp < NQ * 4 + NQ) {
-    // -------------------------------------------------------------- issuing warps
-    // One lane per row tile issues its products. What it runs between them
-    // bounds the kernel (the softmax warps take most issue slots: a wait on a
-    // barrier that is already complete costs ~100-200 cycles, a matrix
-    // instruction of 64 cycles' work ~70): with one warp for both row tiles, whole-
-    // warp waits and descriptors rebuilt per instruction, 8192 tokens, window
-    // 4096, Hq32/Hkv8 took 417 us. So: a warp per row tile, a single lane, the
-    // next keys' wait ahead of P's, no wait between the two products.
-    if (elect_one()) {
-      const int t = warp - NQ * 4;
-      const int n = j.k1 - j.k0;
-      constexpr uint32_t kDescPV = instr_desc<T>(D, true);
-      constexpr uint32_t kStep = C::kKV >> 4;
-      const uint32_t q_desc = smem_desc(sq + t * C::kQTile, 16);
-      const uint32_t k_desc = smem_desc(skv, 16);
-      const uint32_t v_desc = smem_desc(skv, kTN * 128);
-      const uint32_t o_col = tmem + C::kOCol + t * D;
-      const uint32_t s_col = tmem + t * C::kSBufs * kTN;
-      // S from the keys in slot ks
-      auto issue_s = [&](int buf, int ks, const KeyTile& kt) {
-        const uint32_t idesc = instr_desc<T>((kt.to - kt.base + 15) & ~15, false);
-        const uint32_t kb = k_desc + ks * kStep;
+    if (warp < NQ * 4 + NQ) {
+      // -------------------------------------------------------------- issuing warps
+      // One lane per row tile issues its products. What it runs between them
+      // bounds the kernel (the softmax warps take most issue slots: a wait on a
+      // barrier that is already complete costs ~100-200 cycles, a matrix
+      // instruction of 64 cycles' work ~70): with one warp for both row tiles, whole-
+      // warp waits and descriptors rebuilt per instruction, 8192 tokens, window
+      // 4096, Hq32/Hkv8 took 417 us. So: a warp per row tile, a single lane, the
+      // next keys' wait ahead of P's, no wait between the two products.
+      if (elect_one()) {
+        const int t = warp - NQ * 4;
+        const int n = j.k1 - j.k0;
+        constexpr uint32_t kDescPV = instr_desc<T>(D, true);
+        constexpr uint32_t kStep = C::kKV >> 4;
+        const uint32_t q_desc = smem_desc(sq + t * C::kQTile, 16);
+        const uint32_t k_desc = smem_desc(skv, 16);
+        const uint32_t v_desc = smem_desc(skv, kTN * 128);
+        const uint32_t o_col = tmem + C::kOCol + t * D;
+        const uint32_t s_col = tmem + t * C::kSBufs * kTN;
+        // S from the keys in slot ks
+        auto issue_s = [&](int buf, int ks, const KeyTile& kt) {
+          const uint32_t idesc = instr_desc<T>((kt.to - kt.base + 15) & ~15, false);
+          const uint32_t kb = k_desc + ks * kStep;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i)
-          mma_ss(s_col + buf * kTN, q_desc + ((i >> 2) * 128 * 128 + (i & 3) * 32) / 16,
-                 kb + ((i >> 2) * kTN * 128 + (i & 3) * 32) / 16, idesc, i > 0);
-        tc_commit(s_full(t * C::kSBufs + buf));
-      };
-      // O += P V over one half of the tile's 16-token steps, values in slot vs
-      auto issue_o = [&](int buf, int vs, const KeyTile& kt, int half, bool add) {
-        constexpr int kHalf = kTN / 32;
-        const uint32_t pa = s_col + buf * kTN;
-        const uint32_t vb = v_desc + vs * kStep;
-        const int i0 = (kt.from - kt.base) >> 4, i1 = (kt.to - kt.base + 15) >> 4;
-        if (i0 == 0 && i1 == kTN / 16) {
+          for (int i = 0; i < D / 16; ++i)
+            mma_ss(s_col + buf * kTN, q_desc + ((i >> 2) * 128 * 128 + (i & 3) * 32) / 16,
+                   kb + ((i >> 2) * kTN * 128 + (i & 3) * 32) / 16, idesc, i > 0);
+          tc_commit(s_full(t * C::kSBufs + buf));
+        };
+        // O += P V over one half of the tile's 16-token steps, values in slot vs
+        auto issue_o = [&](int buf, int vs, const KeyTile& kt, int half, bool add) {
+          constexpr int kHalf = kTN / 32;
+          const uint32_t pa = s_col + buf * kTN;
+          const uint32_t vb = v_desc + vs * kStep;
+          const int i0 = (kt.from - kt.base) >> 4, i1 = (kt.to - kt.base + 15) >> 4;
+          if (i0 == 0 && i1 == kTN / 16) {
 #pragma unroll
-          for (int i = 0; i < kHalf; ++i)
-            mma_ts(o_col, pa + (half * kHalf + i) * 8, vb + (half * kHalf + i) * (16 * 128 / 16),
-                   kDescPV, i > 0 || half || add);
-        } else {
-          const int e = min(i1, (half + 1) * kHalf);
-          for (int i = max(i0, half * kHalf); i < e; ++i)
-            mma_ts(o_col, pa + i * 8, vb + i * (16 * 128 / 16), kDescPV, i > i0 || add);
+            for (int i = 0; i < kHalf; ++i)
+              mma_ts(o_col, pa + (half * kHalf + i) * 8, vb + (half * kHalf + i) * (16 * 128 / 16),
+                     kDescPV, i > 0 || half || add);
+          } else {
+            const int e = min(i1, (half + 1) * kHalf);
+            for (int i = max(i0, half * kHalf); i < e; ++i)
+              mma_ts(o_col, pa + i * 8, vb + i * (16 * 128 / 16), kDescPV, i > i0 || add);
+          }
+        };
+        auto wait = [&](uint32_t bar, uint32_t parity) {
+          if (ok) ok = mbar_wait(bar, parity);
+          return ok;
+        };
+        // Tile i's keys are fill 2 i of the ring, its values fill 2 i + 1.
+        int ks = 0, vs = 1;
+        uint32_t kph = 0;
+        KeyTile cur = key_tile<kTN>(j, j.k0);
+        // The two row tiles' (P V, next S) blocks alternate on the pipe: mixed, both
+        // would be ready late, and the softmax warps of both would first wait and
+        // then run at the same time.
+        auto my_turn = [&](int block) {
+          return NQ == 1 || (t == 0 && block == 0) || wait(turn(t), (t == 0 ? block - 1 : block) & 1);
+        };
+        auto pass_turn = [&]() {
+          if (NQ == 2) mbar_arrive(turn(1 - t));
+        };
+        if (n > 0 && wait(q_full(t), 0) && wait(kv_full(0), 0) && my_turn(0)) {
+          issue_s(0, 0, cur);
+          if (n > 1) tc_commit(kv_empty(0));
+          pass_turn();
         }
-      };
-      auto wait = [&](uint32_t bar, uint32_t parity) {
-        if (ok) ok = mbar_wait(bar, parity);
-        return ok;
-      };
-      // Tile i's keys are fill 2 i of the ring, its values fill 2 i + 1.
-      int ks = 0, vs = 1;
-      uint32_t kph = 0;
-      KeyTile cur = key_tile<kTN>(j, j.k0);
-      // The two row tiles' (P V, next S) blocks alternate on the pipe: mixed, both
-      // would be ready late, and the softmax warps of both would first wait and
-      // then run at the same time.
-      auto my_turn = [&](int block) {
-        return NQ == 1 || (t == 0 && block == 0) || wait(turn(t), (t == 0 ? block - 1 : block) & 1);
-      };
-      auto pass_turn = [&]() {
-        if (NQ == 2) mbar_arrive(turn(1 - t));
-      };
-      if (n > 0 && wait(q_full(t), 0) && wait(kv_full(0), 0) && my_turn(0)) {
-        issue_s(0, 0, cur);
-        if (n > 1) tc_commit(kv_empty(0));
-        pass_turn();
+        for (int i = 0; i < n && ok; ++i) {
+          const bool more = i + 1 < n;
+          const KeyTile nxt = key_tile<kTN>(j, j.k0 + i + (more ? 1 : 0));
+          ks += 2;
+          if (ks >= C::kSlots) {
+            ks -= C::kSlots;
+            kph ^= 1;
+          }
+          if (more && !wait(kv_full(ks), kph)) break;
+          if (NQ == 1 && more) {
+            // the next tile's S, into the other buffer, during this tile's softmax
+            issue_s((i + 1) & 1, ks, nxt);
+            if (i + 2 < n) tc_commit(kv_empty(ks));
+          }
+          const int buf = NQ == 1 ? i & 1 : 0;
+          if (!wait(v_ready(i), i / C::kVBars & 1) || !wait(p_full(t, 0), i & 1)) break;
+          tc_fence_after();
+          issue_o(buf, vs, cur, 0, i > 0);
+          if (!my_turn(i + 1) || !wait(p_full(t, 1), i & 1)) break;
+          tc_fence_after();
+          issue_o(buf, vs, cur, 1, i > 0);
+          if (NQ == 1 || !more) tc_commit(o_done(t));
+          if (NQ == 2 && more) {
+            issue_s(0, ks, nxt);
+            if (i + 2 < n) tc_commit(kv_empty(ks));
+          }
+          pass_turn();
+          if (more) tc_commit(kv_empty(vs));
+          vs += 2;
+          if (vs >= C::kSlots) vs -= C::kSlots;
+          cur = nxt;
+        }
+        if (!ok) {
+          flag(p, PA_STATUS_TIMEOUT);
+          tc_commit(drained(t));
+          mbar_wait(drained(t), 0);
+        }
       }
-      for (int i = 0; i < n && ok; ++i) {
-        const bool more = i + 1 < n;
-        const KeyTile nxt = key_tile<kTN>(j, j.k0 + i + (more ? 1 : 0));
-        ks += 2;
-        if (ks >= C::kSlots) {
-          ks -= C::kSlots;
-          kph ^= 1;
-        }
-        if (more && !wait(kv_full(ks), kph)) break;
-        if (NQ == 1 && more) {
-          // the next tile's S, into the other buffer, during this tile's softmax
-          issue_s((i + 1) & 1, ks, nxt);
-          if (i + 2 < n) tc_commit(kv_empty(ks));
-        }
-        const int buf = NQ == 1 ? i & 1 : 0;
-        if (!wait(v_ready(i), i / C::kVBars & 1) || !wait(p_full(t, 0), i & 1)) break;
-        tc_fence_after();
-        issue_o(buf, vs, cur, 0, i > 0);
-        if (!my_turn(i + 1) || !wait(p_full(t, 1), i & 1)) break;
-        tc_fence_after();
-        issue_o(buf, vs, cur, 1, i > 0);
-        if (NQ == 1 || !more) tc_commit(o_done(t));
-        if (NQ == 2 && more) {
-          issue_s(0, ks, nxt);
-          if (i + 2 < n) tc_commit(kv_empty(ks));
-        }
-        pass_turn();
-        if (more) tc_commit(kv_empty(vs));
-        vs += 2;
-        if (vs >= C::kSlots) vs -= C::kSlots;
-        cur = nxt;
-      }
-      if (!ok) {
-        flag(p, PA_STATUS_TIMEOUT);
-        tc_commit(drained(t));
-        mbar_wait(drained(t), 0);
-      }
+      __syncwarp();
     }
-    __syncwarp();
-  }
   } else {
     // ----------------------------------------------------------------- softmax
     if constexpr (NQ == 2) regs_up<kSoftmaxRegs>();
@@ -1139,29 +1196,36 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(const TileParams a) {
   if (w >= rows) return;
   const int row = static_cast<int>(w / p.Hq);
   const int hq = static_cast<int>(w - static_cast<long long>(row) * p.Hq);
-  int lo = 0, hi = p.B - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (__ldg(p.starts + mid) <= row) lo = mid; else hi = mid - 1;
-  }
-  bool bad;
-  const Seq s = load_seq(p, lo, bad);
-  if (row < s.start || row >= s.start + s.n) return;
-  float top = kSentinel;
-  for (int k = lane; k < a.splits; k += 32) top = fmaxf(top, a.lse_part[k * rows + w]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, o));
-  float sum = 0.f, acc[N];
+  asm volatile("griddepcontrol.wait;" ::: "memory");   // the splits' partials
+  if (seq_of_row(p, row) < 0) return;
+  // lane = split: its weight, then all splits' rows in flight together
+  float sum = 0.f, acc[N], top = -INFINITY;
 #pragma unroll
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  for (int k = 0; k < a.splits; ++k) {
-    const float l = a.lse_part[k * rows + w];
-    if (l <= -1e29f) continue;
-    const float f = exp2f((l - top) * kLog2e);
-    sum += f;
-    const float* src = a.o_part + (k * rows + w) * D + lane * N;
+  for (int k0 = 0; k0 < a.splits; k0 += 32) {
+    const float l = k0 + lane < a.splits ? __ldcg(a.lse_part + (k0 + lane) * rows + w) : kSentinel;
+    float t = l;
 #pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] = fmaf(f, src[i], acc[i]);
+    for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(kFull, t, o));
+    if (t <= -1e29f) continue;                         // these splits saw nothing
+    t = fmaxf(t, top);
+    const float old = exp2f((top - t) * kLog2e);
+    top = t;
+    sum *= old;
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] *= old;
+    const float mine = l > -1e29f ? exp2f((l - top) * kLog2e) : 0.f;
+    const int cnt = min(32, a.splits - k0);
+#pragma unroll 4
+    for (int k = 0; k < cnt; ++k) {
+      const float f = __shfl_sync(kFull, mine, k);
+      if (f > 0.f) {                                   // (an empty split has no row)
+        const float* src = a.o_part + ((k0 + k) * rows + w) * D + lane * N;
+        sum += f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] = fmaf(f, __ldcg(src + i), acc[i]);
+      }
+    }
   }
   const float inv = sum > 0.f ? 1.f / sum : 0.f;
   uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + row * p.o_st + hq * p.o_sh + lane * N * 2);
@@ -1355,13 +1419,26 @@ static cudaError_t launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, co
   }
   const long long grid = pl.tiles * a.p.Hkv * pl.splits;
   if (grid > 0x7fffffffll) return cudaErrorInvalidConfiguration;
-  prompt_tile_kernel<T, D, NQ>
-      <<<static_cast<unsigned>(grid), C::kThreads, C::kSmem, stream>>>(mk, mv, a);
-  e = cudaGetLastError();
+  // Programmatic stream serialisation: the barriers' and tensor memory's set-up
+  // runs while the previous kernel in the stream ends; griddepcontrol.wait orders
+  // everything else behind it.
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>(grid));
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::kSmem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, prompt_tile_kernel<T, D, NQ>, mk, mv, a);
   if (e == cudaSuccess && pl.splits > 1) {
     const long long warps = static_cast<long long>(a.p.T) * a.p.Hq;
-    prompt_join_kernel<T, D><<<static_cast<unsigned>((warps + 3) / 4), 128, 0, stream>>>(a);
-    e = cudaGetLastError();
+    cfg.gridDim = dim3(static_cast<unsigned>((warps + 3) / 4));
+    cfg.blockDim = dim3(128);
+    cfg.dynamicSmemBytes = 0;
+    e = cudaLaunchKernelEx(&cfg, prompt_join_kernel<T, D>, a);
   }
   return e;
 }
