@@ -265,22 +265,28 @@ struct TC {
   static constexpr int kChunks = D / 64;               // 128-byte chunks of a row
   static constexpr int kQTile = 128 * D * 2;
   static constexpr int kKV = kTN * D * 2;              // one K or V tile
-  static constexpr int kSlots = D == 64 ? 8 : (D == 128 && NQ == 1) ? 6 : 5;
+  static constexpr int kSlots = D == 128 && NQ == 1 ? 6 : 5;
+  // CTAs per SM. head_dim 64 fits two of one row tile each: one's set-up and output
+  // run beside the other's products (8192 tokens, Hq32/Hkv8: 382 us against 410 as
+  // one CTA of two row tiles). At 128 the ring would shrink to two tiles.
+  static constexpr int kCtas = D == 64 ? 2 : 1;
   static constexpr int kSmem = NQ * kQTile + kSlots * kKV + 1024;
-  static constexpr int kSBufs = NQ == 2 ? 1 : 2;       // S buffers per row tile
+  static constexpr int kSBufs = NQ == 2 || kCtas == 2 ? 1 : 2;   // S buffers per row tile
   static constexpr int kOCol = NQ * kSBufs * kTN;      // first TMEM column of O
   // warps: 4 softmax and one issuing warp per row tile, the producers, the cleaner;
-  // NQ = 2: four full warpgroups, whose registers are split unevenly
+  // full warpgroups split their registers unevenly
   static constexpr int kProducers = NQ == 2 ? 4 : 2;
   static constexpr int kThreads = NQ == 2 ? 512 : 128 + (1 + kProducers + 1) * 32;
   // V tiles handed on by the cleaner, at most one ring of them ahead
   static constexpr int kVBars = 4;
   static_assert(2 * kVBars >= kSlots, "V barriers");
   static constexpr int kBars = 2 * kSlots + kVBars + NQ * (7 + kSBufs);
-  static_assert(kOCol + NQ * D <= 512, "tensor memory");
-  static_assert(kSmem <= 232448 - 1024, "shared memory");
+  static constexpr int kTmemCols = 512 / kCtas;
+  // 128 registers a thread at launch, where they are split
+  static constexpr bool kSplitRegs = kThreads * kCtas == 512;
+  static_assert(kOCol + NQ * D <= kTmemCols, "tensor memory");
+  static_assert((kSmem + 2048) * kCtas <= 233472, "shared memory");
 };
-constexpr int kTmemCols = 512;
 constexpr unsigned long long kWaitLimitNs = 2000000000ull;   // 2 s per barrier wait
 constexpr float kRescaleLog2 = 8.f;
 // Registers per thread of a 512-thread CTA: 128 at launch; the two softmax
@@ -288,7 +294,7 @@ constexpr float kRescaleLog2 = 8.f;
 // (At the launch's share the softmax spills, and with shared memory full of tiles
 // the spills miss the first-level cache.)
 constexpr int kLaunchRegs = 128, kSoftmaxRegs = 200, kOtherRegs = 56;
-static_assert(2 * kSoftmaxRegs + 2 * kOtherRegs <= 4 * kLaunchRegs, "register split");
+static_assert(kSoftmaxRegs + kOtherRegs <= 2 * kLaunchRegs, "register split");
 template <int N>
 __device__ __forceinline__ void regs_up() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
@@ -382,8 +388,9 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
                : "memory");
 }
+template <int kCols>
 __device__ __forceinline__ void tmem_free(uint32_t tmem) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kTmemCols)
+  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(kCols)
                : "memory");
 }
 // Shared-memory matrix descriptor, 128-byte swizzle: 8-row groups 1024 bytes
@@ -679,7 +686,7 @@ __device__ __forceinline__ bool find_job(const TileParams& a, Job& j, int* sh) {
 }
 
 template <typename T, int D, int NQ>
-__global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
+__global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
     prompt_tile_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                        const TileParams a) {
   using C = TC<D, NQ>;
@@ -728,7 +735,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
   if (warp == NQ * 4) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(&s_tmem)),
-                 "n"(kTmemCols)
+                 "n"(C::kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
@@ -742,13 +749,13 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = s_tmem;
   if (!found) {
-    if (warp == NQ * 4) tmem_free(tmem);
+    if (warp == NQ * 4) tmem_free<C::kTmemCols>(tmem);
     return;
   }
   bool ok = true;
 
   if (warp >= NQ * 4) {
-    if constexpr (NQ == 2) regs_down<kOtherRegs>();
+    if constexpr (C::kSplitRegs) regs_down<kOtherRegs>();
     if (warp >= NQ * 4 + NQ && warp < NQ * 4 + NQ + C::kProducers) {
       // ---------------------------------------------------------------- producer
       // A box is R token rows of one 64-dim chunk; lane l of producer w has box
@@ -918,20 +925,20 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
             kph ^= 1;
           }
           if (more && !wait(kv_full(ks), kph)) break;
-          if (NQ == 1 && more) {
+          if (C::kSBufs == 2 && more) {
             // the next tile's S, into the other buffer, during this tile's softmax
             issue_s((i + 1) & 1, ks, nxt);
             if (i + 2 < n) tc_commit(kv_empty(ks));
           }
-          const int buf = NQ == 1 ? i & 1 : 0;
+          const int buf = C::kSBufs == 2 ? i & 1 : 0;
           if (!wait(v_ready(i), i / C::kVBars & 1) || !wait(p_full(t, 0), i & 1)) break;
           tc_fence_after();
           issue_o(buf, vs, cur, 0, i > 0);
           if (!my_turn(i + 1) || !wait(p_full(t, 1), i & 1)) break;
           tc_fence_after();
           issue_o(buf, vs, cur, 1, i > 0);
-          if (NQ == 1 || !more) tc_commit(o_done(t));
-          if (NQ == 2 && more) {
+          if (C::kSBufs == 2 || !more) tc_commit(o_done(t));
+          if (C::kSBufs == 1 && more) {
             issue_s(0, ks, nxt);
             if (i + 2 < n) tc_commit(kv_empty(ks));
           }
@@ -951,7 +958,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
     }
   } else {
     // ----------------------------------------------------------------- softmax
-    if constexpr (NQ == 2) regs_up<kSoftmaxRegs>();
+    if constexpr (C::kSplitRegs) regs_up<kSoftmaxRegs>();
     const int t = warp >> 2;
     const int tid = threadIdx.x & 127;
     const int r0 = j.r0 + t * 128;
@@ -991,11 +998,11 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
     const uint32_t o_at = tmem + lanes + C::kOCol + t * D;
     float m = -INFINITY, l = 0.f;
     const int n = j.k1 - j.k0;
-    // NQ = 1: waits for the product of tile i - 1, once per tile and before tile i's
+    // Two S buffers: waits for the product of tile i - 1, once per tile and before tile i's
     // P is handed over, so that no barrier here gets a phase ahead of its reader.
     int waited = 0;
     auto o_free = [&](int i) {
-      if (NQ == 2 || waited == i) return true;
+      if (C::kSBufs == 1 || waited == i) return true;
       ok = mbar_wait(o_done(t), (i - 1) & 1);
       ok = __all_sync(kFull, ok);
       tc_fence_after();
@@ -1003,9 +1010,9 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       return ok;
     };
     for (int i = 0; i < n; ++i) {
-      const int buf = NQ == 1 ? (i & 1) : 0;
+      const int buf = C::kSBufs == 2 ? (i & 1) : 0;
       const uint32_t s_at = tmem + lanes + (t * C::kSBufs + buf) * kTN;
-      ok = mbar_wait(s_full(t * C::kSBufs + buf), NQ == 1 ? (i >> 1) & 1 : i & 1);
+      ok = mbar_wait(s_full(t * C::kSBufs + buf), C::kSBufs == 2 ? (i >> 1) & 1 : i & 1);
       if (!__all_sync(kFull, ok)) {
         ok = false;
         break;
@@ -1044,7 +1051,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
         const float f = mn == -INFINITY ? 1.f : ex2((m - mn) * scl);
         m = mn;
         l *= f;
-        // O is free once the previous tile's product is done (with NQ = 2 the
+        // O is free once the previous tile's product is done (with one S buffer the
         // commit behind this tile's S covers it)
         if (!o_free(i)) break;
 #pragma unroll 1
@@ -1100,7 +1107,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
       l += (x0 + x1) + (x2 + x3);
     }
     if (n > 0 && ok) {
-      ok = mbar_wait(o_done(t), NQ == 1 ? (n - 1) & 1 : 0);
+      ok = mbar_wait(o_done(t), C::kSBufs == 2 ? (n - 1) & 1 : 0);
       ok = __all_sync(kFull, ok);
       tc_fence_after();
     }
@@ -1181,7 +1188,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == NQ * 4) tmem_free(tmem);
+  if (warp == NQ * 4) tmem_free<C::kTmemCols>(tmem);
 }
 
 // Joins the splits of a row: one warp per (row, query head), weights
@@ -1376,7 +1383,8 @@ static Plan make_plan(const pa_prompt_params* p, int sms) {
   const long long packed = static_cast<long long>(p->num_tokens) * g;   // rows of a KV head
   // Two row tiles per CTA keep the matrix pipe busy; a batch whose sequences
   // bring no more than one tile each would leave the second empty.
-  pl.nq = p->head_dim == 256 || packed <= 128ll * p->batch ? 1 : 2;
+  pl.nq = p->head_dim == 256 || p->head_dim == 64 || packed <= 128ll * p->batch ? 1 : 2;
+  const long long slots = static_cast<long long>(sms) * (p->head_dim == 64 ? 2 : 1);   // CTAs at once
   // sum over the sequences of ceil(rows / tile), whatever their shares are
   pl.tiles = packed / (128 * pl.nq) + std::min<long long>(p->batch, p->num_tokens);
   const long long ctas = pl.tiles * p->num_kv_heads;
@@ -1391,7 +1399,7 @@ static Plan make_plan(const pa_prompt_params* p, int sms) {
     const long long seen =
         p->window ? std::min(cap, static_cast<long long>(p->window) + span + p->num_sinks + tn) : cap;
     const long long by_keys = (seen + tn - 1) / tn / 2;
-    pl.splits = static_cast<int>(std::max(1ll, std::min({static_cast<long long>(sms) / ctas, by_keys, 64ll})));
+    pl.splits = static_cast<int>(std::max(1ll, std::min({slots / ctas, by_keys, 64ll})));
   }
   if (pl.splits > 1)
     pl.ws_bytes = static_cast<size_t>(pl.splits) * p->num_tokens * p->num_heads *
@@ -1450,8 +1458,7 @@ static cudaError_t launch_tiles_d(const CUtensorMap& mk, const CUtensorMap& mv, 
   if (D == 128)
     return pl.nq == 2 ? launch_tiles<T, 128, 2>(mk, mv, a, pl, stream)
                       : launch_tiles<T, 128, 1>(mk, mv, a, pl, stream);
-  return pl.nq == 2 ? launch_tiles<T, 64, 2>(mk, mv, a, pl, stream)
-                    : launch_tiles<T, 64, 1>(mk, mv, a, pl, stream);
+  return launch_tiles<T, 64, 1>(mk, mv, a, pl, stream);
 }
 
 }  // namespace pp
