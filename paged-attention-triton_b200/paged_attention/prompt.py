@@ -37,10 +37,14 @@ def paged_prompt_attention(Q: torch.Tensor, K_Cache: torch.Tensor, V_Cache: torc
     ``return_lse=True`` adds ``LSE [T, Hq]`` (fp32, natural log). ``num_splits``: parts of
     the keys that separate CTAs take and a second kernel joins (default: chosen by the
     sizes). Asynchronous on the current stream; scratch comes from ``workspace``
-    (default: the stream's), whose status word gets ``PA_STATUS_*`` bits. Inference only."""
+    (default: the stream's), whose status word gets ``PA_STATUS_*`` bits; as with
+    ``paged_attention``, calls that share one must be ordered, and a graph keeps the one
+    it was captured with, grown by a call before. Inference only."""
     win, sinks = window_args("paged_prompt_attention", window, num_sinks)
     if num_splits is not None and int(num_splits) < 1:
         raise ValueError("paged_prompt_attention: num_splits must be at least 1")
+    if scale is not None and not float(scale) > 0:
+        raise ValueError("paged_prompt_attention: scale must be positive")
     if torch.is_grad_enabled() and (Q.requires_grad or K_Cache.requires_grad
                                     or V_Cache.requires_grad):
         raise RuntimeError("paged_prompt_attention is inference-only.")

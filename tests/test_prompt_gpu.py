@@ -198,6 +198,50 @@ def test_prompt_same_bits_on_every_run_and_stream():
         assert torch.equal(o, o2) and torch.equal(lse, lse2)
 
 
+@pytest.mark.parametrize("count", [31, 32, 33, 300, 1200])
+@pytest.mark.parametrize("d,bs", [(64, 16), (128, 8), (32, 16)])
+def test_prompt_many_sequences(count, d, bs):
+    """More sequences than a warp, than a block: empty ones, single tokens, small chunks."""
+    qs = [(7 * i) % 5 if i % 11 else 23 for i in range(count)]
+    lens = [q + (13 * i) % 70 for i, q in enumerate(qs)]
+    _run(qs, lens, 4, 2, d, bs, torch.float16, 30, 3, seed=count + d, pad=5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hkv,g,d,bs,q,s,window,sinks", [
+    (2, 4, 128, 16, 1500, 3000, 1000, 4),
+    (1, 8, 64, 32, 2000, 2001, None, 0),
+    (4, 1, 128, 128, 900, 5000, 4097, 129),
+    (2, 2, 256, 64, 700, 1400, 513, 65),
+    (1, 5, 128, 8, 1025, 2050, 300, 1),
+])
+def test_prompt_long(dtype, hkv, g, d, bs, q, s, window, sinks):
+    """Many key tiles, against products in 64 bits on the device."""
+    import paged_attention as pa
+    gen = torch.Generator(device="cuda").manual_seed(q)
+    pages = -(-s // bs)
+    k, v = (torch.randn(pages, bs, hkv, d, device="cuda", generator=gen).to(dtype) for _ in range(2))
+    table = torch.randperm(pages, device="cuda", generator=gen).to(torch.int32)[None]
+    x = torch.randn(q, hkv * g, d, device="cuda", generator=gen).to(dtype)
+    lens = torch.tensor([s], dtype=torch.int32, device="cuda")
+    st = torch.tensor([0, q], dtype=torch.int32, device="cuda")
+    o, lse = pa.paged_prompt_attention(x, k, v, table, st, lens, bs, window=window,
+                                       num_sinks=sinks, return_lse=True)
+    t = torch.arange(s, device="cuda")
+    pos = torch.arange(s - q, s, device="cuda")[:, None]
+    seen = (t <= pos) & ((t < sinks) | (t > pos - (window or 10 ** 9)))
+    kk, vv = (c[table[0].long()].reshape(-1, hkv, d)[:s].double() for c in (k, v))
+    half, vmax = torch.finfo(dtype).eps / 2, vv.abs().max().item()
+    for h in range(hkv * g):
+        sc = (x[:, h].double() @ kk[:, h // g].T * d ** -0.5).masked_fill(~seen, float("-inf"))
+        big = (x[:, h].double().abs() @ kk[:, h // g].abs().T * d ** -0.5).amax(1, keepdim=True)
+        norm = torch.logsumexp(sc, 1, keepdim=True)
+        want = (sc - norm).exp() @ vv[:, h // g]
+        tol = half * want.abs() + (half + 2 * d * 2.0 ** -24 * big) * vmax
+        assert_matches(o[:, h], want.cpu(), tol.cpu(), f"head {h}")
+        assert_lse(lse[:, h], norm[:, 0].cpu(), d, f"head {h}")
+
+
 def test_prompt_flags_bad_pages_lengths_and_starts():
     import paged_attention as pa
     from paged_attention import _native
@@ -257,7 +301,7 @@ def test_prompt_refusals_on_the_device():
                 dict(Block_Table=bt.long()), dict(query_starts=st[:2]), dict(seq_lens=st),
                 dict(seq_lens=st[:2].long()), dict(block_size=8), dict(K_Cache=k.cpu()),
                 dict(Q=q.float(), K_Cache=k.float(), V_Cache=k.float()), dict(out=q[:4]),
-                dict(window=0), dict(num_sinks=1), dict(num_splits=0)):
+                dict(window=0), dict(num_sinks=1), dict(num_splits=0), dict(scale=-1.0)):
         with pytest.raises(ValueError):
             pa.paged_prompt_attention(**{**ok, **bad})
 

@@ -79,6 +79,8 @@ def _prompt_args():
     (dict(window=8, num_sinks=-1), "num_sinks must not be negative"),
     (dict(num_sinks=2), "num_sinks goes with a window"),
     (dict(num_splits=0), "num_splits must be at least 1"),
+    (dict(scale=0.0), "scale must be positive"),
+    (dict(scale=float("nan")), "scale must be positive"),
 ])
 def test_prompt_arguments_refused(kw, match):
     with pytest.raises(ValueError, match=match):
