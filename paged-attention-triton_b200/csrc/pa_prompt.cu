@@ -222,9 +222,9 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
 // ----------------------------------------------------------------------------
 // One CTA takes 128 * NQ packed query rows of one (sequence, KV head): row R is
 // token R / G, head R % G of the group, so that the G query heads that share the
-// keys share their tiles. It walks the tiles of kTN keys that any of its rows
-// sees: those that hold visible first tokens, then those from the window's
-// first token to the last row's position. Per tile and 128 rows:
+// keys share their tiles. It walks the keys that any of its rows sees, the visible
+// first tokens and the window's from its first to the last row's position, in
+// tiles of kTN. Per tile and 128 rows:
 //
 //   S (128 x kTN, TMEM) = Q K^T       one tcgen05.mma per 16 dimensions
 //   P = 2^(c S - m), rounded to the 16-bit type, over S in TMEM
@@ -238,8 +238,8 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
 // head_dim 256) S has two buffers and the next tile's S is computed during the
 // current softmax.
 //
-// What bounds it (8192 tokens, Hq32/Hkv8, D 128, window 4096 / none: 368 / 457 us,
-// 1.12 / 1.20 PFLOP/s): the chain from a tile's S to its P. 256 rows x 128 keys
+// What bounds it (8192 tokens, Hq32/Hkv8, D 128, window 4096 / none: 357 / 451 us,
+// 1.15 / 1.22 PFLOP/s): the chain from a tile's S to its P. 256 rows x 128 keys
 // take the matrix pipe 2048 cycles, the special function units as many, and the
 // tile's turn ~3000: load of S 250, maximum 300-400, exponentials 1400 (1024 if no
 // other warp ran), then the rest of P V and the next S 1000. Tried and slower:
@@ -247,7 +247,9 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
 // spill: 481 us where one thread took 425), tiles of 64 keys with two S buffers
 // (S is no longer waited for, but every tile's fixed costs double and the row
 // tile is read twice as often: 418 against 388), P formed against the previous
-// maximum while the new one is taken (430 against 388).
+// maximum while the new one is taken (430 against 388), a grid of one CTA
+// per SM that walks its jobs with the next keys already loading (376 against 361;
+// the hardware's order of CTAs balances better than any fixed one).
 //
 // P is rounded to the operand type once (half a step, relative); its sum, the
 // maxima and O are kept in 32 bits. O is rescaled only when a row's maximum has
@@ -306,7 +308,7 @@ __device__ __forceinline__ void regs_down() {
 
 struct TileParams {
   Params p;
-  int R, lR;                // token rows per TMA box: gcd(page, tile), and its log2
+  int R, lR;                // token rows per TMA box, and its log2
   int bs_log2;              // log2 of the page size, or -1
   FastDiv div_g, div_bs;
   int splits;
@@ -566,34 +568,33 @@ __device__ __forceinline__ void tmem_st(uint32_t addr, const uint32_t (&r)[32]) 
 __device__ __forceinline__ uint32_t ones_below(int n) {
   return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1;
 }
-// A CTA's work: its rows and the key tiles they see.
+// A CTA's work: its rows and the keys they see. The keys are numbered without
+// those that no row sees: the sinks, rounded up to whole boxes of R tokens
+// (`sink_keys`), then the window from the box of its first token on; key v is
+// token v, or v + delta behind the sinks. Tiles are kTN of these keys, so that a
+// few sinks cost a few keys and not a tile, and the window starts at a tile's
+// first columns whatever its place (ragged batch of 8, window 777: 51 us against
+// 61 with separate, aligned tiles).
 struct Job {
   int b, kvh, split;
   Seq s;
   int r0, rows;             // first packed row, packed rows of the sequence
-  int low, hi;              // window: tokens [low, hi) are seen by some row
-  int first, nsink, sink_end;   // first window tile; sink tiles, of tokens [0, sink_end)
-  int sinks;
+  int sink_keys, delta;
+  int gap0, gap1;           // keys [gap0, gap1) are seen by no row
+  int end;                  // keys
+  int sinks;                // visible first tokens (at most the sequence)
   int k0, k1;               // tiles of this CTA
 };
-// First token; some row sees the tokens [from, to) of the tile. `gap`: except
-// [sinks, low), where the window's first tile holds the last sinks too.
-struct KeyTile { int base, from, to, gap; };
+// A tile's first key, and the range [from, to) of its keys that some row sees
+// (except those in the gap).
+struct KeyTile { int base, from, to; };
 template <int kTN>
 __device__ __forceinline__ KeyTile key_tile(const Job& j, int k) {
   KeyTile t;
-  const bool sink = k < j.nsink;
-  t.base = (sink ? k : j.first + k - j.nsink) * kTN;
-  t.gap = !sink && t.base < j.sinks && t.base < j.low;
-  t.from = sink || t.gap ? t.base : max(t.base, j.low);
-  t.to = min(t.base + kTN, sink ? j.sink_end : j.hi);
+  t.base = k * kTN;
+  t.from = t.base >= j.gap0 && t.base < j.gap1 ? j.gap1 : t.base;
+  t.to = min(t.base + kTN, j.end);
   return t;
-}
-
-// Whether some row sees a token of the box of R tokens from `tok` on (else its
-// page is not read).
-__device__ __forceinline__ bool box_seen(const Job& j, const KeyTile& t, int tok, int R) {
-  return tok < t.to && tok + R > t.from && !(t.gap && tok >= j.sinks && tok + R <= j.low);
 }
 
 // The job of block x, or false. Tiles are numbered from the last sequence's last
@@ -673,13 +674,23 @@ __device__ __forceinline__ bool find_job(const TileParams& a, Job& j, int* sh) {
   const int pos0 = j.s.S - j.s.n;
   const int last = min(j.r0 + kRows, j.rows) - 1;
   const int pmin = pos0 + static_cast<int>(fast_div(j.r0, a.div_g));
-  j.hi = max(0, pos0 + static_cast<int>(fast_div(last, a.div_g)) + 1);
-  j.low = pmin >= p.window ? pmin - p.window + 1 : 0;
-  j.sinks = p.sinks;
-  j.first = j.low / kTN;
-  j.sink_end = min(p.sinks, j.first * kTN);
-  j.nsink = (j.sink_end + kTN - 1) / kTN;
-  const int tiles = j.hi > 0 ? j.nsink + (j.hi - 1) / kTN - j.first + 1 : 0;
+  // tokens [low, hi) are in the window of some row
+  const int hi = max(0, pos0 + static_cast<int>(fast_div(last, a.div_g)) + 1);
+  const int low = pmin >= p.window ? pmin - p.window + 1 : 0;
+  const int first = low >> a.lR << a.lR;
+  j.sinks = min(p.sinks, j.s.S);
+  j.sink_keys = (j.sinks + a.R - 1) >> a.lR << a.lR;
+  if (first <= j.sink_keys) {          // one range
+    j.sink_keys = j.delta = 0;
+    j.gap0 = min(j.sinks, low);
+    j.gap1 = low;
+  } else {
+    j.delta = first - j.sink_keys;
+    j.gap0 = j.sinks;
+    j.gap1 = low - j.delta;
+  }
+  j.end = hi - j.delta;
+  const int tiles = hi > 0 ? (j.end + kTN - 1) / kTN : 0;
   j.k0 = static_cast<int>(static_cast<long long>(tiles) * j.split / a.splits);
   j.k1 = static_cast<int>(static_cast<long long>(tiles) * (j.split + 1) / a.splits);
   return true;
@@ -767,9 +778,10 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
       auto lookup = [&](int k, int& phys, int& slot) {
         phys = INT_MIN;
         slot = 0;
-        const KeyTile t = key_tile<kTN>(j, k);
-        const int tok = t.base + (box << a.lR);
-        if (box < (kTN >> a.lR) && box_seen(j, t, tok, a.R)) {
+        const int key = k * kTN + (box << a.lR);
+        // a box in which no row sees a token is not read
+        if (box < (kTN >> a.lR) && key < j.end && !(key >= j.gap0 && key + a.R <= j.gap1)) {
+          const int tok = key < j.sink_keys ? key : key + j.delta;
           const int pg = a.bs_log2 >= 0 ? tok >> a.bs_log2 : static_cast<int>(fast_div(tok, a.div_bs));
           slot = tok - pg * p.bs;
           phys = __ldg(p.bt + j.b * p.bt_sb + pg);
@@ -827,9 +839,9 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
         const KeyTile kt = key_tile<kTN>(j, k);
         const int v0 = kt.from - kt.base, v1 = kt.to - kt.base;
         const int c0 = v0 & ~15, c1 = (v1 + 15) & ~15;
-        if (kt.gap || v0 != c0 || v1 != c1) {
+        const int g0 = j.gap0 - kt.base, g1 = j.gap1 - kt.base;
+        if (v0 != c0 || v1 != c1 || (g0 < c1 && g1 > c0 && g0 < g1)) {
           constexpr int kRowsAtOnce = D / 8 < 32 ? 32 / (D / 8) : 1;
-          const int g0 = kt.gap ? j.sinks - kt.base : c1, g1 = kt.gap ? j.low - kt.base : c1;
           const int c = lane % (D / 8);
           for (int r = c0 + lane / (D / 8); r < c1; r += kRowsAtOnce) {
             if (r >= v0 && r < v1 && !(r >= g0 && r < g1)) continue;
@@ -990,9 +1002,10 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
     const bool live = pr < j.rows;
     const int tok = live ? static_cast<int>(fast_div(pr, a.div_g)) : 0;
     const int pos = j.s.S - j.s.n + tok;
-    // the row sees tokens t < hi with t >= low or t < sinks
-    const int hi = live ? max(pos + 1, 0) : 0;
-    const int low = pos >= p.window ? pos - p.window + 1 : 0;
+    // the row sees keys v < hi with v >= low or v < sinks (its tokens t <= pos with
+    // t > pos - window or t < sinks; behind sinks of their own, delta keys are left out)
+    const int hi = live ? max(pos + 1 - j.delta, 0) : 0;
+    const int low = (pos >= p.window ? pos - p.window + 1 : 0) - j.delta;
     const float scl = p.scale_log2;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;   // TMEM lane 32 * (warp % 4)
     const uint32_t o_at = tmem + lanes + C::kOCol + t * D;
@@ -1025,14 +1038,16 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
 #pragma unroll
       for (int c = 0; c < kTN; ++c) s[c] = __uint_as_float(raw[c]);
       if (__any_sync(kFull, hi < base + kTN || low > base)) {
-        const int h = hi - base, lo = low - base, sk = p.sinks - base;
+        const int h = hi - base, lo = low - base, sk = j.sinks - base;
 #pragma unroll
         for (int c0 = 0; c0 < kTN; c0 += 32) {
           // 32 columns' visibility as one word
           const uint32_t seen = ones_below(h - c0) & (~ones_below(lo - c0) | ones_below(sk - c0));
+          if (__any_sync(kFull, ~seen)) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            s[c0 + c] = seen & 1u << c ? s[c0 + c] : -INFINITY;
+            for (int c = 0; c < 32; ++c)
+              s[c0 + c] = seen & 1u << c ? s[c0 + c] : -INFINITY;
+          }
         }
       }
       float mx[4] = {s[0], s[1], s[2], s[3]};
@@ -1502,8 +1517,10 @@ pa_status_t pa_prompt(const pa_prompt_params* p, cudaStream_t stream) {
     return e == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
   }
   const int tn = p->head_dim == 256 ? 64 : 128;
-  a.R = 8;                                   // the largest power of two in both
-  while (a.R < tn && p->block_size % (2 * a.R) == 0) a.R *= 2;
+  // box rows: a power of two in the page size, at most 32 (where a window starts,
+  // up to R - 1 hidden keys are read)
+  a.R = 8;
+  while (a.R < 32 && p->block_size % (2 * a.R) == 0) a.R *= 2;
   a.lR = 0;
   while ((1 << a.lR) < a.R) ++a.lR;
   a.bs_log2 = -1;
