@@ -258,6 +258,15 @@ typedef struct pa_page_pool {
 PA_API pa_status_t pa_pages_scratch(const pa_page_pool* pool, int32_t rows, int32_t pairs,
                                     size_t* ints);
 
+/* Sets the counts and free bits from tables made elsewhere: page i is used once by
+ * every entry j < ceil(seq_lens[r] / block_size) that names it, pages that none
+ * names are free (rows 0: all are). Entries other than -1 that are no page of the
+ * pool count for nothing (PA_STATUS_BAD_BLOCK); lengths outside the table are cut
+ * (PA_STATUS_BAD_SEQLEN). */
+PA_API pa_status_t pa_pages_adopt(const pa_page_pool* pool, const int32_t* block_table,
+                                  int64_t bt_stride_b, int32_t rows, int32_t max_blocks,
+                                  const int32_t* seq_lens, cudaStream_t stream);
+
 /* Row r goes from seq_lens[r] to new_lens[r] tokens (negative: the row is left
  * alone). First every row releases its pages behind the new length and, with a
  * window (window > 0), the pages in which no token is visible to the next

@@ -327,6 +327,54 @@ __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Resize a) {
 }
 
 // ----------------------------------------------------------------------------
+// adopt
+// ----------------------------------------------------------------------------
+struct Adopt {
+  Pool p;
+  const int* bt;
+  long long sb;
+  int rows, width;
+  const int* lens;
+};
+
+// Counts the entries in use (the counts start at zero); the last block to arrive
+// makes the free bits from the counts.
+__global__ void __launch_bounds__(kPlanThreads) adopt_kernel(const Adopt a) {
+  __shared__ int s_last;
+  const Pool& p = a.p;
+  grid_wait();
+  for (int r = blockIdx.x; r < a.rows; r += gridDim.x) {
+    const int S = __ldg(a.lens + r);
+    const long long cap = static_cast<long long>(a.width) * p.bs;
+    if ((S < 0 || S > cap) && threadIdx.x == 0) flag(p, PA_STATUS_BAD_SEQLEN);
+    const int used = S <= 0 ? 0 : S > cap ? a.width : (S + p.bs - 1) / p.bs;
+    for (int j = threadIdx.x; j < used; j += blockDim.x) {
+      const int e = __ldg(a.bt + r * a.sb + j);
+      if (in_pool(p, e))
+        atomicAdd(p.refs + e, 1);
+      else if (e != -1)
+        flag(p, PA_STATUS_BAD_BLOCK);
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    __threadfence();
+    s_last = atomicAdd(p.scratch + kHArrive, 1) == static_cast<int>(gridDim.x) - 1;
+    __threadfence();
+  }
+  __syncthreads();
+  if (!s_last) return;
+  if (threadIdx.x == 0) p.scratch[kHArrive] = 0;
+  // a warp per word: lane = bit
+  const int lane = threadIdx.x & 31;
+  for (int w = threadIdx.x >> 5; w < p.nwords; w += blockDim.x >> 5) {
+    const int page = w * 32 + lane;
+    const unsigned bits = __ballot_sync(kFull, page < p.NB && __ldcg(p.refs + page) == 0);
+    if (lane == 0) p.words[w] = bits;
+  }
+}
+
+// ----------------------------------------------------------------------------
 // Copies
 // ----------------------------------------------------------------------------
 // A unit is one 32 KB part of the used slots of one page in one cache: all eight
@@ -739,6 +787,26 @@ pa_status_t pa_pages_scratch(const pa_page_pool* pool, int32_t rows, int32_t pai
   if (!pool || !ints || pool->num_blocks <= 0 || rows < 0 || pairs < 0) return PA_ERR_ARG;
   *ints = scratch_ints(pool, rows, pairs);
   return PA_OK;
+}
+
+pa_status_t pa_pages_adopt(const pa_page_pool* pool, const int32_t* block_table,
+                           int64_t bt_stride_b, int32_t rows, int32_t max_blocks,
+                           const int32_t* seq_lens, cudaStream_t stream) {
+  Adopt a;
+  const pa_status_t s = make_pool(pool, rows, 0, a.p);
+  if (s != PA_OK) return s;
+  if (max_blocks < 0 || (rows > 0 && (!seq_lens || (max_blocks > 0 && !block_table))))
+    return PA_ERR_ARG;
+  const int sms = pa_device_sm_count();
+  if (sms <= 0) return PA_ERR_LAUNCH;
+  a.bt = block_table;
+  a.sb = bt_stride_b;
+  a.rows = rows;
+  a.width = max_blocks;
+  a.lens = seq_lens;
+  cudaError_t e = cudaMemsetAsync(a.p.refs, 0, sizeof(int32_t) * static_cast<size_t>(a.p.NB), stream);
+  if (e == cudaSuccess) e = launch(adopt_kernel, std::min(rows, sms), kPlanThreads, a, stream);
+  return e == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 }
 
 pa_status_t pa_pages_resize(const pa_page_pool* pool, int32_t* block_table, int64_t bt_stride_b,

@@ -375,6 +375,23 @@ class PagePool {
     pool_.free_words = reinterpret_cast<uint32_t*>(words_.data_ptr<int32_t>());
     pool_.status = reinterpret_cast<uint32_t*>(status_.data_ptr<int32_t>());
     ensure(1024, 1024);
+    // all pages free
+    done(pa_pages_adopt(&pool_, nullptr, 0, 0, 0, nullptr, stream()), "pa_pages_adopt");
+  }
+
+  // Returns the call's own status word.
+  at::Tensor adopt(const at::Tensor& bt, const at::Tensor& lens) {
+    table(bt);
+    rows(lens, bt, "seq_lens");
+    c10::cuda::CUDAGuard guard(device_);
+    ensure(bt.size(0), 0);
+    at::Tensor word = at::zeros({1}, state_.options());
+    pa_page_pool q = pool_;
+    q.status = reinterpret_cast<uint32_t*>(word.data_ptr<int32_t>());
+    done(pa_pages_adopt(&q, bt.data_ptr<int32_t>(), bt.stride(0), n(bt, 0), n(bt, 1),
+                        lens.data_ptr<int32_t>(), stream()),
+         "pa_pages_adopt");
+    return word;
   }
 
   void resize(const at::Tensor& bt, const at::Tensor& lens, const at::Tensor& new_lens,
@@ -471,6 +488,7 @@ PYBIND11_MODULE(_pa_ext, m) {
   py::class_<PagePool>(m, "PagePool")
       .def(py::init<std::vector<at::Tensor>, std::vector<at::Tensor>, int64_t, int64_t,
                     const at::Device&>())
+      .def("adopt", &PagePool::adopt)
       .def("resize", &PagePool::resize)
       .def("fork", &PagePool::fork)
       .def("compact", &PagePool::compact)

@@ -212,6 +212,9 @@ _SIGNATURES = {
     "pa_prompt": (ctypes.c_int, [ctypes.POINTER(PromptParams), ctypes.c_void_p]),
     "pa_pages_scratch": (ctypes.c_int, [ctypes.POINTER(PagePoolParams), ctypes.c_int32,
                                         ctypes.c_int32, ctypes.POINTER(ctypes.c_size_t)]),
+    "pa_pages_adopt": (ctypes.c_int, [ctypes.POINTER(PagePoolParams), ctypes.c_void_p,
+                                      ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
+                                      ctypes.c_void_p, ctypes.c_void_p]),
     "pa_pages_resize": (ctypes.c_int, [ctypes.POINTER(PagePoolParams), ctypes.c_void_p,
                                        ctypes.c_int64, ctypes.c_int32, ctypes.c_int32,
                                        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int32,

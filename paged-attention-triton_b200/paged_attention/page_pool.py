@@ -51,30 +51,17 @@ class PagePool:
         self.refs = self._pool.refs
         self.free_words = self._pool.free_words
         self.status = self._pool.status
-        self._mark_free()
-
-    def _mark_free(self) -> None:
-        """Free bits from the counts."""
-        words = self.free_words.numel()
-        bits = torch.zeros(words * 32, dtype=torch.int64, device=self.device)
-        bits[: self.num_blocks] = self.refs == 0
-        weight = 1 << torch.arange(32, dtype=torch.int64, device=self.device)
-        value = (bits.view(words, 32) * weight).sum(1)
-        # the same 32 bits as a signed number
-        value = torch.where(value >= 1 << 31, value - (1 << 32), value)
-        self.free_words.copy_(value.to(torch.int32))
 
     def adopt(self, block_table: torch.Tensor, seq_lens: torch.Tensor) -> None:
         """Take over tables made elsewhere: the pages that ``block_table``'s rows use
         (entries ``j < ceil(seq_lens / block_size)`` that are not -1) get their
-        counts, all others become free."""
-        j = torch.arange(block_table.shape[1], device=block_table.device)
-        pages = -(-seq_lens.to(torch.int64) // self.block_size)
-        used = block_table[(j < pages[:, None]) & (block_table != -1)].to(torch.int64)
-        if used.numel() and not (0 <= int(used.min()) and int(used.max()) < self.num_blocks):
+        counts, all others become free. Raises (after a host read) if an entry in use
+        is no page of the pool or a length exceeds the table."""
+        status = int(self._pool.adopt(block_table, seq_lens).item())
+        if status & _native.PA_STATUS_BAD_BLOCK:
             raise ValueError("PagePool.adopt: Block_Table names pages outside the pool")
-        self.refs.copy_(torch.bincount(used, minlength=self.num_blocks).to(torch.int32))
-        self._mark_free()
+        if status:
+            raise ValueError("PagePool.adopt: seq_lens exceeds the Block_Table capacity")
 
     def resize(self, block_table: torch.Tensor, seq_lens: torch.Tensor, new_lens: torch.Tensor, *,
                window: Optional[int] = None, num_sinks: int = 0) -> None:

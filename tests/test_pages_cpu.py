@@ -75,6 +75,9 @@ def test_calls_checked():
     assert lib.pa_pages_fork(ref, at, 4, 2, 4, at, at, at, -1, None) == bad
     assert lib.pa_pages_compact(ref, at, 4, 2, 4, None, None) == bad
     assert lib.pa_pages_scratch(ref, 2, 2, None) == bad
+    assert lib.pa_pages_adopt(ref, at, 4, 2, 4, None, None) == bad
+    assert lib.pa_pages_adopt(ref, None, 4, 2, 4, at, None) == bad
+    assert lib.pa_pages_adopt(ref, at, 4, 2, -1, at, None) == bad
     # nothing to do: no launch, so this works without a GPU
     assert lib.pa_pages_resize(ref, at, 4, 0, 4, at, at, 0, 0, None) == _native.PA_OK
     assert lib.pa_pages_fork(ref, at, 4, 2, 4, at, at, at, 0, None) == _native.PA_OK

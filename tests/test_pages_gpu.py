@@ -171,6 +171,12 @@ def test_adopt_counts_the_pages_in_use():
     w.block_table[0, 0] = 40
     with pytest.raises(ValueError, match="outside the pool"):
         pool.adopt(w.block_table, lens)
+    w.block_table[0, 0] = 0
+    lens[1] = 5 * 16 + 1
+    with pytest.raises(ValueError, match="capacity"):
+        pool.adopt(w.block_table, lens)
+    with pytest.raises(ValueError):
+        pool.adopt(w.block_table, lens.long())
 
 
 def test_captured_step_replays_on_current_state():

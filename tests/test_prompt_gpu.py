@@ -242,6 +242,37 @@ def test_prompt_long(dtype, hkv, g, d, bs, q, s, window, sinks):
         assert_lse(lse[:, h], norm[:, 0].cpu(), d, f"head {h}")
 
 
+def test_prompt_and_decode_on_two_streams_at_once():
+    """Calls that share no workspace, running side by side, give what they give alone."""
+    import paged_attention as pa
+    jobs = []
+    for i, (hkv, g, d) in enumerate([(2, 4, 128), (4, 2, 64), (2, 2, 256)]):
+        qs, lens = [700, 3, 90], [900, 2000, 90]
+        c = PoisonedCache(lens, qs, hkv, d, 16, torch.bfloat16, 400, 4, i)
+        q = torch.randn(sum(qs), hkv * g, d, device="cuda").bfloat16()
+        st = torch.tensor(_starts(qs), dtype=torch.int32, device="cuda")
+        last = q[st[1:].long() - 1].contiguous()
+        jobs.append((c, q, st, last))
+
+    def both(job):
+        c, q, st, last = job
+        return (pa.paged_prompt_attention(q, c.k, c.v, c.table, st, c.lens, 16, window=400, num_sinks=4),
+                pa.paged_attention(last, c.k, c.v, c.table, c.lens, 16, window=400, num_sinks=4))
+
+    alone = [both(j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    got = [[] for _ in jobs]
+    for _ in range(4):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(both(jobs[i]))
+    torch.cuda.synchronize()
+    for want, outs in zip(alone, got):
+        for o in outs:
+            assert torch.equal(o[0], want[0]) and torch.equal(o[1], want[1])
+
+
 def test_prompt_flags_bad_pages_lengths_and_starts():
     import paged_attention as pa
     from paged_attention import _native

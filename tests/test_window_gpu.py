@@ -135,6 +135,17 @@ def test_window_decode_on_another_stream():
     assert_matches(o, want, tol, "side stream")
 
 
+@pytest.mark.parametrize("d,variants", [(128, (1, 2, 3, 4, 5, 10)), (64, (3, 5, 8)), (256, (6, 7, 9))])
+@pytest.mark.parametrize("g", [1, 4, 8])
+def test_window_decode_every_variant(d, variants, g):
+    lens = [1, 30, 31, 140, 900, 0, 333]
+    for v in variants:
+        c, q, o, lse = _run(lens, 2 * g, 2, d, 16, torch.bfloat16, 100, 20, seed=v, kernel_variant=v)
+        want, wl, tol = reference(q, c.k, c.v, c.table, c.lens, 16, 100, 20)
+        assert_matches(o, want, tol, f"variant {v}")
+        assert_lse(lse, wl, d, f"variant {v}")
+
+
 def test_window_decode_flags_bad_page_and_length():
     """A visible page outside the pool and a length beyond the table are flagged, not fatal;
     an invisible page may be anything."""
