@@ -34,7 +34,7 @@ int dtype_code(const at::Tensor& t) {
 // Returns (status, tensors): status 0 and [out[, lse][, o_partial, lse_partial]]
 // on success; when the workspace is too small nothing is launched and the
 // result is (-1, []) with the needed sizes in the last two fields.
-std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> decode(
+std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> window_decode(
     const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& bt,
     const c10::optional<at::Tensor>& seq_lens, int64_t seq_len, int64_t block_size,
     int64_t num_splits, double scale, bool return_lse, bool return_partials,
@@ -167,6 +167,19 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> decode(
     res.push_back(lse_part);
   }
   return {0, std::move(res), 0, 0};
+}
+
+// The full-length step: its argument list, and with it the cost of a call, is the
+// shorter one.
+std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> decode(
+    const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& bt,
+    const c10::optional<at::Tensor>& seq_lens, int64_t seq_len, int64_t block_size,
+    int64_t num_splits, double scale, bool return_lse, bool return_partials,
+    const at::Tensor& ws_buffer, const at::Tensor& ws_counters, const at::Tensor& ws_status,
+    int64_t kernel_variant, const c10::optional<at::Tensor>& out_opt) {
+  return window_decode(q, k, v, bt, seq_lens, seq_len, block_size, num_splits, scale, return_lse,
+                       return_partials, ws_buffer, ws_counters, ws_status, kernel_variant, out_opt,
+                       0, 0);
 }
 
 // Prompt attention (prompt.py): (status, [out[, lse]], bytes); status -1: the
@@ -497,5 +510,6 @@ PYBIND11_MODULE(_pa_ext, m) {
       .def_readonly("free_words", &PagePool::words_)
       .def_readonly("status", &PagePool::status_);
   m.def("prompt", &prompt, "prompt attention over paged caches (see prompt.py)");
+  m.def("window_decode", &window_decode, "a decode step under a sliding window");
   m.def("decode", &decode, "one paged-attention decode step (see torch_kernel.py)");
 }

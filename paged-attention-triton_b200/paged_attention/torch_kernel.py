@@ -152,7 +152,9 @@ def _decode(Q: torch.Tensor, K_Cache: torch.Tensor, V_Cache: torch.Tensor,
             kernel_variant: int = 0, window: Optional[int] = None, num_sinks: int = 0):
     # Argument checks, allocation of the outputs and the launch happen in C++
     # (paged_attention/_pa_ext, csrc/torch_ext.cpp) over the C ABI.
-    win, sinks = window_args("paged_attention", window, num_sinks)
+    windowed = window is not None or num_sinks
+    if windowed:
+        win, sinks = window_args("paged_attention", window, num_sinks)
     if not (Q.is_cuda and K_Cache.is_cuda and V_Cache.is_cuda and Block_Table.is_cuda):
         raise ValueError("paged_attention: Q, K_Cache, V_Cache and Block_Table must be CUDA tensors")
     ws = workspace if workspace is not None else default_workspace(Q.device)
@@ -164,12 +166,13 @@ def _decode(Q: torch.Tensor, K_Cache: torch.Tensor, V_Cache: torch.Tensor,
     args = (Q, K_Cache, V_Cache, Block_Table, seq_t, seq_i, int(block_size), ns,
             0.0 if scale is None else float(scale), bool(return_lse), bool(return_partials))
     ext = _native.ext()
-    status, res, need_bytes, need_counters = ext.decode(
-        *args, ws.buffer, ws.counters, ws.status, int(kernel_variant), out, win, sinks)
+    step, tail = (ext.window_decode, (win, sinks)) if windowed else (ext.decode, ())
+    status, res, need_bytes, need_counters = step(
+        *args, ws.buffer, ws.counters, ws.status, int(kernel_variant), out, *tail)
     if status != 0:
         ws.ensure(need_bytes, need_counters)
-        status, res, _, _ = ext.decode(*args, ws.buffer, ws.counters, ws.status,
-                                       int(kernel_variant), out, win, sinks)
+        status, res, _, _ = step(*args, ws.buffer, ws.counters, ws.status, int(kernel_variant),
+                                 out, *tail)
         if status != 0:
             raise PagedAttentionError("pa_decode", _native.PA_ERR_WORKSPACE)
     return res[0] if len(res) == 1 else tuple(res)
