@@ -118,12 +118,13 @@ __device__ __forceinline__ int seq_of_row(const Params& p, int row) {
 }
 
 // ----------------------------------------------------------------------------
-// CUDA-core path: every shape
+// CUDA-core path: head_dim 32
 // ----------------------------------------------------------------------------
 // One warp per (query row, query head): lane j scores the j-th token of 32
 // against the query (in shared memory), then the lanes, each owning D/32
-// dimensions, accumulate p_j v_j. It serves head_dim 32 and pages that are not
-// a multiple of 8 tokens, which the tile kernel's copies do not cover.
+// dimensions, accumulate p_j v_j. It serves head_dim 32, whose 64-byte rows the
+// tile kernel's layout does not cover (and was the first form of every shape: 87 ms
+// for 8192 tokens, window 4096, Hq32/Hkv8).
 template <typename T, int D>
 __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
   constexpr int N = D / 32;
@@ -696,7 +697,7 @@ __device__ __forceinline__ bool find_job(const TileParams& a, Job& j, int* sh) {
   return true;
 }
 
-template <typename T, int D, int NQ>
+template <typename T, int D, int NQ, bool kGather>
 __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
     prompt_tile_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                        const TileParams a) {
@@ -727,7 +728,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
   auto s_full = [&](int i) { return bar1 + (7 * NQ + i) * 8; };
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kSlots; ++s) {
-      mbar_init(kv_full(s), C::kProducers);
+      mbar_init(kv_full(s), kGather ? C::kProducers * 32 : C::kProducers);
       mbar_init(kv_empty(s), NQ);
     }
     for (int i = 0; i < C::kVBars; ++i) mbar_init(v_ready(i), 32);
@@ -769,6 +770,72 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
     if constexpr (C::kSplitRegs) regs_down<kOtherRegs>();
     if (warp >= NQ * 4 + NQ && warp < NQ * 4 + NQ + C::kProducers) {
       // ---------------------------------------------------------------- producer
+      if constexpr (kGather) {
+        // Pages whose size is not a multiple of 8 tokens: rows by cp.async, 16 bytes a
+        // thread and copy, to where a box would put them. Up to kFly tiles' copies
+        // stay in flight per thread; a tile is handed over when its own have landed
+        // (and the fence has made them visible to the matrix pipe). 8192 tokens,
+        // window 4096, Hq32/Hkv8: pages of 1 and 4 tokens 1049 and 803 us, of 16 by TMA
+        // 357; bound by the copies' address arithmetic beside the softmax warps.
+        constexpr int kPer = D / 8, kThr = C::kProducers * 32, kRows = kTN * kPer / kThr;
+        constexpr int kFly = 2;
+        static_assert(kThr % kPer == 0, "rows per pass");
+        const int me = threadIdx.x - (NQ * 4 + NQ) * 32;
+        const int c = me % kPer, first = me / kPer;
+        int s = 0, out = 0, fills = 0;          // slot to fill, slot to hand over next
+        uint32_t phase = 0;
+        auto hand_over = [&]() {
+          fence_async_smem();
+          mbar_arrive(kv_full(out));
+          if (++out == C::kSlots) out = 0;
+        };
+        for (int k = j.k0; k < j.k1 && ok; ++k) {
+          int page[kRows];
+#pragma unroll
+          for (int i = 0; i < kRows; ++i) {
+            const int key = k * kTN + first + i * (kThr / kPer);
+            page[i] = -1;
+            if (key < j.end && !(key >= j.gap0 && key < j.gap1)) {
+              const int tok = key < j.sink_keys ? key : key + j.delta;
+              page[i] = __ldg(p.bt + j.b * p.bt_sb + static_cast<int>(fast_div(tok, a.div_bs)));
+              if (page[i] < 0 || page[i] >= p.NB) {
+                flag(p, PA_STATUS_BAD_BLOCK);
+                page[i] = -1;
+              }
+            }
+          }
+          for (int kv = 0; kv < 2; ++kv) {
+            ok = __all_sync(kFull, mbar_wait(kv_empty(s), phase ^ 1));
+            if (!ok) break;
+            const char* base = (kv ? p.vc + j.kvh * p.v_sh : p.kc + j.kvh * p.k_sh) + c * 16;
+            const long long sb = kv ? p.v_sb : p.k_sb, ss = kv ? p.v_ss : p.k_ss;
+#pragma unroll
+            for (int i = 0; i < kRows; ++i) {
+              const int r = first + i * (kThr / kPer);
+              if (page[i] < 0) continue;
+              const int key = k * kTN + r;
+              const int tok = key < j.sink_keys ? key : key + j.delta;
+              const int slot = tok - static_cast<int>(fast_div(tok, a.div_bs)) * p.bs;
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+                               skv + s * C::kKV + (c >> 3) * kTN * 128 + r * 128 +
+                               (((c & 7) ^ (r & 7)) << 4)),
+                           "l"(base + page[i] * sb + slot * ss)
+                           : "memory");
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            if (++s == C::kSlots) {
+              s = 0;
+              phase ^= 1;
+            }
+            if (++fills > kFly) {
+              asm volatile("cp.async.wait_group %0;" ::"n"(kFly) : "memory");
+              hand_over();
+            }
+          }
+        }
+        asm volatile("cp.async.wait_all;" ::: "memory");   // also where a wait gave up
+        for (int left = min(fills, kFly); left > 0; --left) hand_over();
+      } else {
       // A box is R token rows of one 64-dim chunk; lane l of producer w has box
       // l * kProducers + w. (A box takes ~60 cycles to set off, whichever lane does
       // it: one warp for all 64 boxes of a tile with pages of 16 tokens kept the
@@ -821,6 +888,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
         // leave no copy in flight: every slot's last fill (a slot that was never
         // filled passes as the phase before its first)
         for (int i = 0; i < C::kSlots; ++i) mbar_wait(kv_full(i), i < s ? phase : phase ^ 1);
+      }
       }
     }
     if (warp == NQ * 4 + NQ + C::kProducers) {
@@ -1335,13 +1403,10 @@ static Params make_params(const pa_prompt_params* p) {
 }
 
 template <typename T>
-static cudaError_t launch_rows(const Params& a, int D, cudaStream_t stream) {
+static cudaError_t launch_rows(const Params& a, cudaStream_t stream) {
   const long long warps = static_cast<long long>(a.T) * a.Hq;
   const dim3 grid(static_cast<unsigned>((warps + 3) / 4));
-  if (D == 32) prompt_rows_kernel<T, 32><<<grid, 128, 0, stream>>>(a);
-  else if (D == 64) prompt_rows_kernel<T, 64><<<grid, 128, 0, stream>>>(a);
-  else if (D == 128) prompt_rows_kernel<T, 128><<<grid, 128, 0, stream>>>(a);
-  else prompt_rows_kernel<T, 256><<<grid, 128, 0, stream>>>(a);
+  prompt_rows_kernel<T, 32><<<grid, 128, 0, stream>>>(a);
   return cudaGetLastError();
 }
 
@@ -1385,6 +1450,7 @@ static bool encode_map(CUtensorMap* map, const pa_prompt_params* p, const void* 
 // in `splits` parts.
 struct Plan {
   bool rows_path;
+  bool gather;              // pages that are not a multiple of 8 tokens: no TMA boxes
   int nq, splits;
   long long tiles;          // bound on the row tiles of a KV head
   size_t ws_bytes;
@@ -1392,8 +1458,9 @@ struct Plan {
 static Plan make_plan(const pa_prompt_params* p, int sms) {
   Plan pl = {};
   pl.splits = 1;
-  pl.rows_path = p->head_dim == 32 || p->block_size % 8 != 0;
+  pl.rows_path = p->head_dim == 32;
   if (pl.rows_path) return pl;
+  pl.gather = p->block_size % 8 != 0;
   const int g = p->num_heads / p->num_kv_heads;
   const long long packed = static_cast<long long>(p->num_tokens) * g;   // rows of a KV head
   // Two row tiles per CTA keep the matrix pipe busy; a batch whose sequences
@@ -1422,8 +1489,8 @@ static Plan make_plan(const pa_prompt_params* p, int sms) {
   return pl;
 }
 
-template <typename T, int D, int NQ>
-static cudaError_t launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams& a,
+template <typename T, int D, int NQ, bool kGather>
+static cudaError_t launch_tiles_as(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams& a,
                                 const Plan& pl, cudaStream_t stream) {
   using C = TC<D, NQ>;
   static std::mutex mu;
@@ -1434,7 +1501,7 @@ static cudaError_t launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, co
   {
     std::lock_guard<std::mutex> lk(mu);
     if (!set[dev]) {
-      e = cudaFuncSetAttribute(prompt_tile_kernel<T, D, NQ>,
+      e = cudaFuncSetAttribute(prompt_tile_kernel<T, D, NQ, kGather>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
       if (e != cudaSuccess) return e;
       set[dev] = true;
@@ -1455,7 +1522,7 @@ static cudaError_t launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, co
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, prompt_tile_kernel<T, D, NQ>, mk, mv, a);
+  e = cudaLaunchKernelEx(&cfg, prompt_tile_kernel<T, D, NQ, kGather>, mk, mv, a);
   if (e == cudaSuccess && pl.splits > 1) {
     const long long warps = static_cast<long long>(a.p.T) * a.p.Hq;
     cfg.gridDim = dim3(static_cast<unsigned>((warps + 3) / 4));
@@ -1464,6 +1531,13 @@ static cudaError_t launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, co
     e = cudaLaunchKernelEx(&cfg, prompt_join_kernel<T, D>, a);
   }
   return e;
+}
+
+template <typename T, int D, int NQ>
+static cudaError_t launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams& a,
+                                const Plan& pl, cudaStream_t stream) {
+  return pl.gather ? launch_tiles_as<T, D, NQ, true>(mk, mv, a, pl, stream)
+                   : launch_tiles_as<T, D, NQ, false>(mk, mv, a, pl, stream);
 }
 
 template <typename T>
@@ -1512,11 +1586,9 @@ pa_status_t pa_prompt(const pa_prompt_params* p, cudaStream_t stream) {
   a.p = make_params(p);
   cudaError_t e;
   if (pl.rows_path) {
-    e = half ? launch_rows<__half>(a.p, p->head_dim, stream)
-             : launch_rows<__nv_bfloat16>(a.p, p->head_dim, stream);
+    e = half ? launch_rows<__half>(a.p, stream) : launch_rows<__nv_bfloat16>(a.p, stream);
     return e == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
   }
-  const int tn = p->head_dim == 256 ? 64 : 128;
   // box rows: a power of two in the page size, at most 32 (where a window starts,
   // up to R - 1 hidden keys are read)
   a.R = 8;
@@ -1532,8 +1604,10 @@ pa_status_t pa_prompt(const pa_prompt_params* p, cudaStream_t stream) {
   a.o_part = static_cast<float*>(p->workspace);
   a.lse_part = a.o_part + static_cast<size_t>(pl.splits) * p->num_tokens * p->num_heads * p->head_dim;
   CUtensorMap mk, mv;
-  if (!encode_map(&mk, p, p->k_cache, p->k_stride_block, p->k_stride_slot, p->k_stride_head, a.R) ||
-      !encode_map(&mv, p, p->v_cache, p->v_stride_block, p->v_stride_slot, p->v_stride_head, a.R))
+  memset(&mk, 0, sizeof(mk));
+  memset(&mv, 0, sizeof(mv));
+  if (!pl.gather && (!encode_map(&mk, p, p->k_cache, p->k_stride_block, p->k_stride_slot, p->k_stride_head, a.R) ||
+       !encode_map(&mv, p, p->v_cache, p->v_stride_block, p->v_stride_slot, p->v_stride_head, a.R)))
     return PA_ERR_ARG;
   e = half ? launch_tiles_d<__half>(mk, mv, a, pl, p->head_dim, stream)
            : launch_tiles_d<__nv_bfloat16>(mk, mv, a, pl, p->head_dim, stream);
