@@ -284,7 +284,7 @@ __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Resize a) {
     const long long all = carry + block_scan(need, s_scan, total);
     const bool ok = need == 0 || all <= avail;
     if (c.active && !ok) flag(p, PA_STATUS_NO_PAGES);
-    // the pages of this round: up to the largest end of a row that gets its pages
+    // the pages of these rows: up to the largest end of a row that gets its pages
     const unsigned top = __reduce_max_sync(kFull, need > 0 && ok ? static_cast<unsigned>(all) : 0u);
     if (lane == 0) s_scan[warp] = static_cast<int>(top);
     __syncthreads();
@@ -298,8 +298,6 @@ __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Resize a) {
       if (cow) {
         const int dst = list[at];
         row[c.S / p.bs] = dst;
-        if (atomicSub(p.refs + tail, 1) == 1)
-          atomicOr(p.words + (tail >> 5), 1u << (tail & 31));
         int* e = p.copies() + 3 * atomicAdd(&s_copies, 1);   // (in any order)
         e[0] = tail;
         e[1] = dst;
@@ -322,6 +320,13 @@ __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Resize a) {
     carry += total;
     given = end;
     __syncthreads();
+  }
+  // The copied pages lose these users. Only here, so that the free pages numbered
+  // above stay the ones they were, and every row found the counts that the releases
+  // left, whichever 1024 rows it was among.
+  for (int k = threadIdx.x; k < s_copies; k += blockDim.x) {
+    const int src = p.copies()[3 * k];
+    if (atomicSub(p.refs + src, 1) == 1) atomicOr(p.words + (src >> 5), 1u << (src & 31));
   }
   if (threadIdx.x == 0) p.scratch[kHCopies] = s_copies;
 }

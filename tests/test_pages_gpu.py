@@ -240,3 +240,30 @@ def test_empty_calls():
     assert int(pool.compact(table)) == 0
     assert int(pool.compact(table[:0])) == 0
     assert_same(model, pool, table, lens, k, v, "empty")
+
+
+@pytest.mark.parametrize("nb", [900, 1400, 4000])
+def test_tails_that_all_users_leave_are_free_only_after_the_call(nb):
+    """Shared last pages among the first 1024 rows lose their last user while later rows
+    still take pages: the numbering of the free pages must not move meanwhile."""
+    rows, bs = 2100, 4
+    pool, model, table, lens, k, v = _setup(rows, 3, nb, bs, 1, 8, 1, seed=nb)
+    r = random.Random(nb)
+    low = r.sample(range(0, nb // 4), 60)
+    start = torch.zeros(rows, dtype=torch.int32)
+    for i, page in enumerate(low):                  # two to four users each, also across 1024
+        for row in r.sample(range(i * 30, i * 30 + 30), r.randint(2, 3)) + [1024 + i]:
+            table[row, 0] = page
+            start[row] = 2
+    lens.copy_(start)
+    model.table, model.lens = table.tolist(), lens.tolist()
+    pool.adopt(table, lens)
+    model.adopt()
+    new = [r.choice([-1, 3, 4, 5, 9]) if s else r.choice([-1, 0, 1, 5]) for s in start.tolist()]
+    pool.resize(table, lens, _t(new))
+    model.resize(new)
+    assert_same(model, pool, table, lens, k, v, "grown")
+    new = [r.choice([-1, 0, 12]) for _ in range(rows)]
+    pool.resize(table, lens, _t(new))
+    model.resize(new)
+    assert_same(model, pool, table, lens, k, v, "again")
