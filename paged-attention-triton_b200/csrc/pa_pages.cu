@@ -88,27 +88,28 @@ __device__ __forceinline__ void grid_wait() {
 }
 
 // Inclusive sum over the block's threads in thread order; `total` gets the sum.
-// Ends with a barrier, so that back-to-back calls may share `sh` (32 ints).
-__device__ __forceinline__ int block_scan(int v, int* sh, int& total) {
+// Ends with a barrier, so that back-to-back calls may share `sh` (32 entries).
+template <class I>
+__device__ __forceinline__ I block_scan(I v, I* sh, I& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int u = __shfl_up_sync(kFull, v, o);
+    const I u = __shfl_up_sync(kFull, v, o);
     if (lane >= o) v += u;
   }
   if (lane == 31) sh[warp] = v;
   __syncthreads();
   if (warp == 0) {
-    int w = lane < nw ? sh[lane] : 0;
+    I w = lane < nw ? sh[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int u = __shfl_up_sync(kFull, w, o);
+      const I u = __shfl_up_sync(kFull, w, o);
       if (lane >= o) w += u;
     }
     sh[lane] = w;
   }
   __syncthreads();
-  const int before = warp ? sh[warp - 1] : 0;
+  const I before = warp ? sh[warp - 1] : 0;
   total = sh[nw - 1];
   __syncthreads();
   return before + v;
@@ -173,13 +174,13 @@ __device__ __forceinline__ RowChange row_change(const Resize& a, int r, bool& ba
   const long long cap = static_cast<long long>(a.t.width) * a.p.bs;
   bad = c.n >= 0 && (c.S < 0 || c.S > cap || c.n > cap);
   c.active = c.n >= 0 && !bad;
-  c.used = (c.S + a.p.bs - 1) / a.p.bs;
-  c.want = (c.n + a.p.bs - 1) / a.p.bs;
+  c.used = c.S > 0 ? (c.S - 1) / a.p.bs + 1 : 0;
+  c.want = c.n > 0 ? (c.n - 1) / a.p.bs + 1 : 0;
   c.keep_sinks = c.first = 0;
   if (c.active && a.window) {
     // The next query sits at min(S, n) or later and sees nothing before
     // token min(S, n) - window + 1 but the sinks.
-    c.keep_sinks = (a.sinks + a.p.bs - 1) / a.p.bs;
+    c.keep_sinks = a.sinks > 0 ? (a.sinks - 1) / a.p.bs + 1 : 0;
     const int low = min(c.S, c.n) - a.window + 1;
     c.first = low > 0 ? low / a.p.bs : 0;
   }
@@ -188,6 +189,7 @@ __device__ __forceinline__ RowChange row_change(const Resize& a, int r, bool& ba
 
 __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Resize a) {
   __shared__ int s_scan[32];
+  __shared__ long long s_needs[32];        // rows may ask for more than 2^31 pages together
   __shared__ int s_list[kListSmem];
   __shared__ int s_last, s_copies;
   const Pool& p = a.p;
@@ -263,7 +265,8 @@ __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Resize a) {
   int given = 0;              // pages given out so far
   for (int r0 = 0; r0 < a.t.rows; r0 += blockDim.x) {
     const int r = r0 + threadIdx.x;
-    int need = 0, cow = 0, tail = 0;
+    long long need = 0;
+    int cow = 0, tail = 0;
     bool bad;
     RowChange c;
     c.active = false;
@@ -280,8 +283,8 @@ __global__ void __launch_bounds__(kPlanThreads) resize_kernel(const Resize a) {
       }
     }
     need += cow;
-    int total;
-    const long long all = carry + block_scan(need, s_scan, total);
+    long long total;
+    const long long all = carry + block_scan(need, s_needs, total);
     const bool ok = need == 0 || all <= avail;
     if (c.active && !ok) flag(p, PA_STATUS_NO_PAGES);
     // the pages of these rows: up to the largest end of a row that gets its pages
@@ -352,7 +355,7 @@ __global__ void __launch_bounds__(kPlanThreads) adopt_kernel(const Adopt a) {
     const int S = __ldg(a.lens + r);
     const long long cap = static_cast<long long>(a.width) * p.bs;
     if ((S < 0 || S > cap) && threadIdx.x == 0) flag(p, PA_STATUS_BAD_SEQLEN);
-    const int used = S <= 0 ? 0 : S > cap ? a.width : (S + p.bs - 1) / p.bs;
+    const int used = S <= 0 ? 0 : S > cap ? a.width : (S - 1) / p.bs + 1;
     for (int j = threadIdx.x; j < used; j += blockDim.x) {
       const int e = __ldg(a.bt + r * a.sb + j);
       if (in_pool(p, e))

@@ -63,3 +63,29 @@ def test_pages_behind_element_2_to_32(far):
         for row in (0, 3):
             assert torch.equal(x[table[row, 650 // bs].long()].view(torch.int16), a.view(torch.int16))
             assert torch.equal(x[table[row, 700 // bs].long(), : 700 % bs], t)
+
+
+def test_rows_that_ask_for_more_than_2_to_31_pages():
+    """Sums and lengths at the end of int32: refused for lack of pages, each by itself."""
+    import paged_attention as pa
+    rows, width = 1100, 2 ** 21
+    k = torch.zeros(64, 1, 1, 8, dtype=torch.float16, device="cuda")
+    pool = pa.PagePool(k, torch.zeros_like(k))
+    table = torch.full((rows, width), -1, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+    new = torch.full_like(lens, width)
+    new[:2] = 20
+    pool.resize(table, lens, new)
+    assert lens.tolist() == [20, 20] + [0] * (rows - 2)
+    assert pool.read_status() == pa._native.PA_STATUS_NO_PAGES
+    assert table[:2, :20].flatten().tolist() == list(range(40))
+    assert int((table >= 0).sum()) == 40 and int(pool.refs.sum()) == 40
+    # one row's length just below 2^31 tokens, in pages of 1024
+    k = torch.zeros(64, 1024, 1, 8, dtype=torch.float16, device="cuda")
+    pool = pa.PagePool(k, torch.zeros_like(k))
+    table = torch.full((3, width), -1, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(3, dtype=torch.int32, device="cuda")
+    new = torch.tensor([5, 2 ** 31 - 1, 0], dtype=torch.int32, device="cuda")
+    pool.resize(table, lens, new)
+    assert lens.tolist() == [5, 0, 0]
+    assert pool.read_status() == pa._native.PA_STATUS_NO_PAGES

@@ -267,3 +267,13 @@ def test_tails_that_all_users_leave_are_free_only_after_the_call(nb):
     pool.resize(table, lens, _t(new))
     model.resize(new)
     assert_same(model, pool, table, lens, k, v, "again")
+
+
+@pytest.mark.parametrize("sinks", [2 ** 31 - 1, 2 ** 31 - 16, 2 ** 40])
+def test_first_tokens_without_end_are_kept(sinks):
+    pool, model, table, lens, k, v = _setup(2, 8, 20)
+    for new in ([128, 70], [128, 100]):
+        pool.resize(table, lens, _t(new), window=16, num_sinks=sinks)
+        model.resize(new, 16, sinks)
+        assert_same(model, pool, table, lens, k, v, f"{new}")
+    assert model.refs.count(1) == 15
