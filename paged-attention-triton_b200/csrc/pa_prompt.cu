@@ -35,6 +35,7 @@ using pa::make_fastdiv;
 constexpr unsigned kFull = 0xffffffffu;
 constexpr float kSentinel = -1e30f;     // LSE of a row that sees nothing
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kNaN = __builtin_nanf("");
 constexpr float kLn2 = 0.6931471805599453f;
 
 struct Params {
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(kFull, cm, o));
     const float mn = fmaxf(m, cm);
-    if (mn == -INFINITY) continue;
+    if (!__any_sync(kFull, sc != -INFINITY)) continue;   // (NaN is a score too)
     const float alpha = exp2f(m - mn);
     const float pv = sc == -INFINITY ? 0.f : exp2f(sc - mn);
     float ps = pv;
@@ -210,12 +211,12 @@ __global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
       for (int i = 0; i < N; ++i) acc[i] = fmaf(pj, to_float<T>(__ldg(vr + i)), acc[i]);
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* dst = reinterpret_cast<uint16_t*>(p.out + row * p.o_st + hq * p.o_sh) + lane * N;
 #pragma unroll
   for (int i = 0; i < N; ++i) dst[i] = static_cast<uint16_t>(pack2<T>(acc[i] * inv, 0.f));
   if (lane == 0 && p.lse)
-    p.lse[static_cast<long long>(row) * p.Hq + hq] = l > 0.f ? (m + log2f(l)) * kLn2 : kSentinel;
+    p.lse[static_cast<long long>(row) * p.Hq + hq] = l == 0.f ? kSentinel : (m + log2f(l)) * kLn2;
 }
 
 // ----------------------------------------------------------------------------
@@ -449,9 +450,9 @@ __device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
 }
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {   // NaN if any is
   float r;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
 }
 __device__ __forceinline__ float max_nan(float a, float b) {   // NaN if either is
@@ -1077,7 +1078,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
     const float scl = p.scale_log2;
     const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;   // TMEM lane 32 * (warp % 4)
     const uint32_t o_at = tmem + lanes + C::kOCol + t * D;
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;                 // of finite scores
     const int n = j.k1 - j.k0;
     // Two S buffers: waits for the product of tile i - 1, once per tile and before tile i's
     // P is handed over, so that no barrier here gets a phase ahead of its reader.
@@ -1124,8 +1125,11 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
 #pragma unroll
         for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], s[c + 2 * e], s[c + 2 * e + 1]);
       }
-      const float top = max3(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]),
-                             max3(fmaxf(s[kTN - 4], s[kTN - 3]), s[kTN - 2], s[kTN - 1]));
+      const float top = max3(max3(mx[0], mx[1], mx[2]), max3(mx[3], s[kTN - 4], s[kTN - 3]),
+                             max_nan(s[kTN - 2], s[kTN - 1]));
+      // a score of NaN or infinity leaves no number (the exponentials on the FMA pipe
+      // would): the sum carries it
+      if (!(top < INFINITY)) l = kNaN;
       if (i == 0) {
         m = top;
       } else if (__any_sync(kFull, (top - m) * scl > kRescaleLog2)) {
@@ -1197,8 +1201,8 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
     if (!ok) {
       if (lane == 0) flag(p, PA_STATUS_TIMEOUT);
     } else {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
-      const float lse = l > 0.f ? (m * scl + log2f(l)) * kLn2 : kSentinel;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const float lse = l == 0.f ? kSentinel : (m * scl + log2f(l)) * kLn2;
       const int hq = j.kvh * p.G + pr - tok * p.G;
       const long long at = static_cast<long long>(j.s.start + tok) * p.Hq + hq;
       if (a.splits == 1) {
@@ -1294,22 +1298,22 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(const TileParams a) {
   for (int i = 0; i < N; ++i) acc[i] = 0.f;
   for (int k0 = 0; k0 < a.splits; k0 += 32) {
     const float l = k0 + lane < a.splits ? __ldcg(a.lse_part + (k0 + lane) * rows + w) : kSentinel;
+    if (__all_sync(kFull, l <= -1e29f)) continue;      // these splits saw nothing (NaN is something)
     float t = l;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) t = fmaxf(t, __shfl_xor_sync(kFull, t, o));
-    if (t <= -1e29f) continue;                         // these splits saw nothing
     t = fmaxf(t, top);
     const float old = exp2f((top - t) * kLog2e);
     top = t;
     sum *= old;
 #pragma unroll
     for (int i = 0; i < N; ++i) acc[i] *= old;
-    const float mine = l > -1e29f ? exp2f((l - top) * kLog2e) : 0.f;
+    const float mine = l <= -1e29f ? 0.f : exp2f((l - top) * kLog2e);
     const int cnt = min(32, a.splits - k0);
 #pragma unroll 4
     for (int k = 0; k < cnt; ++k) {
       const float f = __shfl_sync(kFull, mine, k);
-      if (f > 0.f) {                                   // (an empty split has no row)
+      if (f != 0.f) {                                  // (an empty split has no row)
         const float* src = a.o_part + ((k0 + k) * rows + w) * D + lane * N;
         sum += f;
 #pragma unroll
@@ -1317,11 +1321,11 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(const TileParams a) {
       }
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + row * p.o_st + hq * p.o_sh + lane * N * 2);
 #pragma unroll
   for (int i = 0; i < N / 2; ++i) dst[i] = pack2<T>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
-  if (lane == 0 && p.lse) p.lse[w] = sum > 0.f ? top + logf(sum) : kSentinel;
+  if (lane == 0 && p.lse) p.lse[w] = sum == 0.f ? kSentinel : top + logf(sum);
 }
 
 // ----------------------------------------------------------------------------

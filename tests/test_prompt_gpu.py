@@ -366,3 +366,43 @@ def test_prompt_through_ctypes():
     want, _, tol = reference(q, c.k, c.v, c.table, lens, bs, window, sinks, _starts(qs))
     vmax = c.v[~c.v.isnan()].abs().max().double().item()
     assert_matches(out, want, _tolerance(q, tol, vmax), "ctypes")
+
+
+@pytest.mark.parametrize("splits", [1, 3, 40])
+@pytest.mark.parametrize("d,bs,n,s", [(32, 16, 3, 700), (32, 16, 1, 1), (64, 16, 5, 700), (128, 16, 5, 700),
+                                      (128, 16, 300, 700), (256, 32, 5, 700), (128, 5, 5, 700),
+                                      (64, 16, 1, 1)])
+def test_numbers_that_are_none_in_visible_places_show(d, bs, n, s, splits):
+    """NaN or infinity in a visible key makes the rows that see it NaN, LSE included, in a
+    visible value its dimension; the other KV head's rows keep their bits. The key's place
+    runs through eight neighbours: a quarter of the exponentials is computed another way."""
+    import paged_attention as pa
+    g = torch.Generator().manual_seed(d + n)
+    window, sinks = 350, 3
+    pages = -(-s // bs)
+    k, v = (torch.randn(pages, bs, 2, d, generator=g).half().cuda() for _ in range(2))
+    q = torch.rand(n, 4, d, generator=g).half().cuda() + 0.01
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    starts = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([s], dtype=torch.int32, device="cuda")
+
+    def run():
+        return pa.paged_prompt_attention(q, k, v, table, starts, lens, bs, window=window, num_sinks=sinks,
+                                         return_lse=True, num_splits=splits)
+    clean, clean_lse = run()
+    assert clean.isfinite().all()
+    for t in [1] + [s - n - 20 + i for i in range(8)] if s > 1 else [0]:   # every row sees these
+        for value in (float("nan"), float("inf")):
+            kept = k[t // bs, t % bs, 0].clone()
+            k[t // bs, t % bs, 0, 5] = value
+            o, lse = run()
+            k[t // bs, t % bs, 0] = kept
+            assert o[:, :2].isnan().all() and lse[:, :2].isnan().all(), f"key {t} {value}"
+            assert torch.equal(o[:, 2:], clean[:, 2:]) and torch.equal(lse[:, 2:], clean_lse[:, 2:])
+        kept = v[t // bs, t % bs, 0].clone()
+        v[t // bs, t % bs, 0, 7] = float("nan")
+        o, lse = run()
+        v[t // bs, t % bs, 0] = kept
+        assert o[:, :2, 7].isnan().all(), f"value {t}"
+        o[:, :2, 7] = clean[:, :2, 7]
+        assert torch.equal(o, clean) and torch.equal(lse, clean_lse)
