@@ -2125,7 +2125,8 @@ __global__ void __launch_bounds__(128) generic_split_kernel(const GenParams g) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(kFull, cm, o));
     const float mn = fmaxf(m, cm);
-    if (mn == -INFINITY) continue;           // every page of the step was out of range
+    // every page of the step was out of range (kWin: or scores -inf; a lone NaN counts)
+    if (kWin ? !__any_sync(kFull, sc != -INFINITY) : mn == -INFINITY) continue;
     const float alpha = exp2f(m - mn);
     const float pv = (sc == -INFINITY) ? 0.f : exp2f(sc - mn);
     float ps = pv;
@@ -2151,7 +2152,13 @@ __global__ void __launch_bounds__(128) generic_split_kernel(const GenParams g) {
   const float lv = fmaxf(l, 1e-20f);
 #pragma unroll
   for (int i = 0; i < N; ++i) op[lane * N + i] = acc[i] / lv;
-  if (lane == 0) g.lse_part[w] = (m == -INFINITY) ? kSentinel : (m + log2f(lv)) * kLn2;
+  if (lane == 0) {
+    // (kWin: a split with a NaN is not to be left out by the reduction)
+    if (kWin && l != l)
+      g.lse_part[w] = l;
+    else
+      g.lse_part[w] = (m == -INFINITY) ? kSentinel : (m + log2f(lv)) * kLn2;
+  }
 }
 
 template <typename T, int D>

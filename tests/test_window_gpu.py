@@ -189,3 +189,31 @@ def test_window_decode_through_ctypes_with_its_own_workspace():
         assert_matches(out, want, tol, "ctypes")
         out.zero_()
         assert int(cnt.abs().sum()) == 0
+
+
+@pytest.mark.parametrize("d,bs", [(32, 16), (64, 5), (128, 5), (128, 16), (256, 32)])
+@pytest.mark.parametrize("s", [1, 40, 700])
+def test_nan_in_visible_places_shows(d, bs, s):
+    """A visible key's NaN makes its KV head's rows NaN, a value's its dimension, also where
+    a split holds no other token; the other head's rows keep their bits."""
+    import paged_attention as pa
+    g = torch.Generator().manual_seed(s + d)
+    pages = -(-s // bs)
+    k, v = (torch.randn(pages, bs, 2, d, generator=g).half().cuda() for _ in range(2))
+    q = torch.randn(3, 4, d, generator=g).half().cuda()
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(3, 1)
+    lens = torch.full((3,), s, dtype=torch.int32, device="cuda")
+
+    def run():
+        return pa.paged_attention(q, k, v, table, lens, bs, window=350, num_sinks=2)
+    clean = run()
+    assert clean.isfinite().all()
+    for t in sorted({0, s // 2, s - 1} if s < 700 else {0, 350, 500, 699}):
+        for x, dims in ((k, slice(None)), (v, slice(5, 6))):
+            kept = x[t // bs, t % bs, 0, 5].clone()
+            x[t // bs, t % bs, 0, 5] = float("nan")
+            o = run()
+            x[t // bs, t % bs, 0, 5] = kept
+            assert o[:, :2, dims].isnan().all(), f"token {t}"
+            o[:, :2, dims] = clean[:, :2, dims]
+            assert torch.equal(o, clean)
