@@ -23,6 +23,16 @@ from .torch_kernel import window_args
 Caches = Union[torch.Tensor, Sequence[torch.Tensor]]
 
 
+def int32_vector(who: str, x: torch.Tensor) -> torch.Tensor:
+    """``x`` as the contiguous int32 that the calls take. int64 values beyond int32
+    become its ends, which no table holds, instead of small numbers."""
+    if x.dtype == torch.int64:
+        x = x.clamp(-1, 2 ** 31 - 1).to(torch.int32)
+    elif x.dtype != torch.int32:
+        raise ValueError(f"{who}: lengths and rows must be int32 or int64 tensors")
+    return x.contiguous()
+
+
 class PagePool:
     """The pages that the caches of one or more layers share: page ``i`` is
     ``cache[i]`` of every ``[num_blocks, block_size, Hkv, D]`` cache given.
@@ -77,7 +87,7 @@ class PagePool:
         replaced by a copy of its used slots."""
         win, sinks = window_args("PagePool.resize", window, num_sinks)
         if new_lens.dtype != torch.int32 or not new_lens.is_contiguous():
-            new_lens = new_lens.to(torch.int32).contiguous()
+            new_lens = int32_vector("PagePool.resize", new_lens)
         self._pool.resize(block_table, seq_lens, new_lens, win, sinks)
 
     def fork(self, block_table: torch.Tensor, seq_lens: torch.Tensor, parents: torch.Tensor,
@@ -88,7 +98,7 @@ class PagePool:
         row outside the table, a child that is not empty, or named before;
         ``PA_STATUS_NO_PAGES``: no page for the copy, the child stays empty."""
         parents, children = (x if x.dtype == torch.int32 and x.is_contiguous()
-                             else x.to(torch.int32).contiguous() for x in (parents, children))
+                             else int32_vector("PagePool.fork", x) for x in (parents, children))
         self._pool.fork(block_table, seq_lens, parents, children)
 
     def compact(self, block_table: torch.Tensor) -> torch.Tensor:

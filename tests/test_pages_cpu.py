@@ -117,3 +117,14 @@ def test_model_frees_what_the_window_hides():
     assert m.table[0][:6] == [0, -1, -1, 3, 4, 1] and m.refs == [1, 1, 0, 1, 1, 0, 0, 0]
     m.resize([-1, 17])
     assert m.status == NO_PAGES and m.lens == [21, 0]
+
+
+def test_int64_lengths_and_rows_are_not_wrapped():
+    from paged_attention.page_pool import int32_vector
+    x = int32_vector("who", torch.tensor([0, 5, -1, -2 ** 40, 2 ** 31 - 1, 2 ** 32 + 7]))
+    assert x.dtype == torch.int32 and x.tolist() == [0, 5, -1, -1, 2 ** 31 - 1, 2 ** 31 - 1]
+    y = torch.arange(6, dtype=torch.int32)
+    assert int32_vector("who", y) is y and int32_vector("who", y[::2]).is_contiguous()
+    for bad in (torch.zeros(2), torch.zeros(2, dtype=torch.int16)):
+        with pytest.raises(ValueError, match="who: lengths and rows"):
+            int32_vector("who", bad)
