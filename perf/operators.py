@@ -312,7 +312,7 @@ def _pages_own(st):
         out["lens"] = st["lens"]
     else:
         pool.resize(st["table"], st["lens"], st["new"], window=c["window"] or None,
-                    num_sinks=c["sinks"])
+                    num_sinks=c["sinks"] if c["window"] else 0)
         out["lens"] = st["lens"]
     if c["op"] != "resize" or c["share"]:
         out["kv"] = st["kv"]
