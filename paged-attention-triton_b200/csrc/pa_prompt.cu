@@ -19,6 +19,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <numeric>
 #include <climits>
 #include <mutex>
 #include <type_traits>
@@ -308,11 +309,16 @@ __device__ __forceinline__ void regs_down() {
   asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
+// How the keys' rows come: boxes of a page's rows (page size a multiple of 8), four
+// rows by their numbers in the cache seen as one list of rows (other page sizes), or
+// 16 bytes at a time by cp.async (strides that make no such list).
+enum class Fetch { kBoxes, kRows, kPieces };
 struct TileParams {
   Params p;
   int R, lR;                // token rows per TMA box, and its log2
   int bs_log2;              // log2 of the page size, or -1
   FastDiv div_g, div_bs;
+  int row_b[2], row_s[2], row_h[2];   // kRows: rows from a page, slot, head to the next, of K and V
   int splits;
   float* o_part;            // [splits][T * Hq][D], splits > 1
   float* lse_part;          // [splits][T * Hq]
@@ -364,6 +370,15 @@ __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map
       "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(bar)
+      : "memory");
+}
+// Four rows of 64 dimensions, from column c on.
+__device__ __forceinline__ void tma_load_rows(uint32_t dst, const CUtensorMap* map, int c, int r0,
+                                              int r1, int r2, int r3, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar)
       : "memory");
 }
 // One lane of a converged warp. (A lane elected this way is known to be alone,
@@ -698,7 +713,7 @@ __device__ __forceinline__ bool find_job(const TileParams& a, Job& j, int* sh) {
   return true;
 }
 
-template <typename T, int D, int NQ, bool kGather>
+template <typename T, int D, int NQ, Fetch kFetch>
 __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
     prompt_tile_kernel(const __grid_constant__ CUtensorMap mk, const __grid_constant__ CUtensorMap mv,
                        const TileParams a) {
@@ -729,7 +744,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
   auto s_full = [&](int i) { return bar1 + (7 * NQ + i) * 8; };
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kSlots; ++s) {
-      mbar_init(kv_full(s), kGather ? C::kProducers * 32 : C::kProducers);
+      mbar_init(kv_full(s), kFetch == Fetch::kPieces ? C::kProducers * 32 : C::kProducers);
       mbar_init(kv_empty(s), NQ);
     }
     for (int i = 0; i < C::kVBars; ++i) mbar_init(v_ready(i), 32);
@@ -771,13 +786,13 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
     if constexpr (C::kSplitRegs) regs_down<kOtherRegs>();
     if (warp >= NQ * 4 + NQ && warp < NQ * 4 + NQ + C::kProducers) {
       // ---------------------------------------------------------------- producer
-      if constexpr (kGather) {
-        // Pages whose size is not a multiple of 8 tokens: rows by cp.async, 16 bytes a
-        // thread and copy, to where a box would put them. Up to kFly tiles' copies
-        // stay in flight per thread; a tile is handed over when its own have landed
-        // (and the fence has made them visible to the matrix pipe). 8192 tokens,
-        // window 4096, Hq32/Hkv8: pages of 1 and 4 tokens 1049 and 803 us, of 16 by TMA
-        // 357; bound by the copies' address arithmetic beside the softmax warps.
+      if constexpr (kFetch == Fetch::kPieces) {
+        // Strides that are no whole numbers of rows: 16 bytes a thread and copy, to where a
+        // box would put them. Up to kFly tiles' copies stay in flight per thread; a tile
+        // is handed over when its own have landed (and the fence has made them visible to
+        // the matrix pipe). 8192 tokens, window 4096, Hq32/Hkv8, pages of 1 and 4 tokens:
+        // 1049 and 803 us, bound by the copies' address arithmetic beside the softmax
+        // warps (as lists of rows both take 463, pages of 16 as boxes 363).
         constexpr int kPer = D / 8, kThr = C::kProducers * 32, kRows = kTN * kPer / kThr;
         constexpr int kFly = 2;
         static_assert(kThr % kPer == 0, "rows per pass");
@@ -836,6 +851,76 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
         }
         asm volatile("cp.async.wait_all;" ::: "memory");   // also where a wait gave up
         for (int left = min(fills, kFly); left > 0; --left) hand_over();
+      } else if constexpr (kFetch == Fetch::kRows) {
+        // A copy is four keys' rows of one 64-dim chunk; the lanes share them out as
+        // they do boxes. The four keys' tokens follow each other, their pages do not. A
+        // key of them that no row sees brings a visible one's row. 128 copies a tile at
+        // 25 to 40 cycles each bound it where boxes of 16 rows wait for S and P (8192
+        // tokens, Hq32/Hkv8: window 4096 463 us against 363; head_dim 64, no window 611
+        // against 401).
+        const int f = lane * C::kProducers + warp - (NQ * 4 + NQ);
+        const int group = f / C::kChunks, chunk = f - group * C::kChunks;
+        auto visible = [&](int key) {
+          return group < kTN / 4 && key < j.end && !(key >= j.gap0 && key < j.gap1);
+        };
+        auto lookup = [&](int k, int (&page)[4]) {
+          const int key = k * kTN + group * 4;
+          const int tok = key < j.sink_keys ? key : key + j.delta;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            page[i] = INT_MIN;
+            if (visible(key + i))
+              page[i] = __ldg(p.bt + j.b * p.bt_sb + static_cast<int>(fast_div(tok + i, a.div_bs)));
+          }
+        };
+        int page[4], next[4], s = 0;
+        uint32_t phase = 0;
+        if (j.k0 < j.k1) lookup(j.k0, next);
+        for (int k = j.k0; k < j.k1 && ok; ++k) {
+          const int key = k * kTN + group * 4;
+          const int tok = key < j.sink_keys ? key : key + j.delta;
+          int slot[4], have = -1;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            page[i] = next[i];
+            slot[i] = tok + i - static_cast<int>(fast_div(tok + i, a.div_bs)) * p.bs;
+            if (page[i] != INT_MIN && (page[i] < 0 || page[i] >= p.NB)) {
+              flag(p, PA_STATUS_BAD_BLOCK);
+              page[i] = INT_MIN;
+            }
+            if (page[i] != INT_MIN) have = i;
+          }
+          if (k + 1 < j.k1) lookup(k + 1, next);
+          const bool valid = have >= 0;
+          const uint32_t bytes = __popc(__ballot_sync(kFull, valid)) * 4 * 128;
+          for (int kv = 0; kv < 2; ++kv) {
+            ok = __all_sync(kFull, mbar_wait(kv_empty(s), phase ^ 1));
+            if (!ok) break;
+            if (lane == 0) mbar_expect_tx(kv_full(s), bytes);
+            __syncwarp();
+            if (valid) {
+              int row[4], some = 0;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                row[i] = page[i] * a.row_b[kv] + slot[i] * a.row_s[kv] + j.kvh * a.row_h[kv];
+                if (i == have) some = row[i];
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (page[i] == INT_MIN) row[i] = some;
+              tma_load_rows(skv + s * C::kKV + chunk * kTN * 128 + group * 512, kv ? &mv : &mk,
+                            chunk * 64, row[0], row[1], row[2], row[3], kv_full(s));
+            }
+            if (++s == C::kSlots) {
+              s = 0;
+              phase ^= 1;
+            }
+          }
+        }
+        if (!ok) {
+          // leave no copy in flight (as below)
+          for (int i = 0; i < C::kSlots; ++i) mbar_wait(kv_full(i), i < s ? phase : phase ^ 1);
+        }
       } else {
       // A box is R token rows of one 64-dim chunk; lane l of producer w has box
       // l * kProducers + w. (A box takes ~60 cycles to set off, whichever lane does
@@ -1450,11 +1535,48 @@ static bool encode_map(CUtensorMap* map, const pa_prompt_params* p, const void* 
             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// A paged cache as rows of D dimensions, `unit` elements from one to the next, for
+// caches whose strides are whole numbers of rows; a copy takes four rows of 64.
+struct RowList {
+  int64_t unit, rows;
+  int b, s, h;              // rows from a page, slot, head to the next
+};
+static bool row_list(const pa_prompt_params* p, int64_t s_block, int64_t s_slot, int64_t s_head,
+                     RowList* r) {
+  const int64_t sb = p->num_blocks > 1 ? s_block : 0, ss = p->block_size > 1 ? s_slot : 0,
+                sh = p->num_kv_heads > 1 ? s_head : 0;
+  if (sb < 0 || ss < 0 || sh < 0) return false;
+  int64_t u = std::gcd(std::gcd(sb, ss), sh);
+  if (u == 0) u = p->head_dim;
+  if (u < p->head_dim || u >= (1ll << 38)) return false;
+  r->unit = u;
+  r->rows = (p->num_blocks - 1) * (sb / u) + (p->block_size - 1) * (ss / u) +
+            (p->num_kv_heads - 1) * (sh / u) + 1;
+  if (r->rows > 0x7fffffffll) return false;
+  r->b = static_cast<int>(sb / u);
+  r->s = static_cast<int>(ss / u);
+  r->h = static_cast<int>(sh / u);
+  return true;
+}
+static bool encode_rows(CUtensorMap* map, const pa_prompt_params* p, const void* base,
+                        const RowList& r) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const CUtensorMapDataType dt =
+      p->dtype == PA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p->head_dim), static_cast<cuuint64_t>(r.rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(r.unit) * 2};
+  const cuuint32_t box[2] = {64, 1};
+  const cuuint32_t step[2] = {1, 1};
+  return fn(map, dt, 2, const_cast<void*>(base), dims, strides, box, step,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+            CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // How a call runs: the CUDA-core path, or row tiles of 128 * nq with the keys
 // in `splits` parts.
 struct Plan {
   bool rows_path;
-  bool gather;              // pages that are not a multiple of 8 tokens: no TMA boxes
   int nq, splits;
   long long tiles;          // bound on the row tiles of a KV head
   size_t ws_bytes;
@@ -1464,7 +1586,6 @@ static Plan make_plan(const pa_prompt_params* p, int sms) {
   pl.splits = 1;
   pl.rows_path = p->head_dim == 32;
   if (pl.rows_path) return pl;
-  pl.gather = p->block_size % 8 != 0;
   const int g = p->num_heads / p->num_kv_heads;
   const long long packed = static_cast<long long>(p->num_tokens) * g;   // rows of a KV head
   // Two row tiles per CTA keep the matrix pipe busy; a batch whose sequences
@@ -1493,7 +1614,7 @@ static Plan make_plan(const pa_prompt_params* p, int sms) {
   return pl;
 }
 
-template <typename T, int D, int NQ, bool kGather>
+template <typename T, int D, int NQ, Fetch kFetch>
 static cudaError_t launch_tiles_as(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams& a,
                                 const Plan& pl, cudaStream_t stream) {
   using C = TC<D, NQ>;
@@ -1505,7 +1626,7 @@ static cudaError_t launch_tiles_as(const CUtensorMap& mk, const CUtensorMap& mv,
   {
     std::lock_guard<std::mutex> lk(mu);
     if (!set[dev]) {
-      e = cudaFuncSetAttribute(prompt_tile_kernel<T, D, NQ, kGather>,
+      e = cudaFuncSetAttribute(prompt_tile_kernel<T, D, NQ, kFetch>,
                                cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
       if (e != cudaSuccess) return e;
       set[dev] = true;
@@ -1526,7 +1647,7 @@ static cudaError_t launch_tiles_as(const CUtensorMap& mk, const CUtensorMap& mv,
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, prompt_tile_kernel<T, D, NQ, kGather>, mk, mv, a);
+  e = cudaLaunchKernelEx(&cfg, prompt_tile_kernel<T, D, NQ, kFetch>, mk, mv, a);
   if (e == cudaSuccess && pl.splits > 1) {
     const long long warps = static_cast<long long>(a.p.T) * a.p.Hq;
     cfg.gridDim = dim3(static_cast<unsigned>((warps + 3) / 4));
@@ -1539,19 +1660,20 @@ static cudaError_t launch_tiles_as(const CUtensorMap& mk, const CUtensorMap& mv,
 
 template <typename T, int D, int NQ>
 static cudaError_t launch_tiles(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams& a,
-                                const Plan& pl, cudaStream_t stream) {
-  return pl.gather ? launch_tiles_as<T, D, NQ, true>(mk, mv, a, pl, stream)
-                   : launch_tiles_as<T, D, NQ, false>(mk, mv, a, pl, stream);
+                                const Plan& pl, Fetch fetch, cudaStream_t stream) {
+  if (fetch == Fetch::kRows) return launch_tiles_as<T, D, NQ, Fetch::kRows>(mk, mv, a, pl, stream);
+  if (fetch == Fetch::kPieces) return launch_tiles_as<T, D, NQ, Fetch::kPieces>(mk, mv, a, pl, stream);
+  return launch_tiles_as<T, D, NQ, Fetch::kBoxes>(mk, mv, a, pl, stream);
 }
 
 template <typename T>
 static cudaError_t launch_tiles_d(const CUtensorMap& mk, const CUtensorMap& mv, const TileParams& a,
-                                  const Plan& pl, int D, cudaStream_t stream) {
-  if (D == 256) return launch_tiles<T, 256, 1>(mk, mv, a, pl, stream);
+                                  const Plan& pl, Fetch fetch, int D, cudaStream_t stream) {
+  if (D == 256) return launch_tiles<T, 256, 1>(mk, mv, a, pl, fetch, stream);
   if (D == 128)
-    return pl.nq == 2 ? launch_tiles<T, 128, 2>(mk, mv, a, pl, stream)
-                      : launch_tiles<T, 128, 1>(mk, mv, a, pl, stream);
-  return launch_tiles<T, 64, 1>(mk, mv, a, pl, stream);
+    return pl.nq == 2 ? launch_tiles<T, 128, 2>(mk, mv, a, pl, fetch, stream)
+                      : launch_tiles<T, 128, 1>(mk, mv, a, pl, fetch, stream);
+  return launch_tiles<T, 64, 1>(mk, mv, a, pl, fetch, stream);
 }
 
 }  // namespace pp
@@ -1610,11 +1732,24 @@ pa_status_t pa_prompt(const pa_prompt_params* p, cudaStream_t stream) {
   CUtensorMap mk, mv;
   memset(&mk, 0, sizeof(mk));
   memset(&mv, 0, sizeof(mv));
-  if (!pl.gather && (!encode_map(&mk, p, p->k_cache, p->k_stride_block, p->k_stride_slot, p->k_stride_head, a.R) ||
-       !encode_map(&mv, p, p->v_cache, p->v_stride_block, p->v_stride_slot, p->v_stride_head, a.R)))
-    return PA_ERR_ARG;
-  e = half ? launch_tiles_d<__half>(mk, mv, a, pl, p->head_dim, stream)
-           : launch_tiles_d<__nv_bfloat16>(mk, mv, a, pl, p->head_dim, stream);
+  Fetch fetch = Fetch::kBoxes;
+  RowList rk, rv;
+  if (p->block_size % 8 == 0) {
+    if (!encode_map(&mk, p, p->k_cache, p->k_stride_block, p->k_stride_slot, p->k_stride_head, a.R) ||
+        !encode_map(&mv, p, p->v_cache, p->v_stride_block, p->v_stride_slot, p->v_stride_head, a.R))
+      return PA_ERR_ARG;
+  } else if (row_list(p, p->k_stride_block, p->k_stride_slot, p->k_stride_head, &rk) &&
+             row_list(p, p->v_stride_block, p->v_stride_slot, p->v_stride_head, &rv)) {
+    fetch = Fetch::kRows;
+    if (!encode_rows(&mk, p, p->k_cache, rk) || !encode_rows(&mv, p, p->v_cache, rv))
+      return PA_ERR_ARG;
+    a.row_b[0] = rk.b, a.row_s[0] = rk.s, a.row_h[0] = rk.h;
+    a.row_b[1] = rv.b, a.row_s[1] = rv.s, a.row_h[1] = rv.h;
+  } else {
+    fetch = Fetch::kPieces;
+  }
+  e = half ? launch_tiles_d<__half>(mk, mv, a, pl, fetch, p->head_dim, stream)
+           : launch_tiles_d<__nv_bfloat16>(mk, mv, a, pl, fetch, p->head_dim, stream);
   return e == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 }
 

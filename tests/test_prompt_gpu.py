@@ -406,3 +406,53 @@ def test_numbers_that_are_none_in_visible_places_show(d, bs, n, s, splits):
         assert o[:, :2, 7].isnan().all(), f"value {t}"
         o[:, :2, 7] = clean[:, :2, 7]
         assert torch.equal(o, clean) and torch.equal(lse, clean_lse)
+
+
+def _relayout(x, kind):
+    """The same cache [NB, bs, Hkv, D] under other strides; what lies between is NaN."""
+    nb, bs, hkv, d = x.shape
+    nan = dict(fill_value=float("nan"), dtype=x.dtype, device=x.device)
+    if kind == "heads first":
+        y = torch.full((nb, hkv, bs, d), **nan).transpose(1, 2)
+    elif kind == "half of pairs":
+        y = torch.full((nb, 2, bs, hkv, d), **nan)[:, 1]
+    elif kind == "head outermost":
+        y = torch.full((hkv, nb, bs, d), **nan).permute(1, 2, 0, 3)
+    elif kind == "padded rows":              # strides that are no whole numbers of rows
+        y = torch.full((nb, bs, hkv, d + 8), **nan)[..., :d]
+    elif kind == "padded pages":
+        y = torch.full((nb, bs * hkv * d + 24), **nan)[:, : bs * hkv * d].unflatten(1, (bs, hkv, d))
+    else:
+        y = torch.full((nb, bs, hkv, d), **nan)
+    y.copy_(x)
+    return y
+
+
+@pytest.mark.parametrize("bs", [1, 4, 12, 16])
+@pytest.mark.parametrize("kinds", [("plain", "heads first"), ("half of pairs", "head outermost"),
+                                   ("padded rows", "padded rows"), ("plain", "padded pages")])
+@pytest.mark.parametrize("hkv,d", [(2, 128), (1, 64), (3, 256)])
+def test_prompt_cache_layouts(bs, kinds, hkv, d):
+    """Every way the keys' rows are fetched gives the bits of the plain layout."""
+    import paged_attention as pa
+    qs, lens, window, sinks = [170, 1, 33], [400, 77, 33], 90, 5
+    c = PoisonedCache(lens, qs, hkv, d, bs, torch.float16, window, sinks, bs + d)
+    q = torch.randn(204, hkv * 3, d, device="cuda").half()
+    st = torch.tensor(_starts(qs), dtype=torch.int32, device="cuda")
+    outs = [pa.paged_prompt_attention(q, k, v, c.table, st, c.lens, bs, window=window, num_sinks=sinks)
+            for k, v in ((c.k, c.v), (_relayout(c.k, kinds[0]), _relayout(c.v, kinds[1])))]
+    want, _, tol = reference(q, c.k, c.v, c.table, lens, bs, window, sinks, _starts(qs))
+    vmax = c.v[~c.v.isnan()].abs().max().double().item()
+    assert_matches(outs[0], want, _tolerance(q, tol, vmax), "plain")
+    assert torch.equal(outs[0], outs[1])
+
+
+def test_prompt_pool_of_one_token():
+    import paged_attention as pa
+    for d in (64, 128, 256):
+        k, v = (torch.randn(1, 1, 1, d, device="cuda").half() for _ in range(2))
+        st = torch.tensor([0, 1], dtype=torch.int32, device="cuda")
+        o = pa.paged_prompt_attention(torch.randn(1, 2, d, device="cuda").half(), k, v,
+                                      torch.zeros(1, 1, dtype=torch.int32, device="cuda"), st,
+                                      st[1:], 1)
+        assert torch.equal(o, v[0, 0].expand(1, 2, d))
