@@ -19,9 +19,9 @@
 #include <string.h>
 
 #include <algorithm>
-#include <numeric>
 #include <climits>
 #include <mutex>
+#include <numeric>
 #include <type_traits>
 
 #include "pa_decode.h"
@@ -44,7 +44,7 @@ struct Params {
   long long q_st, q_sh;                           // bytes
   const char* kc;
   const char* vc;
-  long long k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;   // bytes (CUDA-core path)
+  long long k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;   // bytes (Fetch::kPieces)
   const int* bt;
   long long bt_sb;                                // elements
   int max_blocks;
@@ -77,16 +77,6 @@ __device__ __forceinline__ Seq load_seq(const Params& p, int b, bool& bad) {
   return s;
 }
 
-template <typename T>
-__device__ __forceinline__ float to_float(uint16_t x);
-template <>
-__device__ __forceinline__ float to_float<__half>(uint16_t x) {
-  return __half2float(__ushort_as_half(x));
-}
-template <>
-__device__ __forceinline__ float to_float<__nv_bfloat16>(uint16_t x) {
-  return __bfloat162float(__ushort_as_bfloat16(x));
-}
 // (a, b) rounded to the 16-bit type, a in the low half.
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -117,107 +107,6 @@ __device__ __forceinline__ int seq_of_row(const Params& p, int row) {
     if (__ldg(p.starts + mid) <= row) lo = mid; else hi = mid - 1;
   }
   return row >= __ldg(p.starts + lo) && row < __ldg(p.starts + lo + 1) ? lo : -1;
-}
-
-// ----------------------------------------------------------------------------
-// CUDA-core path: head_dim 32
-// ----------------------------------------------------------------------------
-// One warp per (query row, query head): lane j scores the j-th token of 32
-// against the query (in shared memory), then the lanes, each owning D/32
-// dimensions, accumulate p_j v_j. It serves head_dim 32, whose 64-byte rows the
-// tile kernel's layout does not cover (and was the first form of every shape: 87 ms
-// for 8192 tokens, window 4096, Hq32/Hkv8).
-template <typename T, int D>
-__global__ void __launch_bounds__(128) prompt_rows_kernel(const Params p) {
-  constexpr int N = D / 32;
-  __shared__ float qs[4][D];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long w = static_cast<long long>(blockIdx.x) * 4 + warp;
-  if (w >= static_cast<long long>(p.T) * p.Hq) return;
-  const int row = static_cast<int>(w / p.Hq);
-  const int hq = static_cast<int>(w - static_cast<long long>(row) * p.Hq);
-  bool bad;
-  if (w == 0) {                    // every sequence is checked once
-    for (int b = lane; b < p.B; b += 32) {
-      load_seq(p, b, bad);
-      if (bad) flag(p, PA_STATUS_BAD_SEQLEN);
-    }
-    __syncwarp();
-  }
-  const int b = seq_of_row(p, row);
-  if (b < 0) return;               // a row of no sequence
-  const Seq s = load_seq(p, b, bad);
-  const int kvh = hq / p.G;
-  const int pos = s.S - s.n + row - s.start;
-  const int first = pos >= p.window ? pos - p.window + 1 : 0;   // of the window
-  const int a = min(p.sinks, first);                            // visible sinks
-  const int count = pos < 0 ? 0 : a + pos + 1 - first;
-  const uint16_t* qp = reinterpret_cast<const uint16_t*>(p.q + row * p.q_st + hq * p.q_sh);
-  for (int d = lane; d < D; d += 32) qs[warp][d] = to_float<T>(qp[d]);
-  __syncwarp();
-  float m = -INFINITY, l = 0.f, acc[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) acc[i] = 0.f;
-  for (int c = 0; c < count; c += 32) {
-    int t = c + lane;
-    int page = -1, slot = 0;
-    if (t < count) {
-      t = t < a ? t : t - a + first;
-      const int j = t / p.bs;
-      page = __ldg(p.bt + b * p.bt_sb + j);
-      slot = t - j * p.bs;
-      if (page < 0 || page >= p.NB) {
-        flag(p, PA_STATUS_BAD_BLOCK);
-        page = -1;
-      }
-    }
-    float sc = -INFINITY;
-    if (page >= 0) {
-      const uint4* kr = reinterpret_cast<const uint4*>(p.kc + page * p.k_sb + slot * p.k_ss + kvh * p.k_sh);
-      float dot = 0.f;
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i) {
-        const uint4 x = __ldg(kr + i);
-        const uint32_t x4[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          dot = fmaf(to_float<T>(x4[e] & 0xffff), qs[warp][i * 8 + 2 * e], dot);
-          dot = fmaf(to_float<T>(x4[e] >> 16), qs[warp][i * 8 + 2 * e + 1], dot);
-        }
-      }
-      sc = dot * p.scale_log2;
-    }
-    float cm = sc;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) cm = fmaxf(cm, __shfl_xor_sync(kFull, cm, o));
-    const float mn = fmaxf(m, cm);
-    if (!__any_sync(kFull, sc != -INFINITY)) continue;   // (NaN is a score too)
-    const float alpha = exp2f(m - mn);
-    const float pv = sc == -INFINITY ? 0.f : exp2f(sc - mn);
-    float ps = pv;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) ps += __shfl_xor_sync(kFull, ps, o);
-    l = fmaf(l, alpha, ps);
-#pragma unroll
-    for (int i = 0; i < N; ++i) acc[i] *= alpha;
-    m = mn;
-    const int nj = min(32, count - c);
-    for (int j = 0; j < nj; ++j) {
-      const float pj = __shfl_sync(kFull, pv, j);
-      const int pg = __shfl_sync(kFull, page, j);
-      const int sl = __shfl_sync(kFull, slot, j);
-      if (pg < 0) continue;
-      const uint16_t* vr = reinterpret_cast<const uint16_t*>(p.vc + pg * p.v_sb + sl * p.v_ss + kvh * p.v_sh) + lane * N;
-#pragma unroll
-      for (int i = 0; i < N; ++i) acc[i] = fmaf(pj, to_float<T>(__ldg(vr + i)), acc[i]);
-    }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  uint16_t* dst = reinterpret_cast<uint16_t*>(p.out + row * p.o_st + hq * p.o_sh) + lane * N;
-#pragma unroll
-  for (int i = 0; i < N; ++i) dst[i] = static_cast<uint16_t>(pack2<T>(acc[i] * inv, 0.f));
-  if (lane == 0 && p.lse)
-    p.lse[static_cast<long long>(row) * p.Hq + hq] = l == 0.f ? kSentinel : (m + log2f(l)) * kLn2;
 }
 
 // ----------------------------------------------------------------------------
@@ -315,6 +204,7 @@ __device__ __forceinline__ void regs_down() {
 enum class Fetch { kBoxes, kRows, kPieces };
 struct TileParams {
   Params p;
+  int dh;                   // head_dim: D, or 32 in the kernel for 64
   int R, lR;                // token rows per TMA box, and its log2
   int bs_log2;              // log2 of the page size, or -1
   FastDiv div_g, div_bs;
@@ -798,6 +688,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
         static_assert(kThr % kPer == 0, "rows per pass");
         const int me = threadIdx.x - (NQ * 4 + NQ) * 32;
         const int c = me % kPer, first = me / kPer;
+        const int bytes = c * 8 < a.dh ? 16 : 0;   // behind head_dim: zeros
         int s = 0, out = 0, fills = 0;          // slot to fill, slot to hand over next
         uint32_t phase = 0;
         auto hand_over = [&]() {
@@ -823,7 +714,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
           for (int kv = 0; kv < 2; ++kv) {
             ok = __all_sync(kFull, mbar_wait(kv_empty(s), phase ^ 1));
             if (!ok) break;
-            const char* base = (kv ? p.vc + j.kvh * p.v_sh : p.kc + j.kvh * p.k_sh) + c * 16;
+            const char* base = (kv ? p.vc + j.kvh * p.v_sh : p.kc + j.kvh * p.k_sh) + c * bytes;
             const long long sb = kv ? p.v_sb : p.k_sb, ss = kv ? p.v_ss : p.k_ss;
 #pragma unroll
             for (int i = 0; i < kRows; ++i) {
@@ -832,10 +723,10 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
               const int key = k * kTN + r;
               const int tok = key < j.sink_keys ? key : key + j.delta;
               const int slot = tok - static_cast<int>(fast_div(tok, a.div_bs)) * p.bs;
-              asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(
+              asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                                skv + s * C::kKV + (c >> 3) * kTN * 128 + r * 128 +
                                (((c & 7) ^ (r & 7)) << 4)),
-                           "l"(base + page[i] * sb + slot * ss)
+                           "l"(base + page[i] * sb + slot * ss), "r"(bytes)
                            : "memory");
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
@@ -1136,12 +1027,13 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
       for (int i = 0; i < kPer; ++i) {
         const int r = i * (128 / kPer) + tid / kPer;
         const int pr = r0 + r;
-        const bool in = pr < j.rows;
+        const bool in = pr < j.rows && c * 8 < a.dh;
         const int tok = in ? static_cast<int>(fast_div(pr, a.div_g)) : 0;
         const char* src = in ? p.q + (j.s.start + tok) * p.q_st + (j.kvh * p.G + pr - tok * p.G) * p.q_sh + c * 16
                              : p.q;
         // asynchronous, past the first-level cache (which shared memory leaves
-        // smaller than the tile); rows behind the sequence become zero
+        // smaller than the tile); rows behind the sequence, and dimensions behind
+        // head_dim, become zero
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
                          sq + t * C::kQTile + (c >> 3) * 128 * 128 + r * 128 +
                          (((c & 7) ^ (r & 7)) << 4)),
@@ -1325,7 +1217,7 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
         for (int i = 0; i < kPer; ++i) {
           const int r = i * (128 / kPer) + tid / kPer;
           const int q = r0 + r;
-          if (ok && q < j.rows) {
+          if (ok && q < j.rows && c * 8 < a.dh) {
             const int qt = static_cast<int>(fast_div(q, a.div_g));
             uint4 v;
             asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -1409,7 +1301,8 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(const TileParams a) {
   const float inv = sum == 0.f ? 0.f : 1.f / sum;
   uint32_t* dst = reinterpret_cast<uint32_t*>(p.out + row * p.o_st + hq * p.o_sh + lane * N * 2);
 #pragma unroll
-  for (int i = 0; i < N / 2; ++i) dst[i] = pack2<T>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
+  for (int i = 0; i < N / 2; ++i)
+    if (lane * N < a.dh) dst[i] = pack2<T>(acc[2 * i] * inv, acc[2 * i + 1] * inv);
   if (lane == 0 && p.lse) p.lse[w] = sum == 0.f ? kSentinel : top + logf(sum);
 }
 
@@ -1491,14 +1384,6 @@ static Params make_params(const pa_prompt_params* p) {
   return a;
 }
 
-template <typename T>
-static cudaError_t launch_rows(const Params& a, cudaStream_t stream) {
-  const long long warps = static_cast<long long>(a.T) * a.Hq;
-  const dim3 grid(static_cast<unsigned>((warps + 3) / 4));
-  prompt_rows_kernel<T, 32><<<grid, 128, 0, stream>>>(a);
-  return cudaGetLastError();
-}
-
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
   static std::once_flag once;
@@ -1513,16 +1398,22 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+// Dimensions of a row in the kernel that takes it: head_dim 32 runs as 64, the upper
+// half zero.
+static int kernel_dim(const pa_prompt_params* p) { return std::max(64, p->head_dim); }
+
 // A paged cache as (64 dims, slot, 64-dim chunk, head, page); a box is R token
-// rows of one chunk, 128-byte swizzled.
+// rows of one chunk, 128-byte swizzled. Of a head_dim of 32 the box's upper half lies
+// outside the first extent and is filled with zeros.
 static bool encode_map(CUtensorMap* map, const pa_prompt_params* p, const void* base,
                        int64_t s_block, int64_t s_slot, int64_t s_head, int R) {
   auto fn = encode_fn();
   if (!fn) return false;
   const CUtensorMapDataType dt =
       p->dtype == PA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const cuuint64_t dims[5] = {64, static_cast<cuuint64_t>(p->block_size),
-                              static_cast<cuuint64_t>(p->head_dim / 64),
+  const cuuint64_t dims[5] = {static_cast<cuuint64_t>(std::min(64, p->head_dim)),
+                              static_cast<cuuint64_t>(p->block_size),
+                              static_cast<cuuint64_t>(kernel_dim(p) / 64),
                               static_cast<cuuint64_t>(p->num_kv_heads),
                               static_cast<cuuint64_t>(p->num_blocks)};
   const cuuint64_t strides[4] = {static_cast<cuuint64_t>(s_slot) * 2, 128,
@@ -1548,7 +1439,7 @@ static bool row_list(const pa_prompt_params* p, int64_t s_block, int64_t s_slot,
   if (sb < 0 || ss < 0 || sh < 0) return false;
   int64_t u = std::gcd(std::gcd(sb, ss), sh);
   if (u == 0) u = p->head_dim;
-  if (u < p->head_dim || u >= (1ll << 38)) return false;
+  if (p->head_dim < 64 || u < p->head_dim || u >= (1ll << 38)) return false;
   r->unit = u;
   r->rows = (p->num_blocks - 1) * (sb / u) + (p->block_size - 1) * (ss / u) +
             (p->num_kv_heads - 1) * (sh / u) + 1;
@@ -1573,10 +1464,8 @@ static bool encode_rows(CUtensorMap* map, const pa_prompt_params* p, const void*
             CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// How a call runs: the CUDA-core path, or row tiles of 128 * nq with the keys
-// in `splits` parts.
+// How a call runs: row tiles of 128 * nq, the keys in `splits` parts.
 struct Plan {
-  bool rows_path;
   int nq, splits;
   long long tiles;          // bound on the row tiles of a KV head
   size_t ws_bytes;
@@ -1584,14 +1473,12 @@ struct Plan {
 static Plan make_plan(const pa_prompt_params* p, int sms) {
   Plan pl = {};
   pl.splits = 1;
-  pl.rows_path = p->head_dim == 32;
-  if (pl.rows_path) return pl;
   const int g = p->num_heads / p->num_kv_heads;
   const long long packed = static_cast<long long>(p->num_tokens) * g;   // rows of a KV head
   // Two row tiles per CTA keep the matrix pipe busy; a batch whose sequences
   // bring no more than one tile each would leave the second empty.
-  pl.nq = p->head_dim == 256 || p->head_dim == 64 || packed <= 128ll * p->batch ? 1 : 2;
-  const long long slots = static_cast<long long>(sms) * (p->head_dim == 64 ? 2 : 1);   // CTAs at once
+  pl.nq = p->head_dim == 256 || p->head_dim <= 64 || packed <= 128ll * p->batch ? 1 : 2;
+  const long long slots = static_cast<long long>(sms) * (p->head_dim <= 64 ? 2 : 1);   // CTAs at once
   // sum over the sequences of ceil(rows / tile), whatever their shares are
   pl.tiles = packed / (128 * pl.nq) + std::min<long long>(p->batch, p->num_tokens);
   const long long ctas = pl.tiles * p->num_kv_heads;
@@ -1610,7 +1497,7 @@ static Plan make_plan(const pa_prompt_params* p, int sms) {
   }
   if (pl.splits > 1)
     pl.ws_bytes = static_cast<size_t>(pl.splits) * p->num_tokens * p->num_heads *
-                  (p->head_dim + 1) * sizeof(float);
+                  (kernel_dim(p) + 1) * sizeof(float);
   return pl;
 }
 
@@ -1710,11 +1597,7 @@ pa_status_t pa_prompt(const pa_prompt_params* p, cudaStream_t stream) {
   TileParams a;
   memset(&a, 0, sizeof(a));
   a.p = make_params(p);
-  cudaError_t e;
-  if (pl.rows_path) {
-    e = half ? launch_rows<__half>(a.p, stream) : launch_rows<__nv_bfloat16>(a.p, stream);
-    return e == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
-  }
+  a.dh = p->head_dim;
   // box rows: a power of two in the page size, at most 32 (where a window starts,
   // up to R - 1 hidden keys are read)
   a.R = 8;
@@ -1728,7 +1611,7 @@ pa_status_t pa_prompt(const pa_prompt_params* p, cudaStream_t stream) {
   a.div_bs = make_fastdiv(static_cast<uint32_t>(p->block_size));
   a.splits = pl.splits;
   a.o_part = static_cast<float*>(p->workspace);
-  a.lse_part = a.o_part + static_cast<size_t>(pl.splits) * p->num_tokens * p->num_heads * p->head_dim;
+  a.lse_part = a.o_part + static_cast<size_t>(pl.splits) * p->num_tokens * p->num_heads * kernel_dim(p);
   CUtensorMap mk, mv;
   memset(&mk, 0, sizeof(mk));
   memset(&mv, 0, sizeof(mv));
@@ -1748,8 +1631,9 @@ pa_status_t pa_prompt(const pa_prompt_params* p, cudaStream_t stream) {
   } else {
     fetch = Fetch::kPieces;
   }
-  e = half ? launch_tiles_d<__half>(mk, mv, a, pl, fetch, p->head_dim, stream)
-           : launch_tiles_d<__nv_bfloat16>(mk, mv, a, pl, fetch, p->head_dim, stream);
+  const cudaError_t e =
+      half ? launch_tiles_d<__half>(mk, mv, a, pl, fetch, p->head_dim, stream)
+               : launch_tiles_d<__nv_bfloat16>(mk, mv, a, pl, fetch, p->head_dim, stream);
   return e == cudaSuccess ? PA_OK : PA_ERR_LAUNCH;
 }
 

@@ -431,7 +431,7 @@ def _relayout(x, kind):
 @pytest.mark.parametrize("bs", [1, 4, 12, 16])
 @pytest.mark.parametrize("kinds", [("plain", "heads first"), ("half of pairs", "head outermost"),
                                    ("padded rows", "padded rows"), ("plain", "padded pages")])
-@pytest.mark.parametrize("hkv,d", [(2, 128), (1, 64), (3, 256)])
+@pytest.mark.parametrize("hkv,d", [(2, 128), (1, 64), (3, 256), (3, 32)])
 def test_prompt_cache_layouts(bs, kinds, hkv, d):
     """Every way the keys' rows are fetched gives the bits of the plain layout."""
     import paged_attention as pa
