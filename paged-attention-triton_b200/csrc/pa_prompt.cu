@@ -1268,6 +1268,7 @@ __global__ void __launch_bounds__(128) prompt_join_kernel(const TileParams a) {
   const int row = static_cast<int>(w / p.Hq);
   const int hq = static_cast<int>(w - static_cast<long long>(row) * p.Hq);
   asm volatile("griddepcontrol.wait;" ::: "memory");   // the splits' partials
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (seq_of_row(p, row) < 0) return;
   // lane = split: its weight, then all splits' rows in flight together
   float sum = 0.f, acc[N], top = -INFINITY;
