@@ -122,7 +122,7 @@ __device__ __forceinline__ int seq_of_row(const Params& p, int row) {
 //   P = 2^(c S - m), rounded to the 16-bit type, over S in TMEM
 //   O (128 x D, TMEM) += P V          one tcgen05.mma per 16 tokens
 //
-// Roles: producer warps (lane = one TMA box of a page), a warp that cleans V
+// Roles: producer warps (lane = one copy: a box of a page), a warp that cleans V
 // tiles at the edges of what is visible, one issuing warp per 128 rows, and four
 // softmax warps per 128 rows, thread = row, so that row maxima and sums need no
 // exchange. With NQ = 2 the two row tiles alternate on the matrix pipe: while
@@ -130,8 +130,8 @@ __device__ __forceinline__ int seq_of_row(const Params& p, int row) {
 // head_dim 256) S has two buffers and the next tile's S is computed during the
 // current softmax.
 //
-// What bounds it (8192 tokens, Hq32/Hkv8, D 128, window 4096 / none: 357 / 451 us,
-// 1.15 / 1.22 PFLOP/s): the chain from a tile's S to its P. 256 rows x 128 keys
+// What bounds it (8192 tokens, Hq32/Hkv8, D 128, window 4096 / none: 363 / 458 us,
+// 1.13 / 1.20 PFLOP/s): the chain from a tile's S to its P. 256 rows x 128 keys
 // take the matrix pipe 2048 cycles, the special function units as many, and the
 // tile's turn ~3000: load of S 250, maximum 300-400, exponentials 1400 (1024 if no
 // other warp ran), then the rest of P V and the next S 1000. Tried and slower:
