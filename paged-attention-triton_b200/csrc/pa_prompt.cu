@@ -1170,8 +1170,10 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
       f2_split(sum[1], x2, x3);
       l += (x0 + x1) + (x2 + x3);
     }
-    if (n > 0 && ok) {
-      ok = mbar_wait(o_done(t), C::kSBufs == 2 ? (n - 1) & 1 : 0);
+    if (ok) {
+      // No tile: no product has waited for the staged queries, whose place the output
+      // takes below, so their last copies are waited for here.
+      ok = n > 0 ? mbar_wait(o_done(t), C::kSBufs == 2 ? (n - 1) & 1 : 0) : mbar_wait(q_full(t), 0);
       ok = __all_sync(kFull, ok);
       tc_fence_after();
     }

@@ -96,6 +96,26 @@ def test_prompt_rows_before_the_sequence_see_nothing():
         assert (o[40:49] == 0).all() and (lse[40:49] == -1e30).all()
 
 
+@pytest.mark.parametrize("hkv,g,d", [(4, 4, 128), (8, 1, 128), (8, 4, 64), (4, 4, 32), (2, 4, 256)])
+def test_prompt_rows_that_see_nothing_are_zero_over_large_queries(hkv, g, d):
+    """Whole row tiles without a visible token: what is staged of their queries, which come
+    from memory late, must not end up in the output."""
+    import paged_attention as pa
+    n, b = 1024, 6
+    k = torch.full((4, 16, hkv, d), 3.0, device="cuda").half()
+    table = torch.full((b, 4), -1, dtype=torch.int32, device="cuda")
+    starts = torch.arange(0, n * b + 1, n, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(b, dtype=torch.int32, device="cuda")
+    q = torch.full((n * b, hkv * g, d), 5.0, device="cuda").half()
+    big = torch.empty(64 << 20, dtype=torch.float32, device="cuda")
+    for i in range(12):
+        out = torch.full_like(q, 7.0)
+        big.fill_(float(i))                       # the queries leave the caches
+        o, lse = pa.paged_prompt_attention(q, k, k, table, starts, lens, 16, num_splits=1, out=out,
+                                           return_lse=True)
+        assert (o == 0).all() and (lse == -1e30).all(), f"pass {i}"
+
+
 def test_prompt_of_one_token_is_decode():
     import paged_attention as pa
     lens, window, sinks = [1, 40, 700, 64], 100, 4
