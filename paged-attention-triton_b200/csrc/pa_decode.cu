@@ -602,12 +602,24 @@ __device__ __forceinline__ void store_row(float* row, int lane, const RowV<N>& r
   }
 }
 
+// Whether a piece of this LSE goes into a merge, and the LSE of the merged pieces.
+// Under a window a NaN LSE is a piece with a score of NaN or +infinity: it counts, and
+// the row and its LSE become NaN. (Full-length steps leave such pieces out.)
+template <bool kWin>
+__device__ __forceinline__ bool counts(float lse) {
+  return kWin ? !(lse <= kValidLse) : lse > kValidLse;
+}
+template <bool kWin>
+__device__ __forceinline__ float merged_lse(float sum, float lse) {
+  return (kWin ? sum != 0.f : sum > 0.f) ? lse : kSentinel;
+}
+
 // split_kv_kernel.py:101-122: skip lse <= -1e29, merge by running max, divide
 // by max(sum, 1e-20); no valid piece gives 0 and LSE -1e30. `src(k, row, lse)`
 // locates piece k's normalised row (D floats) and LSE; rows are read from
 // global memory through L2 (kGlobal) or from shared memory. Each lane returns
 // its D/32 dims.
-template <bool kGlobal, int D, class Src>
+template <bool kGlobal, int D, bool kWin, class Src>
 __device__ __forceinline__ void merge_rows(int n, int lane, const Src& src,
                                            RowV<HD<D>::kLaneF>& out, float& lse_out) {
   constexpr int N = HD<D>::kLaneF;
@@ -642,11 +654,11 @@ __device__ __forceinline__ void merge_rows(int n, int lane, const Src& src,
     float gmax = kValidLse;
 #pragma unroll
     for (int u = 0; u < kBatch; ++u)
-      if (l[u] > kValidLse) gmax = fmaxf(gmax, l[u]);
+      if (counts<kWin>(l[u])) gmax = fmaxf(gmax, l[u]);
     float gsum = 0.f;
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const float wgt = (l[u] > kValidLse) ? exp2f((l[u] - gmax) * kLog2e) : 0.f;
+      const float wgt = counts<kWin>(l[u]) ? exp2f((l[u] - gmax) * kLog2e) : 0.f;
       gsum += wgt;
 #pragma unroll
       for (int i = 0; i < N; ++i) a.f[i] = fmaf(wgt, v[u].f[i], a.f[i]);
@@ -654,13 +666,13 @@ __device__ __forceinline__ void merge_rows(int n, int lane, const Src& src,
     const float inv = __fdividef(1.f, fmaxf(gsum, 1e-20f));
 #pragma unroll
     for (int i = 0; i < N; ++i) out.f[i] = a.f[i] * inv;
-    lse_out = gsum > 0.f ? gmax + __logf(gsum) : kSentinel;
+    lse_out = merged_lse<kWin>(gsum, gmax + __logf(gsum));
     return;
   }
   const float l0 = (lane < n) ? ld_lse(lane) : kValidLse;
 #pragma unroll
   for (int u = 0; u < kBatch; ++u) v[u] = (u < n) ? ld_row(u) : zero;
-  float gmax = (l0 > kValidLse) ? l0 : kValidLse;
+  float gmax = (l0 > kValidLse) ? l0 : kValidLse;   // (without NaN)
   for (int k = lane + 32; k < n; k += 32) {
     const float l = ld_lse(k);
     if (l > kValidLse) gmax = fmaxf(gmax, l);
@@ -670,7 +682,7 @@ __device__ __forceinline__ void merge_rows(int n, int lane, const Src& src,
   float gsum = 0.f;
   for (int base = 0; base < n; base += 32) {
     const float lb = (base == 0) ? l0 : ((base + lane < n) ? ld_lse(base + lane) : kValidLse);
-    const float wl = (lb > kValidLse) ? exp2f((lb - gmax) * kLog2e) : 0.f;
+    const float wl = counts<kWin>(lb) ? exp2f((lb - gmax) * kLog2e) : 0.f;
     float ws = wl;
 #pragma unroll
     for (int o2 = 16; o2 > 0; o2 >>= 1) ws += __shfl_xor_sync(kFull, ws, o2);
@@ -685,7 +697,7 @@ __device__ __forceinline__ void merge_rows(int n, int lane, const Src& src,
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         const float wgt = __shfl_sync(kFull, wl, (k0 + u) & 31);
-        if (k0 + u < cnt && wgt > 0.f) {
+        if (k0 + u < cnt && (kWin ? wgt != 0.f : wgt > 0.f)) {
 #pragma unroll
           for (int i = 0; i < N; ++i) a.f[i] = fmaf(wgt, v[u].f[i], a.f[i]);
         }
@@ -695,7 +707,7 @@ __device__ __forceinline__ void merge_rows(int n, int lane, const Src& src,
   const float inv = 1.f / fmaxf(gsum, 1e-20f);
 #pragma unroll
   for (int i = 0; i < N; ++i) out.f[i] = a.f[i] * inv;
-  lse_out = gsum > 0.f ? gmax + logf(gsum) : kSentinel;
+  lse_out = merged_lse<kWin>(gsum, gmax + logf(gsum));
 }
 
 // The same rule over rows in shared memory, as one compact loop with a running
@@ -703,7 +715,7 @@ __device__ __forceinline__ void merge_rows(int n, int lane, const Src& src,
 // piece on the step's tail, where straight-line code is paid for in
 // instruction fetch, and shared-memory loads are short enough not to need
 // batching.
-template <int D, class Src>
+template <int D, bool kWin, class Src>
 __device__ __forceinline__ void merge_rows_smem(int n, int lane, const Src& src,
                                                 RowV<HD<D>::kLaneF>& out, float& lse_out) {
   constexpr int N = HD<D>::kLaneF;
@@ -717,7 +729,7 @@ __device__ __forceinline__ void merge_rows_smem(int n, int lane, const Src& src,
     const float* lp;
     src(k, row, lp);
     const float l = *lp;
-    if (l > kValidLse) {
+    if (counts<kWin>(l)) {
       const RowV<N> v = load_row<false, N>(row, lane);
       const float mn = fmaxf(m, l);
       const float f = exp2f((m - mn) * kLog2e);
@@ -731,7 +743,7 @@ __device__ __forceinline__ void merge_rows_smem(int n, int lane, const Src& src,
   const float inv = __fdividef(1.f, fmaxf(sum, 1e-20f));
 #pragma unroll
   for (int i = 0; i < N; ++i) out.f[i] = a.f[i] * inv;
-  lse_out = sum > 0.f ? m + __logf(sum) : kSentinel;
+  lse_out = merged_lse<kWin>(sum, m + __logf(sum));
 }
 
 // Final output row of (b, hq): this lane's D/32 dims in the output dtype.
@@ -764,7 +776,7 @@ __device__ __forceinline__ float* gslot_lse(const KParams& p, long long slot, in
 }
 
 // The last group to finish a segment merges the groups' partials.
-template <typename T, int D>
+template <typename T, int D, bool kWin>
 __device__ __forceinline__ void merge_groups(const KParams& p, const Ranges& rg, int b, int kvh,
                                              int qc, int gc, int seg_lo, int seg_hi, int lane) {
   const int g_first = seg_lo / rg.P;
@@ -809,14 +821,14 @@ __device__ __forceinline__ void merge_groups(const KParams& p, const Ranges& rg,
         float gmax = kValidLse;
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          if (l[jj][k] > kValidLse) gmax = fmaxf(gmax, l[jj][k]);
+          if (counts<kWin>(l[jj][k])) gmax = fmaxf(gmax, l[jj][k]);
         float gsum = 0.f;
         RowV<N> a;
 #pragma unroll
         for (int i = 0; i < N; ++i) a.f[i] = 0.f;
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const float wgt = (l[jj][k] > kValidLse) ? exp2f((l[jj][k] - gmax) * kLog2e) : 0.f;
+          const float wgt = counts<kWin>(l[jj][k]) ? exp2f((l[jj][k] - gmax) * kLog2e) : 0.f;
           gsum += wgt;
 #pragma unroll
           for (int i = 0; i < N; ++i) a.f[i] = fmaf(wgt, v[jj][k].f[i], a.f[i]);
@@ -825,7 +837,7 @@ __device__ __forceinline__ void merge_groups(const KParams& p, const Ranges& rg,
 #pragma unroll
         for (int i = 0; i < N; ++i) a.f[i] *= inv;
         store_out<T, D>(p, b, kvh * p.G + qc * 8 + j0 + jj, lane, a,
-                        gsum > 0.f ? gmax + __logf(gsum) : kSentinel);
+                        merged_lse<kWin>(gsum, gmax + __logf(gsum)));
       }
     }
     return;
@@ -839,7 +851,7 @@ __device__ __forceinline__ void merge_groups(const KParams& p, const Ranges& rg,
     };
     RowV<HD<D>::kLaneF> o;
     float lse;
-    merge_rows<true, D>(n, lane, src, o, lse);
+    merge_rows<true, D, kWin>(n, lane, src, o, lse);
     store_out<T, D>(p, b, kvh * p.G + qc * 8 + j, lane, o, lse);
   }
 }
@@ -857,7 +869,7 @@ __device__ __forceinline__ void merge_splits(const KParams& p, int b, int kvh, i
     };
     RowV<HD<D>::kLaneF> o;
     float lse;
-    merge_rows<true, D>(p.ns, lane, src, o, lse);
+    merge_rows<true, D, false>(p.ns, lane, src, o, lse);
     store_out<T, D>(p, b, hq, lane, o, lse);
   }
 }
@@ -1434,9 +1446,12 @@ __global__ void __launch_bounds__(NW * 32, 1)
       mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 8));
       mx = fmaxf(mx, __shfl_xor_sync(kFull, mx, 16));
       const float mn = fmaxf(m_run[e], mx);
-      alpha[e] = exp2f((m_run[e] - mn) * scl);
+      // Under a window, while every score is -infinity (or NaN, which the maximum leaves
+      // out) the exponents are taken against 0: weights of 0, and of NaN for NaN.
+      const float mref = kWin && mn == -INFINITY ? 0.f : mn;
+      alpha[e] = exp2f((m_run[e] - mref) * scl);
       m_run[e] = mn;
-      mneg[e] = -mn * scl;
+      mneg[e] = -mref * scl;
     }
     float psum[2] = {0.f, 0.f};
 #pragma unroll
@@ -1547,9 +1562,11 @@ __global__ void __launch_bounds__(NW * 32, 1)
       const int c = qd * 2 + e;
       if (c >= gc) continue;
       const int hq = kvh * G + qc * 8 + c;
-      const float lv = fmaxf(lsum[e], 1e-20f);
+      // (under a window NaN stays NaN: the merges and the caller see it in the LSE)
+      const float lv = kWin && lsum[e] != lsum[e] ? lsum[e] : fmaxf(lsum[e], 1e-20f);
       const float inv_l = __fdividef(1.f, lv);
-      const float lse = (m_run[e] * scl + __log2f(lv)) * kLn2;
+      float lse = (m_run[e] * scl + __log2f(lv)) * kLn2;
+      if (kWin && lsum[e] == 0.f) lse = kSentinel;   // every score is -infinity
       if (dest == 0) {
         char* dst = p.out + b * p.o_sb + hq * p.o_sh;
 #pragma unroll
@@ -1628,7 +1645,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
       };
       RowV<H::kLaneF> o4;
       float lse;
-      merge_rows_smem<D>(nw, lane, src, o4, lse);
+      merge_rows_smem<D, kWin>(nw, lane, src, o4, lse);
       if (fl & kGroupSeg) {
         store_out<T, D>(p, b, kvh * G + qc * 8 + j, lane, o4, lse);
       } else if (kClu) {
@@ -1652,7 +1669,7 @@ __global__ void __launch_bounds__(NW * 32, 1)
     for (int k = 0; k < npend; ++k) {
       if (!(merge_mask & (1u << k))) continue;
       const int* r = pend_rec[kSplit ? 0 : warp][k];
-      merge_groups<T, D>(p, rg, r[0], r[1], r[2], r[3], r[4], r[5], lane);
+      merge_groups<T, D, kWin>(p, rg, r[0], r[1], r[2], r[3], r[4], r[5], lane);
       if (lane == 0) atomicExch(pend_counter(r), 0);
     }
   }
@@ -1867,14 +1884,14 @@ __global__ void __launch_bounds__(256) merge_segments_kernel(const MergeParams m
       float bm = mx;
 #pragma unroll
       for (int t = 0; t < kRows; ++t)
-        if (l[t] > kValidLse) bm = fmaxf(bm, l[t]);
+        if (counts<kWin>(l[t])) bm = fmaxf(bm, l[t]);
       const float f = exp2f((mx - bm) * kLog2e);
       sum *= f;
 #pragma unroll
       for (int i = 0; i < N; ++i) acc.f[i] *= f;
 #pragma unroll
       for (int t = 0; t < kRows; ++t) {
-        const float wgt = (l[t] > kValidLse) ? exp2f((l[t] - bm) * kLog2e) : 0.f;
+        const float wgt = counts<kWin>(l[t]) ? exp2f((l[t] - bm) * kLog2e) : 0.f;
         sum += wgt;
 #pragma unroll
         for (int i = 0; i < N; ++i) acc.f[i] = fmaf(wgt, v[t].f[i], acc.f[i]);
@@ -1923,7 +1940,8 @@ __global__ void __launch_bounds__(256) merge_segments_kernel(const MergeParams m
   } else {
     *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  if (lane == 0 && m.lse) m.lse[b * m.G * m.Hkv + hq] = sum > 0.f ? mx + logf(sum) : kSentinel;
+  if (lane == 0 && m.lse)
+    m.lse[b * m.G * m.Hkv + hq] = merged_lse<kWin>(sum, mx + logf(sum));
 }
 
 // ----------------------------------------------------------------------------

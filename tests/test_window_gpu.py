@@ -217,3 +217,75 @@ def test_nan_in_visible_places_shows(d, bs, s):
             assert o[:, :2, dims].isnan().all(), f"token {t}"
             o[:, :2, dims] = clean[:, :2, dims]
             assert torch.equal(o, clean)
+
+
+def _odd_numbers_case(d, bs, hkv, g, batch, s, seed):
+    gen = torch.Generator().manual_seed(seed)
+    pages = -(-s // bs)
+    k, v = (torch.randn(pages, bs, hkv, d, generator=gen).half().cuda() for _ in range(2))
+    q = (torch.rand(batch, hkv * g, d, generator=gen) + 0.01).half().cuda()
+    table = torch.arange(pages, dtype=torch.int32, device="cuda").repeat(batch, 1)
+    return q, k, v, table, torch.full((batch,), s, dtype=torch.int32, device="cuda")
+
+
+# (one row and many, groups and full heads, rows merged in every place where pieces meet)
+ODD_SHAPES = [(128, 16, 8, 4, 1), (128, 16, 32, 1, 1), (128, 16, 2, 4, 3), (128, 16, 2, 8, 2), (128, 32, 4, 3, 40),
+              (64, 16, 2, 4, 1), (64, 32, 3, 1, 30), (256, 32, 2, 2, 1), (256, 16, 1, 8, 9)]
+
+
+@pytest.mark.parametrize("d,bs,hkv,g,batch", ODD_SHAPES)
+@pytest.mark.parametrize("s,window,sinks", [(1, 1, 0), (3000, 1024, 1), (700, 350, 2), (900, 1, 1)])
+def test_nan_and_infinite_scores_show_in_output_and_lse(d, bs, hkv, g, batch, s, window, sinks):
+    """A NaN query, or a visible key that scores NaN or +infinity, makes its rows NaN, their
+    LSE too, also where it is the only token of a tile; the others keep their bits."""
+    import paged_attention as pa
+    q, k, v, table, lens = _odd_numbers_case(d, bs, hkv, g, batch, s, seed=s + d + g)
+
+    def run(q):
+        return pa.paged_attention(q, k, v, table, lens, bs, window=window, num_sinks=sinks, return_lse=True)
+    clean, clean_lse = run(q)
+    assert clean.isfinite().all() and clean_lse.isfinite().all()
+
+    def check(got, rows, heads, what):
+        o, lse = got
+        assert o[rows, heads].isnan().all(), f"{what}: O"
+        assert lse[rows, heads].isnan().all(), f"{what}: LSE"
+        o[rows, heads], lse[rows, heads] = clean[rows, heads], clean_lse[rows, heads]
+        assert torch.equal(o, clean) and torch.equal(lse, clean_lse), f"{what}: other rows"
+    bad = q.clone()
+    bad[batch // 2, hkv * g - 1, 3] = float("nan")
+    check(run(bad), batch // 2, hkv * g - 1, "query")
+    every = slice(None)
+    low = max(0, s - window)
+    for t in sorted({0, low, (low + s) // 2, s - 1} - (set() if sinks or not low else {0})):
+        for value in (float("nan"), float("inf")):
+            kept = k[t // bs, t % bs, hkv - 1, 5].clone()
+            k[t // bs, t % bs, hkv - 1, 5] = value
+            got = run(q)
+            k[t // bs, t % bs, hkv - 1, 5] = kept
+            check(got, every, slice((hkv - 1) * g, hkv * g), f"key {t} {value}")
+
+
+@pytest.mark.parametrize("d,bs,hkv,g,batch", ODD_SHAPES)
+@pytest.mark.parametrize("s,window,sinks", [(1, 1, 0), (3000, 1024, 1), (700, 350, 2)])
+def test_scores_of_minus_infinity_weigh_nothing(d, bs, hkv, g, batch, s, window, sinks):
+    """Visible keys that score -infinity: some, whole tiles of them, all (as if nothing were seen)."""
+    import paged_attention as pa
+    q, k, v, table, lens = _odd_numbers_case(d, bs, hkv, g, batch, s, seed=s + d)
+    seen = torch.tensor([t for t in range(s) if t < sinks or t >= s - window])
+    for dead in (seen[:1], seen[: len(seen) // 2], seen[len(seen) // 3:], seen):
+        kk = k.clone()
+        kk[dead.cuda() // bs, dead.cuda() % bs, :, 5] = float("-inf")
+        o, lse = pa.paged_attention(q, kk, v, table, lens, bs, window=window, num_sinks=sinks, return_lse=True)
+        left = torch.tensor(sorted(set(seen.tolist()) - set(dead.tolist())), dtype=torch.long)
+        if not len(left):
+            assert (o == 0).all() and (lse == -1e30).all()
+            continue
+        # the same rows over the tokens that are left, in 64 bits; tolerances as in the definition's helper
+        k2, v2 = (x.cpu()[left // bs, left % bs].double().repeat_interleave(g, 1) for x in (k, v))
+        sc = torch.einsum("bhd,thd->bht", q.cpu().double(), k2) * d ** -0.5
+        big = (torch.einsum("bhd,thd->bht", q.cpu().double(), k2.abs()) * d ** -0.5).amax(-1, keepdim=True)
+        want = torch.einsum("bht,thd->bhd", torch.softmax(sc, -1), v2)
+        tol = (2 * d * 2.0 ** -24 * big + 2.0 ** -16) * v2.abs().max() + 2.0 ** -11 * want.abs()
+        assert_matches(o, want, tol, f"{len(dead)} of {len(seen)} at -infinity")
+        assert_lse(lse, torch.logsumexp(sc, -1), d, f"{len(dead)} of {len(seen)} at -infinity")
