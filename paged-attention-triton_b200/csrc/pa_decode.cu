@@ -2209,7 +2209,9 @@ __global__ void __launch_bounds__(128) generic_reduce_kernel(const GenParams g) 
   uint16_t* dst = reinterpret_cast<uint16_t*>(g.out + b * g.o_sb + hq * g.o_sh) + lane * N;
 #pragma unroll
   for (int i = 0; i < N; ++i) dst[i] = Mma<T>::from_float(acc[i] * inv);
-  if (lane == 0 && g.lse) g.lse[w] = gsum > 0.f ? gmax + logf(gsum) : kSentinel;
+  // (under a window the LSE of a row with a NaN is NaN, as its output is)
+  if (lane == 0 && g.lse)
+    g.lse[w] = (g.window ? gsum != 0.f : gsum > 0.f) ? gmax + logf(gsum) : kSentinel;
 }
 
 // ----------------------------------------------------------------------------

@@ -230,7 +230,9 @@ def _odd_numbers_case(d, bs, hkv, g, batch, s, seed):
 
 # (one row and many, groups and full heads, rows merged in every place where pieces meet)
 ODD_SHAPES = [(128, 16, 8, 4, 1), (128, 16, 32, 1, 1), (128, 16, 2, 4, 3), (128, 16, 2, 8, 2), (128, 32, 4, 3, 40),
-              (64, 16, 2, 4, 1), (64, 32, 3, 1, 30), (256, 32, 2, 2, 1), (256, 16, 1, 8, 9)]
+              (64, 16, 2, 4, 1), (64, 32, 3, 1, 30), (256, 32, 2, 2, 1), (256, 16, 1, 8, 9),
+              # on the CUDA cores
+              (32, 16, 2, 4, 1), (32, 8, 3, 1, 9), (64, 5, 2, 2, 3), (128, 1, 1, 4, 2), (256, 12, 2, 1, 1)]
 
 
 @pytest.mark.parametrize("d,bs,hkv,g,batch", ODD_SHAPES)
