@@ -251,6 +251,8 @@ def paged_attention(Q, K_Cache, V_Cache, Block_Table, seq_len, block_size, num_s
     ``kernel_variant`` (0 = automatic) pins one tile/warp/stage variant of the
     CUDA kernel; it exists for tuning and tests.
     """
+    if num_sinks and window is None:
+        window_args("paged_attention", window, num_sinks)   # refused, with gradients too
     if torch.is_grad_enabled() and (Q.requires_grad or K_Cache.requires_grad
                                     or V_Cache.requires_grad):
         if scale is None and not return_lse and not return_partials and window is None:

@@ -32,6 +32,13 @@ def test_window_with_grad_is_inference_only():
         pa.paged_attention(q, k, v, bt, s, bs, window=4)
 
 
+def test_sinks_without_a_window_are_refused_with_grad_too():
+    q, k, v, bt, s, bs = _decode_args()
+    q.requires_grad_()
+    with pytest.raises(ValueError, match="num_sinks goes with a window"):
+        pa.paged_attention(q, k, v, bt, s, bs, num_sinks=4)
+
+
 def _params(**kw):
     p = _native.DecodeParams()
     p.batch, p.num_heads, p.num_kv_heads, p.head_dim = 2, 8, 2, 128
