@@ -31,6 +31,16 @@ int dtype_code(const at::Tensor& t) {
   return -1;
 }
 
+// Queries whose rows start on 16 bytes, one element apart: the tensor itself or a copy
+// (clone, as contiguous() hands back a tensor whose address, or the stride of a dimension
+// of one, is the trouble).
+at::Tensor aligned_rows(const at::Tensor& q) {
+  if (q.stride(2) == 1 && q.stride(0) % 8 == 0 && q.stride(1) % 8 == 0 &&
+      reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0)
+    return q;
+  return q.clone(at::MemoryFormat::Contiguous);
+}
+
 // Returns (status, tensors): status 0 and [out[, lse][, o_partial, lse_partial]]
 // on success; when the workspace is too small nothing is launched and the
 // result is (-1, []) with the needed sizes in the last two fields.
@@ -65,12 +75,10 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> window_decode(
   check(bt.size(0) == batch, "Block_Table rows != batch");
   check(q.stride(2) == 1 && k.stride(3) == 1 && v.stride(3) == 1 && bt.stride(1) == 1,
         "last dimensions must be contiguous");
-  at::Tensor Q = q;
-  if (q.stride(0) % 8 || q.stride(1) % 8 || reinterpret_cast<uintptr_t>(q.data_ptr()) % 16)
-    Q = q.contiguous();
   const int64_t max_blocks = bt.size(1);
 
   c10::cuda::CUDAGuard guard(dev);
+  const at::Tensor Q = aligned_rows(q);
   at::Tensor lens;
   if (seq_lens.has_value()) {
     lens = *seq_lens;
@@ -218,10 +226,7 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t> prompt(
   check(tokens <= INT32_MAX && batch < INT32_MAX && bt.size(1) <= INT32_MAX, "sizes beyond int32");
 
   c10::cuda::CUDAGuard guard(dev);
-  at::Tensor Q = q;
-  if (q.stride(2) != 1 || q.stride(0) % 8 || q.stride(1) % 8 ||
-      reinterpret_cast<uintptr_t>(q.data_ptr()) % 16)
-    Q = q.contiguous();
+  const at::Tensor Q = aligned_rows(q);
   at::Tensor out = out_opt.has_value() ? *out_opt : at::empty({tokens, heads, dim}, Q.options());
   check(out.device() == dev && out.sizes() == Q.sizes() && out.scalar_type() == Q.scalar_type() &&
             out.stride(2) == 1,

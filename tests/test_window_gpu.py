@@ -291,3 +291,35 @@ def test_scores_of_minus_infinity_weigh_nothing(d, bs, hkv, g, batch, s, window,
         tol = (2 * d * 2.0 ** -24 * big + 2.0 ** -16) * v2.abs().max() + 2.0 ** -11 * want.abs()
         assert_matches(o, want, tol, f"{len(dead)} of {len(seen)} at -infinity")
         assert_lse(lse, torch.logsumexp(sc, -1), d, f"{len(dead)} of {len(seen)} at -infinity")
+
+
+def _misplaced(q):
+    """The same queries [N, H, D] off their 16 bytes, and a single one with an odd stride."""
+    flat = torch.zeros(q.numel() + 1, dtype=q.dtype, device=q.device)
+    flat[1:] = q.reshape(-1)
+    yield flat[1:].view(q.shape), slice(None)
+    odd = torch.zeros(q[0].numel() + 1, dtype=q.dtype, device=q.device)
+    odd[:-1] = q[0].reshape(-1)
+    yield odd.as_strided((1, *q.shape[1:]), (q[0].numel() + 1, q.shape[2], 1)), slice(0, 1)
+
+
+@pytest.mark.parametrize("window,sinks", [(100, 4), (None, 0)])
+@pytest.mark.parametrize("d,bs", [(128, 16), (32, 16), (64, 5)])
+def test_queries_off_their_alignment_are_copied(d, bs, window, sinks):
+    import paged_attention as pa
+    lens = [150, 3, 40]
+    c = PoisonedCache(lens, [1] * 3, 2, d, bs, torch.float16, window or 10 ** 9, sinks, 5)
+    q = torch.randn(3, 6, d, device="cuda").half()
+    want = pa.paged_attention(q, c.k, c.v, c.table, c.lens, bs, window=window, num_sinks=sinks)
+    starts = torch.arange(4, dtype=torch.int32, device="cuda")
+    pwant = pa.paged_prompt_attention(q, c.k, c.v, c.table, starts, c.lens, bs, window=window,
+                                      num_sinks=sinks, num_splits=1)
+    for x, rows in _misplaced(q):
+        n = len(x)
+        got = pa.paged_attention(x, c.k, c.v, c.table[rows], c.lens[rows], bs, window=window, num_sinks=sinks)
+        # (one row alone may be split elsewhere: a rounding of the output apart)
+        assert_matches(got, want[rows].double().cpu(), (0 if n == 3 else 2 * 2.0 ** -11)
+                       * want[rows].double().cpu().abs() + (0 if n == 3 else 1e-5), "decode")
+        got = pa.paged_prompt_attention(x, c.k, c.v, c.table[rows], starts[: n + 1], c.lens[rows], bs,
+                                        window=window, num_sinks=sinks, num_splits=1)
+        assert torch.equal(got, pwant[rows])
