@@ -9,6 +9,7 @@
 // Reference interface: paged_attention(Q, K_Cache, V_Cache, Block_Table,
 // seq_len, block_size, num_splits) (paged_attention/torch_kernel.py:71-73).
 #include <torch/extension.h>
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
@@ -29,6 +30,11 @@ int dtype_code(const at::Tensor& t) {
   TORCH_CHECK_VALUE(false, "paged_attention: unsupported dtype ", t.scalar_type(),
                     " (fp16 or bf16)");
   return -1;
+}
+
+// Forward-mode tangents would be dropped: such inputs are refused, as gradients are.
+bool has_tangent(const at::Tensor& t) {
+  return c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined();
 }
 
 // Queries whose rows start on 16 bytes, one element apart: the tensor itself or a copy
@@ -93,6 +99,8 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> window_decode(
   check(window >= 0 && window <= INT32_MAX && num_sinks >= 0 && num_sinks <= INT32_MAX,
         "window must be at least 1 and num_sinks at least 0");
   check(window > 0 || num_sinks == 0, "num_sinks goes with a window");
+  TORCH_CHECK(window == 0 || !(has_tangent(q) || has_tangent(k) || has_tangent(v)),
+              "PagedAttentionV2 is inference-only.");
   check(window == 0 || (num_splits == 0 && !return_partials),
         "a window goes with the default schedule (no num_splits, no return_partials)");
   int64_t ns = num_splits;
@@ -224,6 +232,8 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t> prompt(
   check(k.stride(3) == 1 && v.stride(3) == 1 && (bt.size(1) <= 1 || bt.stride(1) == 1),
         "last dimensions must be contiguous");
   check(tokens <= INT32_MAX && batch < INT32_MAX && bt.size(1) <= INT32_MAX, "sizes beyond int32");
+  TORCH_CHECK(!(has_tangent(q) || has_tangent(k) || has_tangent(v)),
+              "paged_prompt_attention is inference-only.");
 
   c10::cuda::CUDAGuard guard(dev);
   const at::Tensor Q = aligned_rows(q);

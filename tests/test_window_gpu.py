@@ -323,3 +323,28 @@ def test_queries_off_their_alignment_are_copied(d, bs, window, sinks):
         got = pa.paged_prompt_attention(x, c.k, c.v, c.table[rows], starts[: n + 1], c.lens[rows], bs,
                                         window=window, num_sinks=sinks, num_splits=1)
         assert torch.equal(got, pwant[rows])
+
+
+def test_tangents_are_refused():
+    """Forward-mode derivatives through the windowed calls and prompt attention do not exist."""
+    import paged_attention as pa
+    import torch.autograd.forward_ad as fw
+    c = PoisonedCache([50, 7], [1, 1], 2, 64, 16, torch.float16, 20, 2, 5)
+    q = torch.randn(2, 4, 64, device="cuda").half()
+    starts = torch.arange(3, dtype=torch.int32, device="cuda")
+
+    def calls(q, k, v):
+        return (lambda: pa.paged_attention(q, k, v, c.table, c.lens, 16, window=20, num_sinks=2),
+                lambda: pa.paged_prompt_attention(q, k, v, c.table, starts, c.lens, 16, window=20, num_sinks=2))
+    want = [f() for f in calls(q, c.k, c.v)]
+    with fw.dual_level():
+        for i in range(3):
+            args = [q, c.k, c.v]
+            args[i] = fw.make_dual(args[i], torch.ones_like(args[i]))
+            for f, w in zip(calls(*args), want):
+                with pytest.raises(RuntimeError, match="inference-only"):
+                    f()
+                with torch.inference_mode():          # asks for no derivative
+                    assert torch.equal(f(), w)
+        for f, w in zip(calls(q, c.k, c.v), want):
+            assert torch.equal(f(), w)
