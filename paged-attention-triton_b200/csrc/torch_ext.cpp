@@ -77,7 +77,7 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> window_decode(
         "head_dim must be 32, 64, 128 or 256");
   check(block_size == bs, "block_size differs from the cache's block dimension");
   check(bs >= 1, "block_size must be positive");
-  check(heads % kv_heads == 0, "Hq must be a multiple of Hkv");
+  check(kv_heads > 0 && heads % kv_heads == 0, "Hq must be a multiple of Hkv");
   check(bt.size(0) == batch, "Block_Table rows != batch");
   check(q.stride(2) == 1 && k.stride(3) == 1 && v.stride(3) == 1 && bt.stride(1) == 1,
         "last dimensions must be contiguous");
@@ -113,8 +113,12 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t, int64_t> window_decode(
 
   const auto opts = Q.options();
   at::Tensor out = out_opt.has_value() ? *out_opt : at::empty({batch, heads, dim}, opts);
+  // (pinned host memory is the device's too; a peer's is the caller's to make reachable)
+  check(out.device() == dev || out.is_pinned() || (window == 0 && out.is_cuda()),
+        "out must be on Q's device");
   check(out.sizes() == Q.sizes() && out.scalar_type() == Q.scalar_type() && out.stride(2) == 1,
         "out must match Q's shape and dtype");
+  check(ws_status.device() == dev, "the workspace is on another device");
   const auto f32 = opts.dtype(at::kFloat);
   at::Tensor lse, o_part, lse_part;
   if (return_lse) lse = at::empty({batch, heads}, f32);
@@ -241,6 +245,7 @@ std::tuple<int64_t, std::vector<at::Tensor>, int64_t> prompt(
   check(out.device() == dev && out.sizes() == Q.sizes() && out.scalar_type() == Q.scalar_type() &&
             out.stride(2) == 1,
         "out must match Q's shape, dtype and device");
+  check(ws_status.device() == dev, "the workspace is on another device");
   at::Tensor lse;
   if (return_lse) lse = at::empty({tokens, heads}, Q.options().dtype(at::kFloat));
 

@@ -348,3 +348,38 @@ def test_tangents_are_refused():
                     assert torch.equal(f(), w)
         for f, w in zip(calls(q, c.k, c.v), want):
             assert torch.equal(f(), w)
+
+
+@pytest.mark.parametrize("kw", [{}, dict(window=20, num_sinks=2)])
+def test_out_and_workspace_of_another_device_are_refused(kw):
+    import paged_attention as pa
+    c = PoisonedCache([50, 7], [1, 1], 2, 64, 16, torch.float16, 20 if kw else 10 ** 9, 2 if kw else 0, 5)
+    q = torch.randn(2, 4, 64, device="cuda").half()
+    starts = torch.arange(3, dtype=torch.int32, device="cuda")
+    for bad in (dict(out=torch.empty(2, 4, 64).half()), dict(workspace=pa.DecodeWorkspace("cpu"))):
+        with pytest.raises(ValueError, match="device"):
+            pa.paged_attention(q, c.k, c.v, c.table, c.lens, 16, **kw, **bad)
+        with pytest.raises(ValueError, match="device"):
+            pa.paged_prompt_attention(q, c.k, c.v, c.table, starts, c.lens, 16, **kw, **bad)
+
+
+def test_out_in_pinned_host_memory():
+    import paged_attention as pa
+    c = PoisonedCache([50, 7], [1, 1], 2, 64, 16, torch.float16, 20, 2, 5)
+    q = torch.randn(2, 4, 64, device="cuda").half()
+    want = pa.paged_attention(q, c.k, c.v, c.table, c.lens, 16, window=20, num_sinks=2)
+    out = torch.empty(2, 4, 64).half().pin_memory()
+    pa.paged_attention(q, c.k, c.v, c.table, c.lens, 16, window=20, num_sinks=2, out=out)
+    torch.cuda.synchronize()
+    assert torch.equal(out, want.cpu())
+
+
+def test_caches_without_heads_are_refused():
+    import paged_attention as pa
+    k = torch.empty(4, 16, 0, 64, device="cuda").half()
+    q = torch.zeros(2, 4, 64, device="cuda").half()
+    i = torch.zeros(3, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="multiple of Hkv"):
+        pa.paged_attention(q, k, k, i.view(3, 1)[:2], i[:2], 16, window=4)
+    with pytest.raises(ValueError, match="multiple of Hkv"):
+        pa.paged_prompt_attention(q, k, k, i.view(3, 1)[:2], i, i[:2], 16)
