@@ -146,7 +146,9 @@ PA_API pa_status_t pa_decode(const pa_decode_params* p, cudaStream_t stream);
 /* The same step under a sliding window: the query of a row of S tokens (at
  * position S - 1) sees the row's last `window` tokens and its first `num_sinks`
  * tokens. No other page is read: their block-table entries may be anything
- * (pages given back to the pool hold -1). window >= 1, num_sinks >= 0, else
+ * (pages given back to the pool hold -1). Lengths go up to 2^31 - 65 (a longer one
+ * in seq_lens is cut and flagged, PA_STATUS_BAD_SEQLEN; a longer seq_len is
+ * PA_ERR_UNSUPPORTED); the table may be wider. window >= 1, num_sinks >= 0, else
  * PA_ERR_ARG; the split schedule (num_splits > 0, partial buffers) has no
  * windowed form: PA_ERR_UNSUPPORTED. Workspace and counters as
  * pa_window_decode_workspace reports. It has no counterpart in the reference. */

@@ -94,7 +94,7 @@ struct KParams {
   float* lse;
   const int* bt;
   long long bt_sb;          // elements
-  int max_blocks;
+  int cap;                  // longest length (table_tokens)
   const int* seq_lens;
   int seq_len;              // uniform length (seq_lens == nullptr)
   int B, Hq, Hkv, G, QC, bs, NB;
@@ -337,9 +337,8 @@ __device__ __forceinline__ uint32_t pack16(uint16_t lo, uint16_t hi) {
 // single range is the split's tiles, and its partial is the split's row.
 
 __device__ __forceinline__ int clamp_len(const KParams& p, int s, bool& bad) {
-  const int cap = p.max_blocks * p.bs;
   if (s < 0) { bad = true; return 0; }
-  if (s > cap) { bad = true; return cap; }
+  if (s > p.cap) { bad = true; return p.cap; }
   return s;
 }
 
@@ -2018,7 +2017,7 @@ struct GenParams {
   long long k_sb, k_ss, k_sh, v_sb, v_ss, v_sh;   // bytes
   const int* bt;
   long long bt_sb;                          // elements
-  int max_blocks;
+  int cap;                                  // longest length (table_tokens)
   const int* seq_lens;
   int seq_len;
   int B, Hq, G, bs, NB, ns;
@@ -2085,10 +2084,9 @@ __global__ void __launch_bounds__(128) generic_split_kernel(const GenParams g) {
   const int kvh = hq / g.G;
   int S = g.seq_len;
   if (g.seq_lens) {
-    const long long cap = static_cast<long long>(g.max_blocks) * g.bs;
     const int raw = __ldg(g.seq_lens + b);
-    S = raw < 0 ? 0 : (raw > cap ? static_cast<int>(cap) : raw);
-    if ((raw < 0 || raw > cap) && lane == 0 && s == 0 && hq == 0 && g.status)
+    S = raw < 0 ? 0 : min(raw, g.cap);
+    if ((raw < 0 || raw > g.cap) && lane == 0 && s == 0 && hq == 0 && g.status)
       atomicOr(g.status, PA_STATUS_BAD_SEQLEN);
   }
   int jump_at = 0, jump = 0;                 // visible token v >= jump_at is token v + jump
@@ -2098,9 +2096,9 @@ __global__ void __launch_bounds__(128) generic_split_kernel(const GenParams g) {
     jump = w.w0 - w.a;
     S -= jump;
   }
-  const int ss = (S + g.ns - 1) / g.ns;      // torch_kernel.py:30
-  const int t0 = s * ss;
-  const int t1 = min(t0 + ss, S);
+  const int ss = S > 0 ? (S - 1) / g.ns + 1 : 0;   // torch_kernel.py:30
+  const int t0 = static_cast<int>(min(static_cast<long long>(s) * ss, static_cast<long long>(S)));
+  const int t1 = t0 + min(ss, S - t0);
   float* op = g.o_part + w * D;
   if (t0 >= t1) {                            // split_kv_kernel.py:32-33: the sentinel stays
     for (int d = lane; d < D; d += 32) op[d] = 0.f;
@@ -2389,6 +2387,14 @@ static int variant_smem_base(int variant, bool dup, int D) {
     case 10: return dup ? smem_base<true, 32, 4, 2, 128>() : smem_base<false, 32, 4, 2, 128>();
     default: return dup ? smem_base<true, 32, 4, 3, 128>() : smem_base<false, 32, 4, 3, 128>();
   }
+}
+
+// Tokens a row's table holds, as the longest length of a row: lengths up to a tile below
+// 2^31 (positions rounded up to a tile's end stay in int32).
+constexpr int kMaxTokens = 0x7fffffff - 64;
+static int table_tokens(const pa_decode_params* p) {
+  return static_cast<int>(std::min<long long>(
+      static_cast<long long>(p->max_blocks) * p->block_size, kMaxTokens));
 }
 
 static pa_status_t validate(const pa_decode_params* p) {
@@ -2950,7 +2956,7 @@ static cudaError_t launch_generic(const pa_decode_params* p, const Plan& pl, int
   g.v_sh = p->v_stride_head * 2;
   g.bt = p->block_table;
   g.bt_sb = p->bt_stride_b;
-  g.max_blocks = p->max_blocks;
+  g.cap = table_tokens(p);
   g.seq_lens = p->seq_lens;
   g.seq_len = p->seq_lens ? 0 : p->seq_len;
   g.B = p->batch;
@@ -3016,7 +3022,7 @@ static void build_kparams(const pa_decode_params* p, const Plan& pl, KParams& kp
   kp.lse = p->lse;
   kp.bt = p->block_table;
   kp.bt_sb = p->bt_stride_b;
-  kp.max_blocks = p->max_blocks;
+  kp.cap = table_tokens(p);
   kp.seq_lens = p->seq_lens;
   kp.seq_len = p->seq_lens ? 0 : p->seq_len;
   kp.B = p->batch;
@@ -3248,7 +3254,7 @@ static pa_status_t run_decode(const pa_decode_params* p, const pa_decode_params*
   const int tile = kVariants[pl.variant - 1].tile;
   build_kparams(q, pl, kp);
   if (window) {
-    kp.max_blocks = p->max_blocks;
+    kp.cap = table_tokens(p);
     kp.seq_len = p->seq_lens ? 0 : p->seq_len;
     kp.zero_rows = 1;
     kp.window = window;
@@ -3304,7 +3310,7 @@ static pa_status_t run_decode(const pa_decode_params* p, const pa_decode_params*
     m.o_sh = kp.o_sh;
     m.lse = kp.lse;
     m.seq_lens = kp.seq_lens;
-    m.cap = kp.max_blocks * kp.bs;
+    m.cap = kp.cap;
     m.B = kp.B;
     m.Hkv = kp.Hkv;
     m.G = kp.G;
@@ -3332,6 +3338,7 @@ static pa_status_t run_decode(const pa_decode_params* p, const pa_decode_params*
 static pa_status_t validate_window(const pa_decode_params* p, int32_t window, int32_t num_sinks) {
   if (!p || window <= 0 || num_sinks < 0) return PA_ERR_ARG;
   if (p->num_splits != 0 || p->o_partial || p->lse_partial) return PA_ERR_UNSUPPORTED;
+  if (!p->seq_lens && p->seq_len > kMaxTokens) return PA_ERR_UNSUPPORTED;
   return PA_OK;
 }
 

@@ -67,6 +67,14 @@ def test_window_c_abi_refusals(kw, window, sinks, code):
     assert lib.pa_window_decode(ctypes.byref(p), window, sinks, None) == code
 
 
+def test_window_c_abi_lengths_that_reach_int32s_end_are_refused():
+    lib = _native.lib()
+    p = _params(block_size=1024, max_blocks=2 ** 21, seq_len=2 ** 31 - 64)
+    assert lib.pa_window_decode(ctypes.byref(p), 100, 4, None) == _native.PA_ERR_UNSUPPORTED
+    p.seq_len = 2 ** 31 - 65                               # not refused for that
+    assert lib.pa_window_decode(ctypes.byref(p), 100, 4, None) == _native.PA_ERR_ARG
+
+
 def test_window_c_abi_null():
     lib = _native.lib()
     assert lib.pa_window_decode(None, 4, 0, None) == _native.PA_ERR_ARG

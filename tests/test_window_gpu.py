@@ -383,3 +383,36 @@ def test_caches_without_heads_are_refused():
         pa.paged_attention(q, k, k, i.view(3, 1)[:2], i[:2], 16, window=4)
     with pytest.raises(ValueError, match="multiple of Hkv"):
         pa.paged_prompt_attention(q, k, k, i.view(3, 1)[:2], i, i[:2], 16)
+
+
+@pytest.mark.parametrize("hkv,g,d", [(1, 4, 64), (2, 1, 128), (1, 8, 256), (1, 3, 32)])
+@pytest.mark.parametrize("lens,window,sinks", [([5, 700, 0, 1024], 100, 4),
+                                               ([2 ** 31 - 65, 2 ** 30 + 3, 1], 130, 3)])
+def test_window_decode_over_a_table_of_two_to_the_31_tokens(hkv, g, d, lens, window, sinks):
+    """Tables wider than int32 counts tokens, nearly all of it pages that are not there; rows
+    at both ends of them."""
+    import paged_attention as pa
+    from paged_attention import _native
+    bs, width = 1024, 2 ** 21
+    c = PoisonedCache(lens, [1] * len(lens), hkv, d, bs, torch.bfloat16, window, sinks, d, width=width)
+    q = torch.randn(len(lens), hkv * g, d, device="cuda").bfloat16()
+    ws = pa.DecodeWorkspace("cuda")
+
+    def run(n, batch):
+        return pa.paged_attention(q[:batch], c.k, c.v, c.table[:batch], n, bs, window=window, num_sinks=sinks,
+                                  return_lse=True, workspace=ws)
+    want, wl, tol = reference(q, c.k, c.v, c.table, lens, bs, window, sinks)
+    o, lse = run(c.lens, len(lens))
+    assert ws.read_status() == 0
+    assert_matches(o, want, tol, f"{lens}")
+    assert_lse(lse, wl, d, f"{lens}")
+    o, lse = run(lens[0], 1)
+    assert_matches(o, want[:1], tol[:1], f"{lens[0]}")
+    assert_lse(lse, wl[:1], d, f"{lens[0]}")
+    assert ws.read_status() == 0
+    c.lens[1] = 2 ** 31 - 1                    # longer than a length can be: cut and flagged
+    c.table[1, -1] = c.table[0, 0] if lens[0] < bs else c.table[0, -1]
+    o, lse = run(c.lens, len(lens))
+    assert ws.read_status() & _native.PA_STATUS_BAD_SEQLEN
+    keep = [0] + list(range(2, len(lens)))
+    assert_matches(o[keep], want[keep], tol[keep], "the other rows")
