@@ -476,3 +476,66 @@ def test_prompt_pool_of_one_token():
                                       torch.zeros(1, 1, dtype=torch.int32, device="cuda"), st,
                                       st[1:], 1)
         assert torch.equal(o, v[0, 0].expand(1, 2, d))
+
+
+@pytest.mark.parametrize("splits", [1, 2, 5])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d", [32, 64, 128, 256])
+def test_prompt_lse_of_large_scores(d, dtype, splits):
+    """Scores in the hundreds under a maximum that keeps growing: the LSE, whose sum is kept
+    against an older maximum, alone and joined from parts with LSEs far apart.
+
+    Tolerance: each score's rounding in 32 bits, 2^-24 D sum|q_i k_i| scale; the scaled maximum,
+    its difference to a score and the parts' LSEs, each rounded a few times (8 * 2^-24 of the
+    largest score or LSE); exponentials and the sum of 1024, 1e-5 relative at most."""
+    import paged_attention as pa
+    n, s, bs = 64, 1024, 16
+    c = PoisonedCache([s], [n], 1, d, bs, dtype, 10 ** 9, 0, 5)
+    ramp = torch.arange(s, device="cuda") / 64.0
+    page, slot = c.table[0, torch.arange(s) // bs].long(), torch.arange(s, device="cuda") % bs
+    c.k[page, slot] = (c.k[page, slot].float() * ramp[:, None, None]).to(dtype)
+    q = torch.randn(n, 4, d, device="cuda", generator=torch.Generator(device="cuda").manual_seed(d)).to(dtype)
+    st = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    o, lse = pa.paged_prompt_attention(q, c.k, c.v, c.table, st, c.lens, bs, scale=0.5, return_lse=True,
+                                       num_splits=splits)
+    want, wl, tol = reference(q, c.k, c.v, c.table, [s], bs, 10 ** 9, 0, [0, n], scale=0.5)
+    vmax = c.v[~c.v.isnan()].abs().max().double().item()
+    assert_matches(o, want, _tolerance(q, tol, vmax), "O")
+    big = (q.double().abs().cpu() @ c.k[page, slot, 0].double().abs().cpu().T * 0.5).amax(-1)
+    bound = d * 2.0 ** -24 * big + 8 * 2.0 ** -24 * torch.maximum(wl.abs(), big) + 1e-5
+    assert not ((lse.double().cpu() - wl).abs() > bound).any(), (lse.double().cpu() - wl).abs().max()
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("g", [1, 4])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("fma_columns", [True, False])
+def test_prompt_exponentials(d, g, dtype, fma_columns):
+    """The sum of exponentials by itself: queries of a single one and keys of the scores wanted,
+    so that the scores are exact. They sit in the columns (of each eight, two) whose exponentials
+    are a polynomial on the FMA pipe, or in the others; token 0 holds the maximum, 0.
+
+    Tolerance of the LSE = log(1 + sum of the others), all relative errors of a sum of positive
+    terms: the polynomial's 2.9e-6 or ex2's 2^-22; the argument, rounded from |x| up to 20,
+    3 * 2^-24 |x| e^x <= 3 * 2^-24; 32 additions a lane, 3 across them and one per tile of 512
+    tokens at most; the result's own 4 * 2^-24 (1 + |LSE|)."""
+    import paged_attention as pa
+    s, bs = 512, 16
+    n = s + d
+    gen = torch.Generator().manual_seed(d + g)
+    x = torch.full((n, d), -100.0)
+    cols = torch.tensor([t for t in range(1, s) if ((t & 6) == 4) == fma_columns])
+    x[cols] = -20 * torch.rand(len(cols), d, generator=gen) ** 2
+    x[0] = 0
+    x = x.to(dtype)
+    k = x.view(n // bs, bs, 1, d).cuda()
+    q = torch.eye(d).to(dtype).cuda()[:, None].expand(d, g, d)
+    table = torch.arange(n // bs, dtype=torch.int32, device="cuda")[None]
+    st = torch.tensor([0, d], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+    _, lse = pa.paged_prompt_attention(q, k, k, table, st, lens, bs, scale=1.0, return_lse=True, num_splits=1)
+    want = torch.logsumexp(x.double()[: s + 1], 0)[:, None]      # (the rest weighs e^-100)
+    ulp = 2.0 ** -24
+    tol = (2.9e-6 if fma_columns else 2.0 ** -22) + 3 * ulp + (32 + 3 + 9) * ulp + 4 * ulp * (1 + want.abs())
+    err = (lse.double().cpu() - want).abs()
+    assert not (err > tol).any(), f"off by {err.max().item():.2e}, allowed {tol.min().item():.2e}"
