@@ -36,7 +36,7 @@ from __future__ import annotations
 import ctypes
 import math
 import threading
-from typing import Dict, Optional, Tuple, Union
+from typing import Dict, List, Optional, Tuple, Union
 
 import torch
 
@@ -58,7 +58,9 @@ class DecodeWorkspace:
     * ``status``: a device word the kernel ORs ``PA_STATUS_*`` bits into.
 
     Growing reallocates, so a CUDA-graph caller sizes it before capture (the
-    graph runner does this in its warm-up).
+    graph runner does this in its warm-up). Earlier buffers stay allocated, as a
+    captured graph may hold their addresses (sizes at least double, so together
+    they are no larger than the newest).
     """
 
     def __init__(self, device: Union[torch.device, str, int]):
@@ -68,12 +70,15 @@ class DecodeWorkspace:
         self.buffer = torch.empty(0, dtype=torch.uint8, device=self.device)
         self.counters = torch.zeros(0, dtype=torch.int32, device=self.device)
         self.status = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._earlier: List[torch.Tensor] = []
 
     def ensure(self, nbytes: int, ncounters: int) -> None:
         if nbytes > self.buffer.numel():
+            self._earlier.append(self.buffer)
             self.buffer = torch.empty(max(nbytes, 2 * self.buffer.numel()), dtype=torch.uint8,
                                       device=self.device)
         if ncounters > self.counters.numel():
+            self._earlier.append(self.counters)
             self.counters = torch.zeros(max(ncounters, 2 * self.counters.numel()),
                                         dtype=torch.int32, device=self.device)
 

@@ -539,3 +539,34 @@ def test_prompt_exponentials(d, g, dtype, fma_columns):
     tol = (2.9e-6 if fma_columns else 2.0 ** -22) + 3 * ulp + (32 + 3 + 9) * ulp + 4 * ulp * (1 + want.abs())
     err = (lse.double().cpu() - want).abs()
     assert not (err > tol).any(), f"off by {err.max().item():.2e}, allowed {tol.min().item():.2e}"
+
+
+def test_prompt_captured_graph_outlives_a_growing_workspace():
+    """A call that grows the workspace leaves a graph captured before it with its own scratch;
+    what is allocated in between is not written by the replay."""
+    import paged_attention as pa
+    qs, lens, window, sinks = [5, 3], [900, 700], 600, 4
+    c = PoisonedCache(lens, qs, 2, 128, 16, torch.float16, window, sinks, 3)
+    q = torch.randn(8, 8, 128, device="cuda").half()
+    st = torch.tensor(_starts(qs), dtype=torch.int32, device="cuda")
+    ws = pa.DecodeWorkspace("cuda")
+    out = torch.zeros_like(q)
+
+    def call(splits):
+        pa.paged_prompt_attention(q, c.k, c.v, c.table, st, c.lens, 16, window=window, num_sinks=sinks,
+                                  workspace=ws, out=out, num_splits=splits)
+    call(3)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(3)
+    graph.replay()
+    want = out.clone()
+    size = ws.buffer.numel()
+    call(40)
+    assert ws.buffer.numel() > size
+    others = [torch.full((size,), 7, dtype=torch.uint8, device="cuda") for _ in range(8)]
+    out.zero_()
+    graph.replay()
+    assert torch.equal(out, want)
+    assert all((x == 7).all() for x in others)

@@ -81,6 +81,18 @@ def test_window_c_abi_null():
     assert lib.pa_window_decode(ctypes.byref(_params()), 4, 0, None) == _native.PA_ERR_ARG
 
 
+def test_workspace_keeps_what_a_captured_graph_may_hold():
+    import weakref
+    ws = pa.DecodeWorkspace("cpu")
+    ws.ensure(100, 10)
+    held = [weakref.ref(ws.buffer), weakref.ref(ws.counters)]
+    ws.ensure(1000, 100)
+    ws.ensure(5000, 100)
+    assert all(x() is not None for x in held)
+    assert ws.buffer.numel() == 5000 and ws.counters.numel() == 100
+    assert sum(x.numel() * x.element_size() for x in ws._earlier) <= 5000 + 400
+
+
 def _prompt_args():
     q = torch.randn(3, 2, 128, dtype=torch.float16)
     k = torch.randn(2, 16, 2, 128, dtype=torch.float16)
