@@ -1019,8 +1019,10 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
     const int t = warp >> 2;
     const int tid = threadIdx.x & 127;
     const int r0 = j.r0 + t * 128;
-    {
-      // the row tile into shared memory: 16-byte pieces, D/8 threads a row
+    if (j.k0 < j.k1) {
+      // the row tile into shared memory: 16-byte pieces, D/8 threads a row. (Not for rows
+      // that see nothing: no product would wait for these copies, and the output takes
+      // their place.)
       constexpr int kPer = D / 8;
       const int c = tid % kPer;
 #pragma unroll
@@ -1170,10 +1172,8 @@ __global__ void __launch_bounds__(TC<D, NQ>::kThreads, TC<D, NQ>::kCtas)
       f2_split(sum[1], x2, x3);
       l += (x0 + x1) + (x2 + x3);
     }
-    if (ok) {
-      // No tile: no product has waited for the staged queries, whose place the output
-      // takes below, so their last copies are waited for here.
-      ok = n > 0 ? mbar_wait(o_done(t), C::kSBufs == 2 ? (n - 1) & 1 : 0) : mbar_wait(q_full(t), 0);
+    if (n > 0 && ok) {
+      ok = mbar_wait(o_done(t), C::kSBufs == 2 ? (n - 1) & 1 : 0);
       ok = __all_sync(kFull, ok);
       tc_fence_after();
     }
