@@ -164,7 +164,8 @@ PA_API pa_status_t pa_window_decode(const pa_decode_params* p, int32_t window, i
  * of n sits at position seq_lens[b] - n + i and sees token t when t <= position
  * and, with a window, t < num_sinks or t > position - window. Rows that see
  * nothing (positions before 0) get O = 0 and LSE = -1e30; rows outside every
- * sequence are not written. Pages with no visible token are not read; their
+ * sequence are not written. Tables of more than 2^31 - 256 tokens, and more than
+ * 2^30 - 1 (token, head) rows, are PA_ERR_UNSUPPORTED. Pages with no visible token are not read; their
  * table entries may be anything. Slots of visible pages behind the sequence's
  * end may hold anything too; a NaN or infinity inside the sequence may reach
  * the rows of the same chunk that do not see it. query_starts has to ascend within

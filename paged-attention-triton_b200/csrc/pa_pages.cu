@@ -65,7 +65,7 @@ struct Pool {
   // carve-up of the scratch
   __host__ __device__ int* copies() const { return scratch + kHeader; }          // [3 * NB]
   __host__ __device__ int* list() const { return copies() + 3 * static_cast<size_t>(NB); }  // [NB]
-  __host__ __device__ int* plan() const { return list() + NB; }                  // [rows or 2 * pairs]
+  __host__ __device__ int* plan() const { return list() + NB; }                  // [2 * pairs] (fork)
 };
 
 struct Table {

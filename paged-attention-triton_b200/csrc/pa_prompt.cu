@@ -130,8 +130,10 @@ __device__ __forceinline__ int seq_of_row(const Params& p, int row) {
 // head_dim 256) S has two buffers and the next tile's S is computed during the
 // current softmax.
 //
-// What bounds it (8192 tokens, Hq32/Hkv8, D 128, window 4096 / none: 363 / 458 us,
-// 1.13 / 1.20 PFLOP/s): the chain from a tile's S to its P. 256 rows x 128 keys
+// What bounds it (8192 tokens, Hq32/Hkv8, D 128, window 4096 / none: 368 / 466 us,
+// 1.12 / 1.18 PFLOP/s, in runs of 100 calls; 410 / 525 us, 1.0 / 1.05 PFLOP/s, once
+// calls follow each other for 0.4 s and the power cap lowers the clock; comparisons
+// here and below are of short runs): the chain from a tile's S to its P. 256 rows x 128 keys
 // take the matrix pipe 2048 cycles, the special function units as many, and the
 // tile's turn ~3000: load of S 250, maximum 300-400, exponentials 1400 (1024 if no
 // other warp ran), then the rest of P V and the next S 1000. Tried and slower:
@@ -144,8 +146,12 @@ __device__ __forceinline__ int seq_of_row(const Params& p, int row) {
 // the hardware's order of CTAs balances better than any fixed one).
 //
 // P is rounded to the operand type once (half a step, relative); its sum, the
-// maxima and O are kept in 32 bits. O is rescaled only when a row's maximum has
-// grown by more than 2^8: until then P and the sum are relative to an older
+// maxima and O are kept in 32 bits. The roundings of P are independent of the one of
+// the output and for values of random sign add up to as much: the error against 64
+// bits is up to sqrt(2) times that of rounding the exact result (measured 1.25-1.4),
+// and in each element at most half a step of the largest value more. Keeping P as a
+// pair of 16-bit parts, as decode does, would make P V two products (half as much
+// again on the matrix pipe). O is rescaled only when a row's maximum has grown by more than 2^8: until then P and the sum are relative to an older
 // maximum, which changes neither's relative rounding (P <= 2^8).
 //
 // Masks: a tile that is not entirely visible to all rows of a warp compares

@@ -32,7 +32,12 @@ def paged_prompt_attention(Q: torch.Tensor, K_Cache: torch.Tensor, V_Cache: torc
     counting them in. The row at position p sees token t when ``t <= p`` and, with a
     ``window``, ``t < num_sinks or t > p - window``. Pages with no visible token are not
     read (entry -1 will do). Rows that see nothing get 0 and LSE -1e30; rows outside
-    every sequence (padding) are left as they were in ``out``.
+    every sequence (padding) are left as they were in ``out``, their LSE is not set.
+    Scores of NaN or +infinity make their row and its LSE NaN.
+
+    Probabilities are rounded once to Q's type before the product with V (sums, maxima
+    and outputs are held in 32 bits), where ``paged_attention`` keeps twice as many bits
+    of them: one token through either differs by a rounding.
 
     ``return_lse=True`` adds ``LSE [T, Hq]`` (fp32, natural log). ``num_splits``: parts of
     the keys that separate CTAs take and a second kernel joins (default: chosen by the
