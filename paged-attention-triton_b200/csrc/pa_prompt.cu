@@ -1488,7 +1488,9 @@ static Plan make_plan(const pa_prompt_params* p, int sms) {
   // bring no more than one tile each would leave the second empty.
   pl.nq = p->head_dim == 256 || p->head_dim <= 64 || packed <= 128ll * p->batch ? 1 : 2;
   const long long slots = static_cast<long long>(sms) * (p->head_dim <= 64 ? 2 : 1);   // CTAs at once
-  // sum over the sequences of ceil(rows / tile), whatever their shares are
+  // Sum over the sequences of ceil(rows / tile), whatever their shares are: a bound, one
+  // too many for each whose rows are whole tiles (one chunk of 32 tokens at G = 4 gets 9
+  // parts of its keys where 18 would fill the SMs).
   pl.tiles = packed / (128 * pl.nq) + std::min<long long>(p->batch, p->num_tokens);
   const long long ctas = pl.tiles * p->num_kv_heads;
   if (p->num_splits > 0) {
